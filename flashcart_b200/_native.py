@@ -30,6 +30,8 @@ FC_F64 = 1
 FC_BF16 = 2
 FC_ACT_NONE = 0
 FC_ACT_SILU = 1
+FC_GATE_SILU = 0
+FC_GATE_SIGMOID = 1
 FC_PREC_IEEE = 0
 FC_PREC_TF32 = 1
 FC_MAX_L = 3
@@ -45,6 +47,8 @@ EXPORTED_SYMBOLS = (
     "fc_linear_fwd_residual", "fc_linear_bwd_residual", "fc_tp_bwd_residual",
     "fc_linear_dbwd", "fc_halo_pack", "fc_halo_unpack", "fc_edge_geometry_fwd", "fc_edge_geometry_bwd",
     "fc_edge_geometry_vec_fwd", "fc_edge_geometry_vec_bwd",
+    "fc_embedding_fwd", "fc_embedding_bwd_workspace_bytes", "fc_embedding_bwd", "fc_irreps_dropout",
+    "fc_gated_ff_workspace_bytes", "fc_gated_ff_fwd", "fc_gated_ff_bwd",
 )
 
 
@@ -77,6 +81,10 @@ class NlDesc(ctypes.Structure):
     _fields_ = [("lengths", ctypes.c_double * 3), ("inv_lengths", ctypes.c_double * 3),
                 ("bin_widths", ctypes.c_double * 3), ("r_max_sq", ctypes.c_double),
                 ("bins", ctypes.c_int32 * 3), ("reserved", ctypes.c_int32)]
+
+
+class GatedFfDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("l_max", "in_features", "hidden_features", "act", "dtype")]
 
 
 class NativeError(RuntimeError):
@@ -165,6 +173,22 @@ def bind(path: str) -> ctypes.CDLL:
     lib.fc_edge_geometry_vec_fwd.argtypes = [ctypes.POINTER(EdgeGeometryDesc), _P, _I64, _P, _P, _P, _P]
     lib.fc_edge_geometry_vec_bwd.restype = ctypes.c_int
     lib.fc_edge_geometry_vec_bwd.argtypes = [ctypes.POINTER(EdgeGeometryDesc), _P, _I64, _P, _P, _P, _P, _P]
+    _F64 = ctypes.c_double
+    lib.fc_embedding_fwd.restype = ctypes.c_int
+    lib.fc_embedding_fwd.argtypes = [_P, _I64, _I64, _I32, _P, _I64, _F64, _F64, _P, _P, _P]
+    lib.fc_embedding_bwd_workspace_bytes.restype = ctypes.c_int64
+    lib.fc_embedding_bwd_workspace_bytes.argtypes = [_I64, _I64, _I64, _I32]
+    lib.fc_embedding_bwd.restype = ctypes.c_int
+    lib.fc_embedding_bwd.argtypes = [_P, _P, _I64, _I64, _I64, _I32, _F64, _P, _P, _P, _P]
+    lib.fc_irreps_dropout.restype = ctypes.c_int
+    lib.fc_irreps_dropout.argtypes = [_I32, _I32, _I32, _P, _P, _F64, _I64, _P, _P]
+    lib.fc_gated_ff_workspace_bytes.restype = ctypes.c_int64
+    lib.fc_gated_ff_workspace_bytes.argtypes = [ctypes.POINTER(GatedFfDesc), _I64, _I32]
+    lib.fc_gated_ff_fwd.restype = ctypes.c_int
+    lib.fc_gated_ff_fwd.argtypes = [ctypes.POINTER(GatedFfDesc), _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P]
+    lib.fc_gated_ff_bwd.restype = ctypes.c_int
+    lib.fc_gated_ff_bwd.argtypes = [ctypes.POINTER(GatedFfDesc), _P, _P, _P, _P, _P, _P, _I64, _P, _P, _P, _P, _P, _P,
+                                    _P]
     lib.fc_gate_fwd.restype = ctypes.c_int
     lib.fc_gate_fwd.argtypes = [_I32, _I32, _I32, _P, _P, _I64, _P, _P]
     lib.fc_gate_bwd.restype = ctypes.c_int

@@ -9,6 +9,7 @@
 
 #include "tp_common.cuh"
 #include "linear.cuh"
+#include "gated_ff.cuh"
 #include "gen/tp_dispatch.inc"
 
 #ifndef FC_VERSION_STRING
@@ -56,6 +57,14 @@ template <typename T>
 int add_rows_dispatch(T*, const T*, int64_t, cudaStream_t);
 template <typename T>
 int gate_bwd_dispatch(int, const T*, const T*, const T*, T*, T*, int, int64_t, cudaStream_t);
+
+template <typename T>
+int embed_fwd(const void*, int64_t, int64_t, const int64_t*, int64_t, double, double, void*, int*, cudaStream_t);
+template <typename T>
+int embed_bwd(const void*, const int64_t*, int64_t, int64_t, int64_t, double, void*, void*, int*, cudaStream_t);
+int64_t embed_bwd_workspace(int64_t R, int64_t V, int64_t D, int dtype);
+template <typename T>
+int irreps_dropout(int, int, const void*, const int64_t*, double, int64_t, void*, cudaStream_t);
 
 static thread_local std::string g_last_error;
 
@@ -869,6 +878,158 @@ int fc_halo_unpack(const void* buf, int64_t n_idx, int64_t row_elems, int32_t dt
   return launch_status(halo_unpack_dispatch<double>((const double*)buf, row_elems, idx, n_idx, (double*)x, n_rows,
                                                     accumulate, st, s),
                        "fc_halo_unpack");
+}
+
+// ------------------------------------------------------------------ training blocks
+
+static int block_dtype_check(int32_t dtype, const char* what) {
+  if (dtype == FC_F32 || dtype == FC_F64 || dtype == FC_BF16) return FC_OK;
+  return fail(FC_ERR_INVALID, "%s: dtype must be f32, f64 or bf16", what);
+}
+
+int fc_embedding_fwd(const void* table, int64_t n_types, int64_t features, int32_t dtype, const int64_t* idx,
+                     int64_t n_rows, double scale, double offset, void* out, int32_t* status, fc_stream_t stream) {
+  const char* what = "fc_embedding_fwd";
+  if (int rc = block_dtype_check(dtype, what)) return rc;
+  if (n_types < 0 || features < 0 || n_rows < 0) return fail(FC_ERR_INVALID, "%s: negative size", what);
+  if (n_rows == 0 || features == 0) return FC_OK;
+  if (!idx || !out || (n_types > 0 && !table)) return fail(FC_ERR_INVALID, "%s: null tensor", what);
+  const cudaStream_t s = (cudaStream_t)stream;
+  int* st = reinterpret_cast<int*>(status);
+  const auto run = dtype == FC_F32 ? embed_fwd<float> : dtype == FC_F64 ? embed_fwd<double> : embed_fwd<bf16_t>;
+  return launch_status(run(table, n_types, features, idx, n_rows, scale, offset, out, st, s), what);
+}
+
+static int embed_bwd_check(int64_t n_rows, int64_t n_types, int64_t features, int32_t dtype, const char* what) {
+  if (int rc = block_dtype_check(dtype, what)) return rc;
+  if (n_types < 0 || features < 0 || n_rows < 0) return fail(FC_ERR_INVALID, "%s: negative size", what);
+  const int64_t most = (int64_t(1) << 31) - 4096;
+  if (n_rows > most || n_types > most || features > (int64_t(1) << 22))
+    return fail(FC_ERR_CAPACITY, "%s: at most %lld rows, %lld types and %lld features", what, (long long)most,
+                (long long)most, (long long)(int64_t(1) << 22));
+  return FC_OK;
+}
+
+int64_t fc_embedding_bwd_workspace_bytes(int64_t n_rows, int64_t n_types, int64_t features, int32_t dtype) {
+  if (int rc = embed_bwd_check(n_rows, n_types, features, dtype, "fc_embedding_bwd_workspace_bytes")) return rc;
+  if (n_types == 0 || features == 0) return 0;
+  return embed_bwd_workspace(n_rows, n_types, features, dtype);
+}
+
+int fc_embedding_bwd(const void* grad_out, const int64_t* idx, int64_t n_rows, int64_t n_types, int64_t features,
+                     int32_t dtype, double scale, void* workspace, void* grad_table, int32_t* status,
+                     fc_stream_t stream) {
+  const char* what = "fc_embedding_bwd";
+  if (int rc = embed_bwd_check(n_rows, n_types, features, dtype, what)) return rc;
+  if (n_types == 0 || features == 0) return FC_OK;
+  if (!grad_table || !workspace || (n_rows > 0 && (!grad_out || !idx)))
+    return fail(FC_ERR_INVALID, "%s: null tensor", what);
+  if (reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(FC_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
+  const cudaStream_t s = (cudaStream_t)stream;
+  int* st = reinterpret_cast<int*>(status);
+  const auto run = dtype == FC_F32 ? embed_bwd<float> : dtype == FC_F64 ? embed_bwd<double> : embed_bwd<bf16_t>;
+  return launch_status(run(grad_out, idx, n_rows, n_types, features, scale, workspace, grad_table, st, s), what);
+}
+
+int fc_irreps_dropout(int32_t l_max, int32_t features, int32_t dtype, const void* x, const int64_t* rng, double p,
+                      int64_t n_rows, void* y, fc_stream_t stream) {
+  const char* what = "fc_irreps_dropout";
+  if (l_max < 0 || l_max > FC_MAX_L)
+    return fail(FC_ERR_UNSUPPORTED, "%s: l_max %d outside [0, %d]", what, l_max, FC_MAX_L);
+  if (int rc = block_dtype_check(dtype, what)) return rc;
+  if (features < 0 || n_rows < 0) return fail(FC_ERR_INVALID, "%s: negative size", what);
+  if (!(p >= 0.0 && p <= 1.0)) return fail(FC_ERR_INVALID, "%s: p must lie in [0, 1], got %g", what, p);
+  if (n_rows == 0 || features == 0) return FC_OK;
+  if (!x || !y || !rng) return fail(FC_ERR_INVALID, "%s: null tensor", what);
+  const cudaStream_t s = (cudaStream_t)stream;
+  const auto run = dtype == FC_F32 ? irreps_dropout<float>
+                   : dtype == FC_F64 ? irreps_dropout<double>
+                                     : irreps_dropout<bf16_t>;
+  return launch_status(run(l_max, features, x, rng, p, n_rows, y, s), what);
+}
+
+static int gated_check(const fc_gated_ff_desc* d, int64_t n_rows, const char* what) {
+  if (!d) return fail(FC_ERR_INVALID, "%s: null descriptor", what);
+  if (d->l_max < 0 || d->l_max > FC_MAX_L)
+    return fail(FC_ERR_UNSUPPORTED, "%s: l_max %d outside [0, %d]", what, d->l_max, FC_MAX_L);
+  if (int rc = block_dtype_check(d->dtype, what)) return rc;
+  if (d->act != FC_GATE_SILU && d->act != FC_GATE_SIGMOID)
+    return fail(FC_ERR_INVALID, "%s: unknown gate activation %d", what, d->act);
+  if (d->in_features <= 0 || d->hidden_features <= 0 || n_rows < 0)
+    return fail(FC_ERR_INVALID, "%s: features must be positive and n_rows not negative", what);
+  if (d->in_features > (1 << 20) || d->hidden_features > (1 << 20) || n_rows > ((int64_t(1) << 31) - 1) / 8)
+    return fail(FC_ERR_CAPACITY, "%s: at most 2^20 features and 2^28 rows", what);
+  return FC_OK;
+}
+
+int64_t fc_gated_ff_workspace_bytes(const fc_gated_ff_desc* desc, int64_t n_rows, int32_t backward) {
+  if (int rc = gated_check(desc, n_rows, "fc_gated_ff_workspace_bytes")) return rc;
+  return gated_simple_ws(desc->l_max, desc->in_features, desc->hidden_features, n_rows, desc->dtype, backward);
+}
+
+static int gated_args(const fc_gated_ff_desc* d, const void* x, const void* const* value_weights,
+                      const void* gate_weight, const void* gate_bias, const void* scales, int64_t n_rows,
+                      void* workspace, int32_t* status, const char* what, GatedArgs& a) {
+  if (int rc = gated_check(d, n_rows, what)) return rc;
+  if (!value_weights || !gate_weight || !scales || (n_rows > 0 && (!x || !workspace)))
+    return fail(FC_ERR_INVALID, "%s: null tensor", what);
+  if (reinterpret_cast<uintptr_t>(workspace) & 15)
+    return fail(FC_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
+  a = GatedArgs{};
+  a.L = d->l_max;
+  a.C = d->in_features;
+  a.H = d->hidden_features;
+  a.act = d->act;
+  a.n = n_rows;
+  a.x = x;
+  for (int l = 0; l <= d->l_max; ++l) {
+    if (!value_weights[l]) return fail(FC_ERR_INVALID, "%s: null weight for rank %d", what, l);
+    a.wv[l] = value_weights[l];
+  }
+  a.wg = gate_weight;
+  a.bias = gate_bias;
+  a.scales = scales;
+  a.ws = workspace;
+  a.status = reinterpret_cast<int*>(status);
+  return FC_OK;
+}
+
+int fc_gated_ff_fwd(const fc_gated_ff_desc* desc, const void* x, const void* const* value_weights,
+                    const void* gate_weight, const void* gate_bias, const void* scales, int64_t n_rows,
+                    void* workspace, void* y, int32_t* status, fc_stream_t stream) {
+  const char* what = "fc_gated_ff_fwd";
+  GatedArgs a;
+  if (int rc = gated_args(desc, x, value_weights, gate_weight, gate_bias, scales, n_rows, workspace, status, what, a))
+    return rc;
+  if (n_rows == 0) return FC_OK;
+  if (!y) return fail(FC_ERR_INVALID, "%s: null tensor", what);
+  a.y = y;
+  const auto run = desc->dtype == FC_F32 ? gated_simple_fwd<float>
+                   : desc->dtype == FC_F64 ? gated_simple_fwd<double>
+                                           : gated_simple_fwd<bf16_t>;
+  return launch_status(run(a, (cudaStream_t)stream), what);
+}
+
+int fc_gated_ff_bwd(const fc_gated_ff_desc* desc, const void* grad_y, const void* x,
+                    const void* const* value_weights, const void* gate_weight, const void* gate_bias,
+                    const void* scales, int64_t n_rows, void* workspace, void* grad_x,
+                    void* const* grad_value_weights, void* grad_gate_weight, void* grad_gate_bias, int32_t* status,
+                    fc_stream_t stream) {
+  const char* what = "fc_gated_ff_bwd";
+  GatedArgs a;
+  if (int rc = gated_args(desc, x, value_weights, gate_weight, gate_bias, scales, n_rows, workspace, status, what, a))
+    return rc;
+  if (n_rows > 0 && !grad_y) return fail(FC_ERR_INVALID, "%s: null tensor", what);
+  a.gy = grad_y;
+  a.gx = grad_x;
+  for (int l = 0; l <= desc->l_max; ++l) a.gwv[l] = grad_value_weights ? grad_value_weights[l] : nullptr;
+  a.gwg = grad_gate_weight;
+  a.gbias = grad_gate_bias;
+  const auto run = desc->dtype == FC_F32 ? gated_simple_bwd<float>
+                   : desc->dtype == FC_F64 ? gated_simple_bwd<double>
+                                           : gated_simple_bwd<bf16_t>;
+  return launch_status(run(a, (cudaStream_t)stream), what);
 }
 
 // ------------------------------------------------------------------ linear maps, split weights

@@ -1572,3 +1572,440 @@ class timed_region:
 
     def __exit__(self, *exc):
         return self._t.__exit__(*exc)
+
+
+# --------------------------------------------------------------------------- training blocks
+#
+# Element embedding, gated feed-forward and irreps dropout. They take float32, float64 and
+# bfloat16 rows, return every gradient, and may be differentiated twice (force training). The
+# entry points run as autograd functions on the impl functions below, without the dispatcher's
+# cost per call; the same operators are registered as flashcart::* for traced programs.
+
+
+def _block_code(dtype: torch.dtype, what: str) -> int:
+    if dtype == torch.bfloat16:
+        return N.FC_BF16
+    if dtype in (torch.float32, torch.float64):
+        return _code(dtype)
+    raise ValueError(f"{what} supports float32, float64 and bfloat16, got {dtype}")
+
+
+def _grad_needed(*tensors: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _same_device(what: str, ref: Tensor, *tensors: Optional[Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.device != ref.device:
+            raise ValueError(f"{what}: tensors on different devices ({ref.device}, {t.device})")
+
+
+def _embedding_args(table: Tensor, index: Tensor) -> None:
+    _require_cuda(table, index)
+    _same_device("embedding", table, index)
+    if table.dim() != 2:
+        raise ValueError(f"embedding: table must be (n_types, features), got shape {tuple(table.shape)}")
+    if index.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"embedding: index must be int64 or int32, got {index.dtype}")
+
+
+def _embedding_fwd(table: Tensor, index: Tensor, scale: float, offset: float) -> Tensor:
+    _embedding_args(table, index)
+    code = _block_code(table.dtype, "embedding")
+    t, idx = table.contiguous(), _idx(index)
+    out = t.new_empty(tuple(idx.shape) + (t.shape[1],))
+    lib = N.lib()
+    with _timed("embedding_fwd", 1, _nbytes(t, idx, out)):
+        rc = lib.fc_embedding_fwd(_p(t), t.shape[0], t.shape[1], code, _p(idx), idx.numel(), float(scale),
+                                  float(offset), _p(out), _p(status_word(t.device)), _stream(t.device))
+    _after(lib, rc, "fc_embedding_fwd", t.device)
+    return out
+
+
+def _embedding_bwd(grad_out: Tensor, index: Tensor, n_types: int, scale: float) -> Tensor:
+    _require_cuda(grad_out, index)
+    _same_device("embedding", grad_out, index)
+    code = _block_code(grad_out.dtype, "embedding")
+    if grad_out.dim() < 1 or tuple(grad_out.shape[:-1]) != tuple(index.shape):
+        raise ValueError(f"embedding: grad_out must be index.shape + (features,), got {tuple(grad_out.shape)} for "
+                         f"{tuple(index.shape)}")
+    g, idx = grad_out.contiguous(), _idx(index)
+    d = g.shape[-1]
+    out = g.new_empty((int(n_types), d))
+    lib = N.lib()
+    nb = lib.fc_embedding_bwd_workspace_bytes(idx.numel(), int(n_types), d, code)
+    if nb < 0:
+        N.check(lib, int(nb), "fc_embedding_bwd_workspace_bytes")
+    ws = torch.empty(int(nb), dtype=torch.uint8, device=g.device)
+    with _timed("embedding_bwd", 4, _nbytes(g, idx, out)):
+        rc = lib.fc_embedding_bwd(_p(g), _p(idx), idx.numel(), int(n_types), d, code, float(scale), _p(ws), _p(out),
+                                  _p(status_word(g.device)), _stream(g.device))
+    _after(lib, rc, "fc_embedding_bwd", g.device)
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, index, scale, offset):
+        ctx.save_for_backward(index)
+        ctx.args = (table.shape[0], scale)
+        return _embedding_fwd(table, index, scale, offset)
+
+    @staticmethod
+    def backward(ctx, g):
+        (index,) = ctx.saved_tensors
+        n, scale = ctx.args
+        if _grad_needed(g):
+            return _EmbeddingGrad.apply(g, index, n, scale), None, None, None
+        return _embedding_bwd(g, index, n, scale), None, None, None
+
+
+class _EmbeddingGrad(torch.autograd.Function):
+    """The table gradient as a function of the output gradient (its gradient is a lookup)."""
+
+    @staticmethod
+    def forward(ctx, g, index, n_types, scale):
+        ctx.save_for_backward(index)
+        ctx.scale = scale
+        return _embedding_bwd(g, index, n_types, scale)
+
+    @staticmethod
+    def backward(ctx, v):
+        (index,) = ctx.saved_tensors
+        return embedding(v, index, ctx.scale), None, None, None
+
+
+def embedding(table: Tensor, index: Tensor, scale: float = 1.0, offset: float = 0.0) -> Tensor:
+    """``offset + scale * table[index]`` for a (n_types, features) table: element features
+    (reference ``model/flashcart.py:160``) and element-dependent path weights ``1 +
+    delta[type]`` (``nn/layers.py:701-765``) in one pass.
+
+    The table gradient is summed over sorted tokens in an order fixed by the sizes (equal
+    inputs give equal bits), in float32 (float64 for float64 tables) and rounded once. An
+    index outside the table sets ``FC_DEV_BAD_INDEX`` (:func:`check_device_status`); its row
+    is zeros and its gradient is dropped."""
+    if torch.compiler.is_compiling():
+        return torch.ops.flashcart.embedding_fwd(table, index, float(scale), float(offset))
+    if _grad_needed(table):
+        return _Embedding.apply(table, index, float(scale), float(offset))
+    return _embedding_fwd(table, index, scale, offset)
+
+
+def _dropout_args(x: Tensor, rng: Tensor, p: float, l_max: int) -> int:
+    _require_cuda(x, rng)
+    _same_device("irreps_dropout", x, rng)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"irreps_dropout: p must lie in [0, 1], got {p}")
+    if rng.dtype != torch.int64 or rng.numel() != 2:
+        raise ValueError("irreps_dropout: rng must hold two int64 values (seed, offset)")
+    if l_max < 0 or l_max > N.FC_MAX_L:
+        raise NotImplementedError(f"irreps_dropout supports l_max up to {N.FC_MAX_L}, got {l_max}")
+    if x.dim() != 2 or x.shape[1] % (l_max + 1) ** 2:
+        raise ValueError(f"irreps_dropout: x must be (n, (l_max+1)^2 * features), got shape {tuple(x.shape)}")
+    return x.shape[1] // (l_max + 1) ** 2
+
+
+def _irreps_dropout(x: Tensor, rng: Tensor, p: float, l_max: int) -> Tensor:
+    features = _dropout_args(x, rng, p, l_max)
+    code = _block_code(x.dtype, "irreps_dropout")
+    x, rng = x.contiguous(), rng.contiguous()
+    y = torch.empty_like(x)
+    lib = N.lib()
+    with _timed("irreps_dropout", 1, _nbytes(x, y)):
+        rc = lib.fc_irreps_dropout(int(l_max), features, code, _p(x), _p(rng), float(p), x.shape[0], _p(y),
+                                   _stream(x.device))
+    _after(lib, rc, "fc_irreps_dropout", x.device)
+    return y
+
+
+class _IrrepsDropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, rng, p, l_max):
+        ctx.save_for_backward(rng)
+        ctx.args = (p, l_max)
+        return _irreps_dropout(x, rng, p, l_max)
+
+    @staticmethod
+    def backward(ctx, g):
+        (rng,) = ctx.saved_tensors
+        return irreps_dropout(g, rng, *ctx.args), None, None, None
+
+
+def irreps_dropout(x: Tensor, rng: Tensor, p: float, l_max: int = 0) -> Tensor:
+    """``x * keep / (1 - p)`` on rank-block rows, one decision per (row, rank, channel) shared
+    by the rank's components (so the operator commutes with rotations); ``l_max = 0`` is
+    elementwise dropout of plain rows.
+
+    ``rng`` holds (seed, offset) as two int64 values on the device: the mask is regenerated
+    from them in the gradient and never stored, so they must not change in between (advance a
+    copy, as :class:`flashcart_b200.nn.blocks.IrrepsDropout` does). ``p = 1`` drops everything;
+    a dropped element is 0 whatever it held."""
+    if torch.compiler.is_compiling():
+        return torch.ops.flashcart.irreps_dropout(x, rng, float(p), int(l_max))
+    if _grad_needed(x):
+        return _IrrepsDropout.apply(x, rng, float(p), int(l_max))
+    return _irreps_dropout(x, rng, float(p), int(l_max))
+
+
+_GATE_ACTS = {"silu": N.FC_GATE_SILU, "sigmoid": N.FC_GATE_SIGMOID}
+
+
+def _gated_args(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor, gate_bias: Optional[Tensor],
+                scales: Tensor, l_max: int, activation: str) -> N.GatedFfDesc:
+    what = "gated_feed_forward"
+    _require_cuda(x, gate_weight, gate_bias, scales, *value_weights)
+    _same_device(what, x, gate_weight, gate_bias, scales, *value_weights)
+    if activation not in _GATE_ACTS:
+        raise ValueError(f"{what}: activation must be 'silu' or 'sigmoid', got {activation!r}")
+    if l_max < 0 or l_max > N.FC_MAX_L:
+        raise NotImplementedError(f"{what} supports l_max up to {N.FC_MAX_L}, got {l_max}")
+    ranks = l_max + 1
+    if len(value_weights) != ranks:
+        raise ValueError(f"{what}: {ranks} value weights expected, got {len(value_weights)}")
+    h, c = value_weights[0].shape if value_weights[0].dim() == 2 else (0, 0)
+    if h <= 0 or c <= 0 or any(tuple(w.shape) != (h, c) for w in value_weights):
+        raise ValueError(f"{what}: value weights must all be (hidden, in), got "
+                         f"{[tuple(w.shape) for w in value_weights]}")
+    if tuple(gate_weight.shape) != (ranks * h, c):
+        raise ValueError(f"{what}: gate_weight must be ({ranks * h}, {c}), got {tuple(gate_weight.shape)}")
+    if gate_bias is not None and tuple(gate_bias.shape) != (ranks * h,):
+        raise ValueError(f"{what}: gate_bias must be ({ranks * h},), got {tuple(gate_bias.shape)}")
+    if x.dim() != 2 or x.shape[1] != ranks * ranks * c:
+        raise RuntimeError(f"Incorrect last dimension for x. Expected {ranks * ranks * c}, got {x.shape[-1]}.")
+    code = _block_code(x.dtype, what)
+    for t in (gate_weight, gate_bias, *value_weights):
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError(f"{what}: weights must have the type of x ({x.dtype}), got {t.dtype}")
+    acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+    if scales.dtype != acc or scales.numel() != l_max + 3:
+        raise ValueError(f"{what}: scales must hold {l_max + 3} {acc} values (one per rank, the gate map's, the "
+                         f"activation's), got {scales.numel()} of {scales.dtype}")
+    return N.GatedFfDesc(int(l_max), int(c), int(h), _GATE_ACTS[activation], code)
+
+
+def _gated_workspace(lib, d: N.GatedFfDesc, n: int, backward: bool, device) -> Tensor:
+    nb = lib.fc_gated_ff_workspace_bytes(ctypes.byref(d), n, int(backward))
+    if nb < 0:
+        N.check(lib, int(nb), "fc_gated_ff_workspace_bytes")
+    return torch.empty(max(16, int(nb)), dtype=torch.uint8, device=device)
+
+
+def _gated_ff_fwd(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor, gate_bias: Optional[Tensor],
+                  scales: Tensor, l_max: int, activation: str) -> Tensor:
+    d = _gated_args(x, value_weights, gate_weight, gate_bias, scales, l_max, activation)
+    x, wg, sc = x.contiguous(), gate_weight.contiguous(), scales.contiguous()
+    wv = [w.contiguous() for w in value_weights]
+    b = None if gate_bias is None else gate_bias.contiguous()
+    y = x.new_empty((x.shape[0], (l_max + 1) ** 2 * d.hidden_features))
+    lib = N.lib()
+    ws = _gated_workspace(lib, d, x.shape[0], False, x.device)
+    with _timed("gated_ff_fwd", 2, _nbytes(x, y, wg, b, *wv)):
+        rc = lib.fc_gated_ff_fwd(ctypes.byref(d), _p(x), _ptr_array(wv), _p(wg), _p(b), _p(sc), x.shape[0], _p(ws),
+                                 _p(y), _p(status_word(x.device)), _stream(x.device))
+    _after(lib, rc, "fc_gated_ff_fwd", x.device)
+    return y
+
+
+def _gated_ff_bwd(grad_y: Tensor, x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor,
+                  gate_bias: Optional[Tensor], scales: Tensor, l_max: int, activation: str,
+                  need: Sequence[bool]) -> List[Optional[Tensor]]:
+    """Gradients of (x, gate_weight, gate_bias, *value_weights), None where ``need`` is false."""
+    d = _gated_args(x, value_weights, gate_weight, gate_bias, scales, l_max, activation)
+    if tuple(grad_y.shape) != (x.shape[0], (l_max + 1) ** 2 * d.hidden_features) or grad_y.dtype != x.dtype:
+        raise ValueError(f"gated_feed_forward: grad_y must be {(x.shape[0], (l_max + 1) ** 2 * d.hidden_features)} of "
+                         f"{x.dtype}, got {tuple(grad_y.shape)} of {grad_y.dtype}")
+    _require_cuda(grad_y)
+    _same_device("gated_feed_forward", x, grad_y)
+    g, x, wg, sc = grad_y.contiguous(), x.contiguous(), gate_weight.contiguous(), scales.contiguous()
+    wv = [w.contiguous() for w in value_weights]
+    b = None if gate_bias is None else gate_bias.contiguous()
+    ins = [x, wg, b, *wv]
+    outs = [torch.empty_like(t) if t is not None and n else None for t, n in zip(ins, need)]
+    if not any(t is not None for t in outs):
+        return outs
+    lib = N.lib()
+    ws = _gated_workspace(lib, d, x.shape[0], True, x.device)
+    with _timed("gated_ff_bwd", 8, _nbytes(g, *ins, *outs)):
+        rc = lib.fc_gated_ff_bwd(ctypes.byref(d), _p(g), _p(x), _ptr_array(wv), _p(wg), _p(b), _p(sc), x.shape[0],
+                                 _p(ws), _p(outs[0]), _ptr_array(outs[3:]), _p(outs[1]), _p(outs[2]),
+                                 _p(status_word(x.device)), _stream(x.device))
+    _after(lib, rc, "fc_gated_ff_bwd", x.device)
+    return outs
+
+
+def _gated_composed(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor, gate_bias: Optional[Tensor],
+                    scales: Tensor, l_max: int, activation: str) -> Tensor:
+    """The same block out of twice-differentiable operators (bfloat16 in float32)."""
+    dtype, n = x.dtype, x.shape[0]
+    acc = torch.float64 if dtype == torch.float64 else torch.float32
+    ranks = l_max + 1
+    h, c = value_weights[0].shape
+    x, wg, wv = x.to(acc), gate_weight.to(acc), [w.to(acc) for w in value_weights]
+    squares = [l * l for l in range(ranks)]
+    lists = ([q * c for q in squares], [q * h for q in squares], [l * c * h for l in range(ranks)],
+             [2 * l + 1 for l in range(ranks)], [c] * ranks, [h] * ranks)
+    meta = torch.zeros(1, 6, dtype=torch.int64)
+    is64 = acc == torch.float64
+    prec = "ieee"
+    v = torch.ops.flashcart.linear_fwd(x, wv, meta, ranks * ranks * h, is64, prec, *lists, scales[:ranks])
+    z = torch.ops.flashcart.linear_fwd(x[:, :c], [wg], meta, ranks * h, is64, prec, [0], [0], [0], [1], [c],
+                                       [ranks * h], scales[ranks:ranks + 1])
+    if gate_bias is not None:
+        z = z + gate_bias.to(acc)
+    s = torch.sigmoid(z)
+    a = (scales[ranks + 1] * (s if activation == "sigmoid" else z * s)).view(n, ranks, h)
+    of = _expand_index(l_max, x.device)
+    return (v.view(n, ranks * ranks, h) * a.index_select(1, of)).reshape(n, ranks * ranks * h).to(dtype)
+
+
+class _GatedFeedForward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_weight, gate_bias, scales, l_max, activation, *value_weights):
+        ctx.save_for_backward(x, gate_weight, gate_bias, scales, *value_weights)
+        ctx.args = (l_max, activation)
+        return _gated_ff_fwd(x, value_weights, gate_weight, gate_bias, scales, l_max, activation)
+
+    @staticmethod
+    def backward(ctx, g):
+        x, wg, b, scales, *wv = ctx.saved_tensors
+        l_max, activation = ctx.args
+        need = [ctx.needs_input_grad[i] for i in (0, 1, 2, *range(6, 6 + len(wv)))]
+        if torch.is_grad_enabled():
+            # a second derivative is wanted: the gradient as a differentiable composition
+            ins = [x, wg, b, *wv]
+            y = _gated_composed(x, wv, wg, b, scales, l_max, activation)
+            got = iter(torch.autograd.grad(y, [t for t, n in zip(ins, need) if n], g, create_graph=True))
+            outs = [next(got) if n else None for n in need]
+        else:
+            outs = _gated_ff_bwd(g, x, wv, wg, b, scales, l_max, activation, need)
+        return (*outs[:3], None, None, None, *outs[3:])
+
+
+def gated_feed_forward(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor, gate_bias: Optional[Tensor],
+                       scales: Tensor, l_max: int, activation: str) -> Tensor:
+    """``y_k = a_l * (s_l x_k Wv_l^T)`` with ``a_l = s_act act(s_gate x_0 Wg_l^T + b_l)`` for
+    every component k of rank l: the gate and value maps, the activation and the product of
+    ``EquivariantGatedLayer`` (reference ``nn/layers.py:543-648``) in one kernel; with ``l_max =
+    0`` the usual gated feed-forward block of plain rows.
+
+    ``x`` (n, (l_max+1)^2 * in), ``value_weights`` l_max+1 of (hidden, in), ``gate_weight``
+    ((l_max+1) * hidden, in), ``gate_bias`` or None, all of one type (float32, float64 or
+    bfloat16); ``scales`` (l_max+3 values: s_0 .. s_l_max, s_gate, s_act) float32, float64 with
+    float64 rows, and constant. float32 products are 3xTF32 on the tensor cores. The backward
+    recomputes the products from ``x``; weight gradients do not depend on timing. A backward
+    that builds a graph (force training) runs as a composition of twice-differentiable maps."""
+    if torch.compiler.is_compiling():
+        return torch.ops.flashcart.gated_ff_fwd(x, list(value_weights), gate_weight, gate_bias, scales, int(l_max),
+                                                activation)
+    if _grad_needed(x, gate_weight, gate_bias, *value_weights):
+        return _GatedFeedForward.apply(x, gate_weight, gate_bias, scales, int(l_max), activation, *value_weights)
+    return _gated_ff_fwd(x, value_weights, gate_weight, gate_bias, scales, int(l_max), activation)
+
+
+@torch.library.custom_op("flashcart::embedding_fwd", mutates_args=())
+def embedding_fwd(table: Tensor, index: Tensor, scale: float, offset: float) -> Tensor:
+    return _embedding_fwd(table, index, scale, offset)
+
+
+@embedding_fwd.register_fake
+def _(table, index, scale, offset):
+    return table.new_empty(tuple(index.shape) + (table.shape[1],))
+
+
+@torch.library.custom_op("flashcart::embedding_bwd", mutates_args=())
+def embedding_bwd(grad_out: Tensor, index: Tensor, n_types: int, scale: float) -> Tensor:
+    return _embedding_bwd(grad_out, index, n_types, scale)
+
+
+@embedding_bwd.register_fake
+def _(grad_out, index, n_types, scale):
+    return grad_out.new_empty((n_types, grad_out.shape[-1]))
+
+
+def _embedding_setup(ctx, inputs, output):
+    table, index, scale, _ = inputs
+    ctx.save_for_backward(index)
+    ctx.args = (table.shape[0], scale)
+
+
+def _embedding_backward(ctx, g):
+    return torch.ops.flashcart.embedding_bwd(g, ctx.saved_tensors[0], *ctx.args), None, None, None
+
+
+def _embedding_bwd_setup(ctx, inputs, output):
+    _, index, _, scale = inputs
+    ctx.save_for_backward(index)
+    ctx.scale = scale
+
+
+def _embedding_bwd_backward(ctx, v):
+    return torch.ops.flashcart.embedding_fwd(v, ctx.saved_tensors[0], ctx.scale, 0.0), None, None, None
+
+
+embedding_fwd.register_autograd(_embedding_backward, setup_context=_embedding_setup)
+embedding_bwd.register_autograd(_embedding_bwd_backward, setup_context=_embedding_bwd_setup)
+
+
+@torch.library.custom_op("flashcart::irreps_dropout", mutates_args=())
+def irreps_dropout_op(x: Tensor, rng: Tensor, p: float, l_max: int) -> Tensor:
+    return _irreps_dropout(x, rng, p, l_max)
+
+
+@irreps_dropout_op.register_fake
+def _(x, rng, p, l_max):
+    return torch.empty_like(x)
+
+
+def _dropout_setup(ctx, inputs, output):
+    ctx.save_for_backward(inputs[1])
+    ctx.args = tuple(inputs[2:])
+
+
+def _dropout_backward(ctx, g):
+    return torch.ops.flashcart.irreps_dropout(g, ctx.saved_tensors[0], *ctx.args), None, None, None
+
+
+irreps_dropout_op.register_autograd(_dropout_backward, setup_context=_dropout_setup)
+
+
+@torch.library.custom_op("flashcart::gated_ff_fwd", mutates_args=())
+def gated_ff_fwd(x: Tensor, value_weights: List[Tensor], gate_weight: Tensor, gate_bias: Optional[Tensor],
+                 scales: Tensor, l_max: int, activation: str) -> Tensor:
+    return _gated_ff_fwd(x, value_weights, gate_weight, gate_bias, scales, l_max, activation)
+
+
+@gated_ff_fwd.register_fake
+def _(x, value_weights, gate_weight, gate_bias, scales, l_max, activation):
+    return x.new_empty((x.shape[0], (l_max + 1) ** 2 * value_weights[0].shape[0]))
+
+
+@torch.library.custom_op("flashcart::gated_ff_bwd", mutates_args=())
+def gated_ff_bwd(grad_y: Tensor, x: Tensor, value_weights: List[Tensor], gate_weight: Tensor,
+                 gate_bias: Optional[Tensor], scales: Tensor, l_max: int,
+                 activation: str) -> Tuple[Tensor, Tensor, Tensor, List[Tensor]]:
+    """First-order gradients (x, gate_weight, gate_bias or an empty tensor, value_weights)."""
+    gx, gwg, gb, *gwv = _gated_ff_bwd(grad_y, x, value_weights, gate_weight, gate_bias, scales, l_max, activation,
+                                      [True] * (3 + len(value_weights)))
+    return gx, gwg, x.new_empty((0,)) if gb is None else gb, gwv
+
+
+@gated_ff_bwd.register_fake
+def _(grad_y, x, value_weights, gate_weight, gate_bias, scales, l_max, activation):
+    return (torch.empty_like(x), torch.empty_like(gate_weight),
+            x.new_empty((0,)) if gate_bias is None else torch.empty_like(gate_bias),
+            [torch.empty_like(w) for w in value_weights])
+
+
+def _gated_setup(ctx, inputs, output):
+    x, wv, wg, b, scales, l_max, activation = inputs
+    ctx.save_for_backward(x, wg, b, scales, *wv)
+    ctx.args = (l_max, activation)
+
+
+def _gated_backward(ctx, g):
+    x, wg, b, scales, *wv = ctx.saved_tensors
+    gx, gwg, gb, gwv = torch.ops.flashcart.gated_ff_bwd(g, x, wv, wg, b, scales, *ctx.args)
+    return gx, gwv, gwg, None if b is None else gb, None, None, None
+
+
+gated_ff_fwd.register_autograd(_gated_backward, setup_context=_gated_setup)

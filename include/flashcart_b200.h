@@ -53,7 +53,7 @@ typedef void* fc_stream_t;
 /* dtypes */
 #define FC_F32 0
 #define FC_F64 1
-#define FC_BF16 2  /* fc_newton_schulz input; fc_linear_fwd storage (x, weights, y in bf16) */
+#define FC_BF16 2  /* fc_newton_schulz input; fc_linear_fwd storage (x, weights, y in bf16); training blocks */
 
 /* activation applied to a linear map's input (fc_linear_desc.act): the radial MLP's SiLU
  * between its layers (nn/layers.py:12-44) folded into the next layer's GEMM */
@@ -323,6 +323,64 @@ int fc_gate_fwd(int32_t l_max, int32_t features, int32_t dtype, const void* valu
                 int64_t n_rows, void* y, fc_stream_t stream);
 int fc_gate_bwd(int32_t l_max, int32_t features, int32_t dtype, const void* grad_y, const void* values,
                 const void* gates, int64_t n_rows, void* grad_values, void* grad_gates, fc_stream_t stream);
+
+/* ---------------------------------------------------------------- element embedding
+ * out[i, :] = offset + scale * table[idx[i], :] for i < n_rows (the element embeddings and
+ * element-dependent path weights 1 + delta[type], nn/layers.py:701-765), and its gradient
+ * grad_table[v, :] = scale * sum of grad_out[i, :] over idx[i] == v, computed by sorting the
+ * tokens: no atomics, equal inputs give equal bits, every row of grad_table is written.
+ * table, grad_table: (n_types, features); out, grad_out: (n_rows, features); dtype FC_F32,
+ * FC_F64 or FC_BF16 for all of them (sums in float, in double for FC_F64). An index outside
+ * [0, n_types) sets FC_DEV_BAD_INDEX; its output row is zeros and its gradient is dropped.
+ * n_rows and n_types must be below 2^31 - 4096 in the backward (FC_ERR_CAPACITY). workspace:
+ * fc_embedding_bwd_workspace_bytes bytes of device memory, 16-byte aligned (negative: an
+ * error code). */
+int fc_embedding_fwd(const void* table, int64_t n_types, int64_t features, int32_t dtype, const int64_t* idx,
+                     int64_t n_rows, double scale, double offset, void* out, int32_t* status, fc_stream_t stream);
+int64_t fc_embedding_bwd_workspace_bytes(int64_t n_rows, int64_t n_types, int64_t features, int32_t dtype);
+int fc_embedding_bwd(const void* grad_out, const int64_t* idx, int64_t n_rows, int64_t n_types, int64_t features,
+                     int32_t dtype, double scale, void* workspace, void* grad_table, int32_t* status,
+                     fc_stream_t stream);
+
+/* ---------------------------------------------------------------- irreps dropout
+ * y = x * keep / (1 - p) on rank-block rows (n_rows, (l_max+1)^2 * features), one decision
+ * per (row, rank, channel) shared by the rank's components. keep comes from a counter-based
+ * generator (Philox 4x32-10) with rng[0] = seed as key and rng[1] = offset in the upper half
+ * of the counter (device int64 values), so the mask is never stored: the gradient is this
+ * call on the output gradient with the same rng. p in [0, 1]; a dropped element is 0. dtype
+ * FC_F32, FC_F64 or FC_BF16; x and y must not overlap. */
+int fc_irreps_dropout(int32_t l_max, int32_t features, int32_t dtype, const void* x, const int64_t* rng, double p,
+                      int64_t n_rows, void* y, fc_stream_t stream);
+
+/* ---------------------------------------------------------------- gated feed-forward
+ * The products of EquivariantGatedLayer.forward before its output map (nn/layers.py:543-648)
+ * in one kernel: for every row and rank l, with x_k the in_features channels of component k,
+ *   a_l = s_act * act(s_gate * x_0 Wg_l^T + b_l),   y_k = a_l * (s_l * x_k Wv_l^T).
+ * l_max = 0 is the usual gated feed-forward block of plain rows. x: (n_rows, (l_max+1)^2 *
+ * in_features); y: (n_rows, (l_max+1)^2 * hidden_features); value_weights: l_max+1 device
+ * pointers (in host memory) to (hidden_features, in_features); gate_weight: ((l_max+1) *
+ * hidden_features, in_features); gate_bias: (l_max+1) * hidden_features values or NULL;
+ * scales: s_0 .. s_l_max, s_gate, s_act on the device (float; double for FC_F64). dtype
+ * FC_F32 (3xTF32 tensor-core products), FC_F64 or FC_BF16 (float accumulation and gates, one
+ * rounding of y). The backward recomputes the products from x and writes the gradients that
+ * are not NULL (grad_value_weights: NULL, or l_max+1 pointers, each of which may be NULL);
+ * none depends on timing. workspace: fc_gated_ff_workspace_bytes bytes, 16-byte aligned. */
+#define FC_GATE_SILU 0
+#define FC_GATE_SIGMOID 1
+typedef struct fc_gated_ff_desc {
+  int32_t l_max, in_features, hidden_features;
+  int32_t act;   /* FC_GATE_SILU / FC_GATE_SIGMOID */
+  int32_t dtype; /* FC_F32, FC_F64 or FC_BF16 */
+} fc_gated_ff_desc;
+int64_t fc_gated_ff_workspace_bytes(const fc_gated_ff_desc* desc, int64_t n_rows, int32_t backward);
+int fc_gated_ff_fwd(const fc_gated_ff_desc* desc, const void* x, const void* const* value_weights,
+                    const void* gate_weight, const void* gate_bias, const void* scales, int64_t n_rows,
+                    void* workspace, void* y, int32_t* status, fc_stream_t stream);
+int fc_gated_ff_bwd(const fc_gated_ff_desc* desc, const void* grad_y, const void* x,
+                    const void* const* value_weights, const void* gate_weight, const void* gate_bias,
+                    const void* scales, int64_t n_rows, void* workspace, void* grad_x,
+                    void* const* grad_value_weights, void* grad_gate_weight, void* grad_gate_bias, int32_t* status,
+                    fc_stream_t stream);
 
 /* ---------------------------------------------------------------- edge expansion
  * Cartesian expansion of edge features: out[e, k, c] = moments[e, k] * h[e, r, c] over the
