@@ -66,6 +66,18 @@ int64_t embed_bwd_workspace(int64_t R, int64_t V, int64_t D, int dtype);
 template <typename T>
 int irreps_dropout(int, int, const void*, const int64_t*, double, int64_t, void*, cudaStream_t);
 
+#ifndef FC_HOST_EMU
+template <typename T>
+static int gated_fwd(const GatedArgs& a, cudaStream_t s) { return gated_tc_fwd<T>(a, s); }
+template <typename T>
+static int gated_bwd(const GatedArgs& a, cudaStream_t s) { return gated_tc_bwd<T>(a, s); }
+#else
+template <typename T>
+static int gated_fwd(const GatedArgs& a, cudaStream_t s) { return gated_simple_fwd<T>(a, s); }
+template <typename T>
+static int gated_bwd(const GatedArgs& a, cudaStream_t s) { return gated_simple_bwd<T>(a, s); }
+#endif
+
 static thread_local std::string g_last_error;
 
 static int fail(int code, const char* fmt, ...) {
@@ -965,6 +977,10 @@ static int gated_check(const fc_gated_ff_desc* d, int64_t n_rows, const char* wh
 
 int64_t fc_gated_ff_workspace_bytes(const fc_gated_ff_desc* desc, int64_t n_rows, int32_t backward) {
   if (int rc = gated_check(desc, n_rows, "fc_gated_ff_workspace_bytes")) return rc;
+#ifndef FC_HOST_EMU
+  if (desc->dtype != FC_F64)
+    return gated_tc_ws(desc->l_max, desc->in_features, desc->hidden_features, n_rows, desc->dtype, backward);
+#endif
   return gated_simple_ws(desc->l_max, desc->in_features, desc->hidden_features, n_rows, desc->dtype, backward);
 }
 
@@ -1005,9 +1021,9 @@ int fc_gated_ff_fwd(const fc_gated_ff_desc* desc, const void* x, const void* con
   if (n_rows == 0) return FC_OK;
   if (!y) return fail(FC_ERR_INVALID, "%s: null tensor", what);
   a.y = y;
-  const auto run = desc->dtype == FC_F32 ? gated_simple_fwd<float>
+  const auto run = desc->dtype == FC_F32   ? gated_fwd<float>
                    : desc->dtype == FC_F64 ? gated_simple_fwd<double>
-                                           : gated_simple_fwd<bf16_t>;
+                                           : gated_fwd<bf16_t>;
   return launch_status(run(a, (cudaStream_t)stream), what);
 }
 
@@ -1026,9 +1042,9 @@ int fc_gated_ff_bwd(const fc_gated_ff_desc* desc, const void* grad_y, const void
   for (int l = 0; l <= desc->l_max; ++l) a.gwv[l] = grad_value_weights ? grad_value_weights[l] : nullptr;
   a.gwg = grad_gate_weight;
   a.gbias = grad_gate_bias;
-  const auto run = desc->dtype == FC_F32 ? gated_simple_bwd<float>
+  const auto run = desc->dtype == FC_F32   ? gated_bwd<float>
                    : desc->dtype == FC_F64 ? gated_simple_bwd<double>
-                                           : gated_simple_bwd<bf16_t>;
+                                           : gated_bwd<bf16_t>;
   return launch_status(run(a, (cudaStream_t)stream), what);
 }
 

@@ -1,5 +1,5 @@
-// Gated feed-forward block over Cartesian features, every type and size (the tensor-core
-// form of 32- and 16-bit rows is in gated_ff_tc.cu).
+// Gated feed-forward block over Cartesian features: 64-bit rows, and the host emulation of
+// every type (the tensor-core form of 32- and 16-bit rows is in gated_ff_tc.cu).
 //
 // For row n, rank l, component m (x_k: the C channels of component k = l^2 + m):
 //   z_l = s_g x_0 Wg_l^T + b_l,   a_l = s_a act(z_l),   v_k = s_l x_k Wv_l^T,   y_k = a_l v_k
@@ -376,8 +376,10 @@ int gated_simple_bwd(const GatedArgs& a, cudaStream_t s) {
 #define FC_GATED_INST(T)                                           \
   template int gated_simple_fwd<T>(const GatedArgs&, cudaStream_t); \
   template int gated_simple_bwd<T>(const GatedArgs&, cudaStream_t);
-FC_GATED_INST(float)
 FC_GATED_INST(double)
+#ifdef FC_HOST_EMU
+FC_GATED_INST(float)
 FC_GATED_INST(bf16_t)
+#endif
 
 }  // namespace fc

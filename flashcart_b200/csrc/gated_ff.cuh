@@ -43,11 +43,20 @@ FC_HD FC_INLINE A gated_dact(int act, A z) {
   return act == FC_GATE_SIGMOID ? s * (A(1) - s) : s * (A(1) + z * (A(1) - s));
 }
 
-// The one-thread-per-output-tile kernels (gated_ff.cu): every type and size.
+// Plain multiply-add tiles (gated_ff.cu): 64-bit rows, and every type in the host emulation.
 int64_t gated_simple_ws(int L, int C, int H, int64_t n, int dtype, int backward);
 template <typename T>
 int gated_simple_fwd(const GatedArgs& a, cudaStream_t s);
 template <typename T>
 int gated_simple_bwd(const GatedArgs& a, cudaStream_t s);
+
+#ifndef FC_HOST_EMU
+// Tensor-core form of float and bfloat16 rows (gated_ff_tc.cu).
+int64_t gated_tc_ws(int L, int C, int H, int64_t n, int dtype, int backward);
+template <typename T>
+int gated_tc_fwd(const GatedArgs& a, cudaStream_t s);
+template <typename T>
+int gated_tc_bwd(const GatedArgs& a, cudaStream_t s);
+#endif
 
 }  // namespace fc

@@ -32,10 +32,9 @@
 // go to the tensor cores as they land. Operand boxes start at k = 32 * slab (128-byte
 // aligned x coordinate); store boxes start at n = 32 * chunk.
 #include "linear.cuh"
+#include "tc_common.cuh"
 
 #ifndef FC_HOST_EMU
-
-#include <cuda.h>  // CUtensorMap and the driver enums (header only; the entry point is fetched at run time)
 
 #include <algorithm>
 #include <mutex>
@@ -43,7 +42,6 @@
 namespace fc {
 namespace tma {
 
-constexpr int BM = 128;
 constexpr int BK = 32;
 #ifndef FC_TMA_SPLIT_WARPS
 #define FC_TMA_SPLIT_WARPS 4
@@ -55,7 +53,6 @@ constexpr int THREADS = (EPI_WARP0 + 4) * 32;
 constexpr int RING_BYTES = 192 * 1024;
 constexpr int EPI_BYTES = 4 * 2 * 32 * 128;  // two 4 KB staging buffers per epilogue warp
 constexpr int BAR_BYTES = 256;
-constexpr long long WAIT_LIMIT = 1ll << 22;
 // k slabs per accumulation unit. The tensor cores accumulate in fp32 but not with
 // IEEE round-to-nearest at every step; over thousands of k the error grows beyond
 // what an fp32 dot product shows. Each unit of KG slabs (128 k; as accurate against float64
@@ -128,41 +125,6 @@ struct BMaps {
   CUtensorMap r;  // ACT >= 2: the aux rows, laid out like C (loaded per 32 x 32 box by the epilogue)
 };
 
-__device__ __forceinline__ uint32_t smem_u32(const void* p) {
-  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-
-// 32 consecutive tensor-memory columns of this thread's lane (warp-collective).
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]),
-      "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]),
-      "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]),
-      "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-
-#ifndef FC_TMA_INT_ROUND
-#define FC_TMA_INT_ROUND 1
-#endif
-// fp32 -> tf32 (10 explicit mantissa bits), round to nearest with ties away from zero:
-// add half a tf32 unit in the last place to the magnitude bits and clear the 13 dropped
-// bits (integer add + and; a carry into the exponent is the correct rounding up to the
-// next binade). Infinities are kept; a NaN whose payload sits only in the dropped bits
-// becomes an infinity, and in the 3xTF32 split the residual x - hi is then NaN, so NaN
-// still reaches the result.
-__device__ __forceinline__ float round_tf32(float x) {
-#if FC_TMA_INT_ROUND
-  return __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xFFFFE000u);
-#else
-  uint32_t r;
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-  return __uint_as_float(r);
-#endif
-}
-
 // SiLU and its derivative for the activation modes (fast exp / divide intrinsics; the
 // argument is clamped to +-80, where the sigmoid is 0 or 1 to float32 precision).
 __device__ __forceinline__ float act_sigmoid(float z) {
@@ -173,114 +135,6 @@ __device__ __forceinline__ float act_silu(float z) { return z * act_sigmoid(z); 
 __device__ __forceinline__ float act_dsilu(float z) {
   const float sg = act_sigmoid(z);
   return sg * (1.f + z * (1.f - sg));
-}
-
-__device__ __forceinline__ uint64_t make_desc(uint32_t saddr) {
-  // K-major, 128-byte swizzle, descriptor version 1; 1024 B between 8-row groups.
-  uint64_t d = 0;
-  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
-}
-
-template <int BN>
-__host__ __device__ constexpr uint32_t idesc_tf32() {
-  // D f32, A / B tf32, both K-major, M = 128, N = BN.
-  return (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
-}
-
-// D (tensor memory) += A (tensor memory: row m in lane m, 8 k in consecutive columns) x B.
-template <int BN>
-__device__ __forceinline__ void mma_ta(uint32_t d, uint32_t ta, uint64_t db, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::tf32 [%0], [%1], %2, %3, p;\n\t}\n"
-      :
-      : "r"(d), "r"(ta), "l"(db), "r"(idesc_tf32<BN>()), "r"(acc));
-}
-
-template <int BN>
-__device__ __forceinline__ void mma(uint32_t d, uint64_t da, uint64_t db, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}\n"
-      :
-      : "r"(d), "l"(da), "l"(db), "r"(idesc_tf32<BN>()), "r"(acc));
-}
-
-__device__ __forceinline__ void commit(uint32_t mbar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(mbar) : "memory");
-}
-
-__device__ __forceinline__ void arrive(uint32_t mbar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(mbar) : "memory");
-}
-
-__device__ __forceinline__ void arrive_tx(uint32_t mbar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mbar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ bool test_parity(uint32_t mbar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(ok)
-      : "r"(mbar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
-// Bounded wait for the phase of the given parity. Gives up early (returning false)
-// once another role has raised the CTA's abort flag.
-__device__ __forceinline__ bool wait_parity(uint32_t mbar, uint32_t parity, volatile int* abort_flag,
-                                            int* status) {
-  for (long long it = 0; it < WAIT_LIMIT; ++it) {
-    if (test_parity(mbar, parity)) return true;
-    if ((it & 255) == 255 && *abort_flag) return false;
-  }
-  *abort_flag = 1;
-  fc_flag(status, FC_DEV_TIMEOUT);
-  return false;
-}
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z,
-                                            uint32_t mbar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-          "r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(mbar)
-      : "memory");
-}
-
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t mbar) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
-          dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(mbar)
-      : "memory");
-}
-
-// L2 prefetch of a box of A (no shared-memory destination): keeps more HBM traffic in
-// flight than the shared-memory ring alone can hold.
-__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int x, int y, int z) {
-  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global.tile [%0, {%1, %2, %3}];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(x), "r"(y), "r"(z)
-               : "memory");
-}
-
-__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(src), "r"(x), "r"(y), "r"(z)
-               : "memory");
 }
 
 struct TileCoord {
@@ -684,10 +538,6 @@ __global__ void presplit_kernel(const float* __restrict__ w, int ldw, int trans_
 }
 
 // ---------------------------------------------------------------------------------- host
-
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 struct DeviceState {
   bool ready = false;
