@@ -4,31 +4,39 @@
 // Mathematics and row layout: gated_ff.cu. The scales s_l, s_g are folded into the split
 // weights, so the accumulators hold v_k and z_l - b_l themselves.
 //
-// gated_tc_kernel, one persistent CTA per SM, 16 warps:
-//   warp 0       TMA producer, and the CTA's draw from the work list (an atomic counter)
-//   warp 1       MMA issue (one thread)
-//   warps 4-7    splitters: the A slab (128 rows x 32 channels) to tf32 parts in tensor memory
-//   warps 8-15   epilogue: two warps per lane quarter, 64 columns each
-// A work item is one rank l of 128 rows (and 128 hidden channels): first the gate product
-// x_0 Wg_l, whose activation the epilogue warps keep in registers (64 columns of their row),
-// then the 2l+1 value products, each multiplied by the gate on its way out. So x is read
-// once per component (x_0 once more per rank), y is written once, and neither gates nor
-// values touch memory. Three modes share the pipeline:
+// A work item is one rank l of 128 rows and 64 output channels: first the gate product
+// x_0 Wg_l, kept by the epilogue warps in registers, then the 2l+1 value products, each
+// multiplied by the gate's activation on its way out. So y is written once, and neither gates
+// nor values touch memory. Three modes share the kernel:
 //   FWD  y_k = a_l v_k
 //   PRE  the backward's first half: z_l and v_k again; g comes in by TMA while they are
 //        computed; dv_k = g a_l goes out, sum_m g v_k stays in registers until the rank is
 //        done and dz_l goes out
 //   DX   dx_k = dv_k Wv_l (+ sum_l dz_l Wg_l for k = 0): items are (128 rows, component)
-// wgrad_kernel forms dWv_l and dWg_l: the rows are the reduction, so both operands have to be
-// transposed; the splitters do that on the way (a lane of tensor memory or a row of the
-// K-major B tile is one channel, and a thread gathers its 32 rows' values from the row-major
-// slab without bank conflicts). Every CTA takes an equal share of the slabs of all weight
-// matrices, and a second kernel adds the partial matrices in order.
 //
+// What bounds it: DRAM (x in, y out: 453 MB for 27,648 x 16 rows of 128 channels, 70 us at the
+// copy rate), with the tensor cores close behind (63 us). A ring whose stages held A and the
+// weights' slabs together was three deep in shared memory and waited for its copies (149 us:
+// gated_ff_stream.cu, still used above 128 channels). Here the item's two weight matrices stay
+// in shared memory (64 output channels x 128 x hi, lo: 64 KB each), work lists are ordered by
+// rank so that they are loaded a few times per launch, and the ring holds A slabs alone. The
+// price is that x is read from L2 once per 64 output channels.
+//
+// A tensor-core accumulation truncates the running sum (measured relative error of one
+// accumulator: 4.5e-7 after 12 instructions, 8.2e-7 after 24, 1.6e-6 after 48), so a slab's
+// small products (Ahi Wlo, Alo Whi) go in before its Ahi Whi, the even and the odd slabs of a
+// pass go to two accumulators, and the epilogue adds them.
+//
+// Roles of the 20 warps (one persistent CTA per SM):
+//   warp 0       TMA producer of A slabs, and the CTA's draw from its work list
+//   warps 1, 3   MMA issue
+//   warp 2       TMA producer of the weights
+//   warps 4-11   splitters: the slab (128 rows x 32 channels) to tf32 parts in tensor memory;
+//                two groups of four take the slabs in turn
+//   warps 12-19  epilogue: two per lane quarter, 32 columns each
 // Waits are bounded: on expiry the CTA raises FC_DEV_TIMEOUT, all roles stop, copies and MMAs
 // in flight are drained and tensor memory is freed.
-#include "gated_ff.cuh"
-#include "tc_common.cuh"
+#include "gated_ff_tc.cuh"
 
 #ifndef FC_HOST_EMU
 
@@ -37,195 +45,92 @@
 namespace fc {
 namespace gtc {
 
-using namespace tma;
-
-constexpr int BN = 128, BK = 32, THREADS = 512;
-constexpr int EPI_WARPS = 8, EPI_BUF = 4096, EPI_BYTES = EPI_WARPS * 2 * EPI_BUF;
-constexpr int BAR_BYTES = 512;
-constexpr int TILE_B = BN * BK * 4;
-constexpr int A_COLS = 128;  // tensor-memory columns of the A parts' ring
-constexpr int NACC = 3;      // accumulators behind them
-constexpr int SCHED = 4;
-// Slabs per accumulation unit. A tensor-core accumulation truncates the running sum (measured
-// relative error: 4.5e-7 after 12 instructions, 8.2e-7 after 24, 1.6e-6 after 48), so a unit
-// is 64 products, its small terms (hi x lo, lo x hi) go in before the slab's hi x hi while
-// the sum is small, and the units are added in fp32 registers.
-constexpr int KG = 2;
-enum { FWD = 0, PRE = 1, DX = 2 };
+constexpr int BN = 64;
+constexpr int W_LO = (BN * BK * 4) >> 4;  // descriptor step from a slab's Whi to its Wlo
+constexpr int W_SLAB = 2 * BN * BK * 4;  // [Whi | Wlo] of one k slab: 128 K-major rows, 16 KB
+constexpr int MAX_NK = 4;                // k slabs of a resident matrix
+// Tensor memory: four A slots of hi | lo columns (an MMA's slot is refilled about 700 cycles
+// after it is issued, two slabs' worth of MMAs) and two accumulators.
+constexpr int NACC = 2 /* (the code flips between them) */, ACC_W = 2 * BN, A_COLS = 256;
+constexpr int MAX_STAGES = 8;
+constexpr int SMEM_MAX = 227 * 1024;
+constexpr int SPLIT_WARP0 = 4, EPI_WARP0 = 12, EPI_WARPS = 8, TC_THREADS = (EPI_WARP0 + EPI_WARPS) * 32;
+constexpr int TC_REGS = 96;  // per thread at launch; the epilogue takes what the first four warps leave
 
 template <int MODE, typename T>
 struct Cfg {
   static constexpr bool A32 = MODE == DX || sizeof(T) == 4;  // A in float32: hi and lo parts
   static constexpr int TILE_A = BM * BK * (A32 ? 4 : 2);
-  static constexpr int STAGE = TILE_A + 2 * TILE_B;
   static constexpr int A_STAGE = A32 ? 2 * BK : BK;  // tensor-memory columns
-  static constexpr int STAGES = A32 ? 3 : 4;
-  static constexpr int A_RING = A_COLS / A_STAGE;
-  static constexpr int SMEM = STAGES * STAGE + EPI_BYTES + BAR_BYTES + 1024;
-  static_assert(A_COLS + NACC * BN <= 512, "tensor memory");
-  static_assert(SMEM <= 227 * 1024, "shared memory per CTA");
+  // Slots of the A ring. Even, so that a slot belongs to one splitter group and one MMA warp,
+  // whose waits miss none of its barriers' phases. PRE keeps pre-activations behind them.
+  static constexpr int A_RING = MODE == PRE && A32 ? 2 : 4, Z_COL = 192;
+  static constexpr int BUFS = MODE == PRE ? 2 : 1;   // staging boxes per epilogue warp
+  static constexpr int FIXED = EPI_WARPS * BUFS * EPI_BUF + BAR_BYTES + 1024;
+  static_assert(A_RING * A_STAGE <= (MODE == PRE ? Z_COL : A_COLS) && A_COLS + NACC * ACC_W <= 512, "tensor memory");
+  // even, so that a stage always belongs to the same splitter group: its waits tell one phase
+  // of a stage's barrier from the next only if they miss none
+  static int stages(int nk) { return std::min(MAX_STAGES, (SMEM_MAX - FIXED - 2 * nk * W_SLAB) / TILE_A) & ~1; }
+  static int smem(int nk, int st) { return FIXED + 2 * nk * W_SLAB + st * TILE_A; }
 };
 
-struct Args {
-  int64_t items;
-  int L, ranks, comps;
-  int N;                  // output columns of a component: H (FWD, PRE), C (DX)
-  int nk, kg, nu;         // 32-wide slabs of a segment, slabs per unit, units per segment
-  int n_ct, tiles, main_tiles, per_comp;
-  int act;
-  const void* bias;       // T, or null
-  const float* act_scale;
-  int* counter;           // work list, zeroed before the launch
-  int* status;
-};
-
-struct Maps {
-  CUtensorMap a;   // x (FWD, PRE) or dv (DX): (channel, row, component)
-  CUtensorMap a2;  // dz (DX): (channel, row, rank)
-  CUtensorMap b;   // split weights: (k, output channel, matrix)
-  CUtensorMap o;   // y, dv or dx, 32 x 32 boxes
-  CUtensorMap g;   // g (PRE)
-  CUtensorMap o2;  // dz (PRE)
-};
-
-// A work item: rows 128 tile.., columns 128 ct.., and rank l's components m0 .. m0+nm-1 (FWD,
-// PRE) or component k (DX).
+// Work item: 128 rows, and rank l's components k0 .. k0+nm-1.
 struct Item {
-  int tile, ct, l, k0, nm;
+  int tile, l, k0, nm;
 };
 
-template <int MODE>
+// Lists run through the ranks (high ones first: most work), all tiles of one before the next.
 __device__ __forceinline__ Item item_of(const Args& a, int it) {
   Item w;
-  if (MODE == DX || a.per_comp) {
-    const int per_tile = a.comps * a.n_ct;
-    w.tile = it / per_tile;
-    const int r = it - w.tile * per_tile;
-    w.k0 = r / a.n_ct;
-    w.ct = r - w.k0 * a.n_ct;
+  const int q = it / a.tiles;
+  w.tile = it - q * a.tiles;
+  if (a.per_comp) {
+    w.k0 = a.comps - 1 - q;
     w.l = gated_rank_of(w.k0);
     w.nm = 1;
-    return w;
-  }
-  // ranks of a tile one after the other, high ranks (most work) first; the last tiles rank by
-  // rank, so that the work list ends with its smallest items
-  const int group = a.ranks * a.n_ct, split = a.main_tiles * group;
-  if (it < split) {
-    w.tile = it / group;
-    const int r = it - w.tile * group;
-    w.l = a.L - r / a.n_ct;
-    w.ct = r % a.n_ct;
   } else {
-    const int tail = (a.tiles - a.main_tiles) * a.n_ct, r0 = it - split, r = r0 % tail;
-    w.l = a.L - r0 / tail;
-    w.tile = a.main_tiles + r / a.n_ct;
-    w.ct = r % a.n_ct;
+    w.l = a.L - q;
+    w.k0 = w.l * w.l;
+    w.nm = 2 * w.l + 1;
   }
-  w.k0 = w.l * w.l;
-  w.nm = 2 * w.l + 1;
   return w;
 }
 
-template <int N>
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, float* f);
-template <>
-__device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, float* f) {
-  uint32_t v[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
-        "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
-        "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(v[c]);
-}
-template <>
-__device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, float* f) {
-  uint32_t v[16];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int c = 0; c < 16; ++c) f[c] = __uint_as_float(v[c]);
-}
-
-// 32 floats -> the tf32 parts of a lane's 32 columns
-template <bool LO>
-__device__ __forceinline__ void store_parts(uint32_t ta, const float* x) {
-  uint32_t p[32];
-#pragma unroll
-  for (int e = 0; e < 32; ++e) p[e] = __float_as_uint(round_tf32(x[e]));
-  tmem_st32(ta, p);
-  if (LO) {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) p[e] = __float_as_uint(round_tf32(x[e] - round_tf32(x[e])));
-    tmem_st32(ta + BK, p);
-  }
-}
-
-// wait_parity for a whole warp: one answer, so that no lane leaves a collective alone
-__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int* abort_flag, int* status) {
-  return __all_sync(0xffffffffu, wait_parity(bar, parity, abort_flag, status));
-}
-
-__device__ __forceinline__ void drain_bar(uint32_t bar, uint32_t parity) {
-  for (long long it = 0; it < WAIT_LIMIT; ++it)
-    if (test_parity(bar, parity)) break;
-}
-
-// A warp's 32 x 32 staging box: row r in 32 * sizeof(E) bytes, its 16-byte chunks swizzled as
-// TMA does for that row width (128 bytes: c ^ (r & 7); 64 bytes: c ^ ((r >> 1) & 3)).
-template <typename E>
-__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-  return sizeof(E) == 4 ? r * 128 + ((c ^ (r & 7)) << 4) : r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-}
-
-// one row of 32 floats into the staging box
-template <typename E>
-__device__ __forceinline__ void put_row(uint8_t* buf, int r, const float* f) {
-  constexpr int PER = 16 / sizeof(E);
-#pragma unroll
-  for (int c = 0; c < 32 / PER; ++c) {
-    Pack<E, PER> p;
-#pragma unroll
-    for (int k = 0; k < PER; ++k) p.set(k, Io<E>::put(f[c * PER + k]));
-    p.store(reinterpret_cast<E*>(buf + chunk_at<E>(r, c)));
-  }
-}
-
-#define FC_SETMAXNREG_DEC(n) asm volatile("setmaxnreg.dec.sync.aligned.u32 " #n ";")
-#define FC_SETMAXNREG_INC(n) asm volatile("setmaxnreg.inc.sync.aligned.u32 " #n ";")
-
+// An item's product passes: FWD, PRE the gate, then a value product per component, by the
+// rank's gate matrix (weight slot 0) and value matrix (slot 1), which stay until the rank
+// changes. DX one pass per component by the rank's transposed value matrix (slot 0); component
+// 0 adds up ranks + 1 passes, through all transposed gate matrices in alternating slots (with
+// one rank both simply stay).
 template <int MODE, typename T>
-__global__ void __launch_bounds__(THREADS, 1) gated_tc_kernel(const __grid_constant__ Maps mp, const Args a) {
+__global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_constant__ Maps mp, const Args a) {
   using C = Cfg<MODE, T>;
-  constexpr int S = C::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* epi = smem + S * C::STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(epi + EPI_BYTES);
-  uint64_t* split = full + S;
-  uint64_t* empty = split + S;
-  uint64_t* a_free = empty + S;  // the MMAs have read a slot of the A ring
-  uint64_t* acc_full = a_free + C::A_RING;
+  const int S = a.stages, nk = a.nk;
+  uint8_t* wmem = smem;                          // two weight slots of nk slabs
+  uint8_t* ring = wmem + 2 * nk * W_SLAB;        // A stages
+  uint8_t* epi = ring + S * C::TILE_A;           // staging boxes
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi + EPI_WARPS * C::BUFS * EPI_BUF);
+  uint64_t* empty = full + MAX_STAGES;
+  uint64_t* a_full = empty + MAX_STAGES;
+  uint64_t* a_free = a_full + C::A_RING;
+  uint64_t* w_full = a_free + C::A_RING;         // [slot][k slab]
+  uint64_t* w_free = w_full + 2 * MAX_NK;
+  uint64_t* acc_full = w_free + 2;
   uint64_t* acc_empty = acc_full + NACC;
   uint64_t* sched_full = acc_empty + NACC;
   uint64_t* sched_empty = sched_full + SCHED;
   uint64_t* drain = sched_empty + SCHED;
-  uint64_t* aux = drain + 1;  // per epilogue warp and buffer: the box of g has landed
-  int* sched = reinterpret_cast<int*>(aux + 2 * EPI_WARPS);
+  uint64_t* aux = drain + 1;                     // per epilogue warp and box: g has landed
+  int* sched = reinterpret_cast<int*>(aux + EPI_WARPS * C::BUFS);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sched + SCHED);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((3 * S + C::A_RING + 2 * NACC + 2 * SCHED + 1 + 2 * EPI_WARPS) * 8 + SCHED * 4 + 8 <= BAR_BYTES, "barriers");
+  static_assert((2 * MAX_STAGES + 2 * C::A_RING + 2 * MAX_NK + 2 + 2 * NACC + 2 * SCHED + 1 + EPI_WARPS * C::BUFS) * 8 +
+                        SCHED * 4 + 8 <=
+                    BAR_BYTES,
+                "barriers");
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512));
@@ -235,22 +140,26 @@ __global__ void __launch_bounds__(THREADS, 1) gated_tc_kernel(const __grid_const
     auto init = [](uint64_t* b, int n) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n));
     };
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < MAX_STAGES; ++s) {
       init(&full[s], 1);
-      init(&split[s], 128);
-      init(&empty[s], 1);
+      init(&empty[s], 4);
     }
-    for (int b = 0; b < C::A_RING; ++b) init(&a_free[b], 1);
+    for (int b = 0; b < C::A_RING; ++b) {
+      init(&a_full[b], 4);
+      init(&a_free[b], 1);
+    }
+    for (int b = 0; b < 2 * MAX_NK; ++b) init(&w_full[b], 1);
+    for (int b = 0; b < 2; ++b) init(&w_free[b], 2);
     for (int b = 0; b < NACC; ++b) {
-      init(&acc_full[b], 1);
+      init(&acc_full[b], 2);
       init(&acc_empty[b], EPI_WARPS);
     }
     for (int b = 0; b < SCHED; ++b) {
       init(&sched_full[b], 1);
-      init(&sched_empty[b], 1 + 4 + EPI_WARPS);
+      init(&sched_empty[b], 3 + 8 + EPI_WARPS);  // MMA, weights, splitter and epilogue warps
     }
-    init(drain, 1);
-    for (int b = 0; b < 2 * EPI_WARPS; ++b) init(&aux[b], 1);
+    init(drain, 2);
+    for (int b = 0; b < EPI_WARPS * C::BUFS; ++b) init(&aux[b], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -258,749 +167,512 @@ __global__ void __launch_bounds__(THREADS, 1) gated_tc_kernel(const __grid_const
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;");
   const uint32_t tmem = *tmem_slot;
+  const int ct = (int)blockIdx.x % a.n_ct;  // this CTA's 64 output channels
+  const bool cycle = MODE == DX && a.ranks > 1;
 
-  // the q-th item of this CTA for a warp (-1: no more, or a wait gave up)
-  auto next_item = [&](int q) -> int {
+  // the q-th item of this CTA (-1: no more, or a wait gave up), for one thread or a whole warp
+  auto item_one = [&](int q) -> int {
     const int s = q % SCHED;
-    if (!wait_warp(smem_u32(&sched_full[s]), (uint32_t)((q / SCHED) & 1), abort_flag, a.status)) return -1;
+    if (!wait_phase(smem_u32(&sched_full[s]), (uint32_t)((q / SCHED) & 1), abort_flag)) return -1;
+    const int it = *reinterpret_cast<volatile int*>(&sched[s]);
+    arrive(smem_u32(&sched_empty[s]));
+    return it;
+  };
+  auto item_warp = [&](int q) -> int {
+    const int s = q % SCHED;
+    if (!wait_warp(smem_u32(&sched_full[s]), (uint32_t)((q / SCHED) & 1), abort_flag)) return -1;
     const int it = *reinterpret_cast<volatile int*>(&sched[s]);
     __syncwarp();
     if (lane == 0) arrive(smem_u32(&sched_empty[s]));
     return it;
   };
-  auto segments = [&](const Item& w) { return MODE == DX && w.k0 == 0 ? a.ranks + 1 : 1; };
-  auto substeps = [&](const Item& w) { return MODE == DX ? 1 : 1 + w.nm; };
+  auto passes_of = [&](const Item& w) { return MODE == DX ? (w.k0 == 0 ? a.ranks + 1 : w.nm) : 1 + w.nm; };
 
-  if (warp < 4) {
-    FC_SETMAXNREG_DEC(48);
-    if (warp == 0 && lane == 0) {
-      // ---------------------------------------------------------------- TMA producer
-      constexpr uint32_t bytes = C::TILE_A + 2 * TILE_B;
-      int next = (int)blockIdx.x;
+  if (warp < SPLIT_WARP0) {
+    FC_SETMAXNREG_DEC(40);
+    if (warp == 0 && elect_one()) {
+      // ---------------------------------------------------------------- A producer, work list
+      const int first = (int)blockIdx.x / a.n_ct, group = (int)gridDim.x / a.n_ct;
+      int next = first;
+      int s = 0;
+      uint32_t lap = 0;  // of the ring
       int64_t g = 0;
       bool ok = true;
       for (int q = 0; ok; ++q) {
         const int s4 = q % SCHED;
         if (q >= SCHED &&
-            !wait_parity(smem_u32(&sched_empty[s4]), (uint32_t)((q / SCHED - 1) & 1), abort_flag, a.status))
+            !wait_phase(smem_u32(&sched_empty[s4]), (uint32_t)((q / SCHED - 1) & 1), abort_flag))
           break;
         const int it = next < a.items ? next : -1;
         *reinterpret_cast<volatile int*>(&sched[s4]) = it;
         arrive(smem_u32(&sched_full[s4]));
         if (it < 0) break;
-        next = (int)gridDim.x + atomicAdd(a.counter, 1);
-        const Item w = item_of<MODE>(a, it);
-        const int subs = substeps(w), segs = segments(w);
-        for (int sub = 0; sub < subs && ok; ++sub)
-          for (int seg = 0; seg < segs && ok; ++seg) {
-            const CUtensorMap* ma = &mp.a;
-            int z = MODE == DX ? w.k0 : (sub == 0 ? 0 : w.k0 + sub - 1);
-            int mat = w.l;
-            if (MODE == DX) {
-              if (seg > 0) {
-                ma = &mp.a2;
-                z = seg - 1;
-                mat = a.ranks + seg - 1;
-              }
-            } else if (sub == 0) {
-              mat = a.ranks + w.l;
-            }
-            for (int kt = 0; kt < a.nk; ++kt, ++g) {
-              const int s = (int)(g % S);
-              if (g >= S && !wait_parity(smem_u32(&empty[s]), (uint32_t)(((g / S) - 1) & 1), abort_flag, a.status)) {
-                ok = false;
-                break;
-              }
-              uint8_t* st = smem + s * C::STAGE;
-              const uint32_t fb = smem_u32(&full[s]);
-              arrive_tx(fb, bytes);
-              tma_load_3d(smem_u32(st), ma, kt * BK, w.tile * BM, z, fb);
-              tma_load_3d(smem_u32(st + C::TILE_A), &mp.b, kt * BK, w.ct * BN, mat, fb);
-              tma_load_3d(smem_u32(st + C::TILE_A + TILE_B), &mp.b, kt * BK, w.ct * BN, mat + 2 * a.ranks, fb);
-            }
+        next = group + atomicAdd(a.counter + ct, 1);
+        const Item w = item_of(a, it);
+        const int passes = passes_of(w);
+        for (int p = 0; p < passes && ok; ++p) {
+          const bool gates = MODE == DX && w.k0 == 0 && p > 0;
+          const CUtensorMap* ma = gates ? &mp.a2 : &mp.a;
+          const int z = gates ? p - 1 : MODE == DX ? w.k0 + p : (p == 0 ? 0 : w.k0 + p - 1);
+          if (MODE == PRE && p + 1 < passes) {
+            // two A stages are too few to cover DRAM: have the next pass's operands in L2
+            tma_prefetch_3d(&mp.ap, 0, w.tile * BM, w.k0 + p);
+            tma_prefetch_3d(&mp.gp, ct * BN, w.tile * BM, w.k0 + p);
           }
-      }
-      // the last load issued into every stage must have landed before the CTA exits
-      for (int s = 0; s < S; ++s) {
-        const int64_t uses = g > s ? (g - 1 - s) / S + 1 : 0;
-        if (uses > 0) drain_bar(smem_u32(&full[s]), (uint32_t)((uses - 1) & 1));
-      }
-    } else if (warp == 1 && lane == 0) {
-      // ---------------------------------------------------------------- MMA issue
-      int64_t g = 0, u = 0;
-      bool ok = true;
-      for (int q = 0; ok; ++q) {
-        const int s4 = q % SCHED;
-        if (!wait_parity(smem_u32(&sched_full[s4]), (uint32_t)((q / SCHED) & 1), abort_flag, a.status)) break;
-        const int it = *reinterpret_cast<volatile int*>(&sched[s4]);
-        arrive(smem_u32(&sched_empty[s4]));
-        if (it < 0) break;
-        const Item w = item_of<MODE>(a, it);
-        const int passes = substeps(w) * segments(w);
-        for (int p = 0; p < passes && ok; ++p)
-          for (int j = 0; j < a.nu && ok; ++j, ++u) {
-            const int b = (int)(u % NACC);
-            const int64_t v = u / NACC;
-            if (v >= 1 && !wait_parity(smem_u32(&acc_empty[b]), (uint32_t)((v - 1) & 1), abort_flag, a.status)) {
+          for (int kt = 0; kt < nk; ++kt, ++g) {
+            if (lap > 0 && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
               ok = false;
               break;
             }
+            const uint32_t fb = smem_u32(&full[s]);
+            arrive_tx(fb, C::TILE_A);
+            tma_load_3d(smem_u32(ring + s * C::TILE_A), ma, kt * BK, w.tile * BM, z, fb);
+            if (++s == S) {
+              s = 0;
+              ++lap;
+            }
+          }
+        }
+      }
+      // the last copy into every stage must have landed before the CTA exits
+      for (int t = 0; t < S; ++t) {
+        const int64_t uses = g > t ? (g - 1 - t) / S + 1 : 0;
+        if (uses > 0) drain_bar(smem_u32(&full[t]), (uint32_t)((uses - 1) & 1));
+      }
+    } else if (warp == 2 && elect_one()) {
+      // ---------------------------------------------------------------- weight producer
+      int rank = -1, loads0 = 0, loads1 = 0;
+      bool ok = true;
+      auto load = [&](int slot, int mat, int& loads) {
+        if (loads > 0 && !wait_phase(smem_u32(&w_free[slot]), (uint32_t)((loads - 1) & 1), abort_flag)) {
+          ok = false;
+          return;
+        }
+        for (int kt = 0; kt < nk; ++kt) {
+          uint8_t* to = wmem + (slot * nk + kt) * W_SLAB;
+          const uint32_t fb = smem_u32(&w_full[slot * MAX_NK + kt]);
+          arrive_tx(fb, W_SLAB);
+          tma_load_3d(smem_u32(to), &mp.b, kt * BK, ct * BN, mat, fb);
+          tma_load_3d(smem_u32(to + W_SLAB / 2), &mp.b, kt * BK, ct * BN, mat + 2 * a.ranks, fb);
+        }
+        ++loads;
+      };
+      for (int q = 0; ok; ++q) {
+        const int it = item_one(q);
+        if (it < 0) break;
+        const Item w = item_of(a, it);
+        if (cycle && w.k0 == 0) {
+          for (int p = 0; p <= a.ranks && ok; ++p) {
+            const int mat = p == 0 ? 0 : a.ranks + p - 1;
+            if (p & 1) load(1, mat, loads1);
+            else load(0, mat, loads0);
+          }
+          rank = -1;
+        } else if (w.l != rank) {
+          rank = w.l;
+          load(0, MODE == DX ? w.l : a.ranks + w.l, loads0);
+          if (!cycle && ok) load(1, MODE == DX ? a.ranks : w.l, loads1);
+        }
+      }
+      for (int kt = 0; kt < nk; ++kt) {
+        if (loads0 > 0) drain_bar(smem_u32(&w_full[kt]), (uint32_t)((loads0 - 1) & 1));
+        if (loads1 > 0) drain_bar(smem_u32(&w_full[MAX_NK + kt]), (uint32_t)((loads1 - 1) & 1));
+      }
+    } else if (warp == 1 || warp == 3) {
+      // ---------------------------------------------------------------- MMA issue
+      // Two warps, one for the even slabs of the ring and one for the odd: a slab's MMAs take 385
+      // cycles, and the barrier operations around them as long again, so each warp issues while
+      // the other one asks. Their sums go to the two halves of the accumulator. A whole warp
+      // walks the loop (its addresses and descriptors stay uniform) and one lane issues.
+      const int mine = warp >> 1;
+      const uint64_t desc = make_desc(smem_u32(wmem));
+      const uint32_t slot_step = (uint32_t)(nk * (W_SLAB >> 4));
+      int rank = -1;
+      uint32_t w_phase = 3u, held = 0u, check = 0u;  // per slot: phase of its last load, unreleased, not yet seen
+      int par = 0;  // parity of the pass's first slab
+      uint32_t as = (uint32_t)mine, a_phase = 0, ab = 0, acc_phase = 0;  // own A slot in turn, accumulator
+      bool ok = true;
+      bool a_ready = false, acc_ready = false;  // answers about the next slab and accumulator
+      auto fresh = [&](int slot) {  // the slot's next matrix: all that read its last one is issued
+        const uint32_t bit = 1u << slot;
+        if ((held & bit) && elect_one()) commit(smem_u32(&w_free[slot]));
+        held |= bit;
+        check |= bit;
+        w_phase ^= bit;
+      };
+      for (int q = 0; ok; ++q) {
+        const int it = item_warp(q);
+        if (it < 0) break;
+        const Item w = item_of(a, it);
+        const int passes = passes_of(w);
+        const bool through = cycle && w.k0 == 0;
+        if (through) {
+          rank = -1;
+        } else if (w.l != rank) {
+          rank = w.l;
+          fresh(0);
+          if (!cycle) fresh(1);
+        }
+        for (int p = 0; p < passes; ++p) {
+          const int slot = through ? (p & 1) : (cycle || p == 0) ? 0 : 1;
+          if (through) fresh(slot);
+          if (!acc_ready) ok = wait_warp(smem_u32(&acc_empty[ab]), acc_phase ^ 1u, abort_flag);
+          acc_ready = false;
+          const uint32_t d = tmem + (uint32_t)A_COLS + ab * (uint32_t)ACC_W + (uint32_t)(mine * BN);
+          const uint32_t ab_next = ab ^ 1u, acc_next = acc_phase ^ ab;
+          const uint64_t db0 = desc + (slot ? slot_step : 0u);
+          const bool check_w = (check >> slot) & 1u;
+          const int first = mine ^ par;
+#pragma unroll 1
+          for (int kt = first; kt < nk; kt += 2) {
+            if (check_w)
+              ok = ok && wait_warp(smem_u32(&w_full[slot * MAX_NK + kt]), (w_phase >> slot) & 1u, abort_flag);
+            if (!a_ready) ok = ok && wait_warp(smem_u32(&a_full[as]), a_phase, abort_flag);
+            if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;");
-            const uint32_t d = tmem + (uint32_t)(A_COLS + b * BN);
-            const int k_end = min(a.nk, (j + 1) * a.kg);
-            for (int kt = j * a.kg; kt < k_end; ++kt, ++g) {
-              const int s = (int)(g % S);
-              if (!wait_parity(smem_u32(&split[s]), (uint32_t)((g / S) & 1), abort_flag, a.status)) {
-                ok = false;
-                break;
-              }
-              asm volatile("tcgen05.fence::after_thread_sync;");
-              uint8_t* st = smem + s * C::STAGE;
-              const uint64_t dbh = make_desc(smem_u32(st + C::TILE_A));
-              const uint64_t dbl = make_desc(smem_u32(st + C::TILE_A + TILE_B));
-              const int slot = (int)(g % C::A_RING);
-              const uint32_t tah = tmem + (uint32_t)(slot * C::A_STAGE), tal = tah + (uint32_t)BK;
+            const bool wrap = as + 2 >= (uint32_t)C::A_RING;
+            const uint32_t as_next = wrap ? (uint32_t)mine : as + 2, ph_next = a_phase ^ (wrap ? 1u : 0u);
+            const bool peek_a = peek_parity(smem_u32(&a_full[as_next]), ph_next);
+            const bool peek_acc = peek_parity(smem_u32(&acc_empty[ab_next]), acc_next ^ 1u);
+            const uint64_t db = db0 + (uint64_t)(kt * (W_SLAB >> 4));
+            const uint32_t tah = tmem + as * (uint32_t)C::A_STAGE, tal = tah + (uint32_t)BK;
+            if (elect_one()) {
+              // the small products first: the sum that each accumulation truncates is then small
 #pragma unroll
               for (int kk = 0; kk < BK / 8; ++kk) {
-                const uint64_t off = (uint64_t)((kk * 32) >> 4);
-                mma_ta<BN>(d, tah + kk * 8, dbl + off, (kt > j * a.kg || kk > 0) ? 1u : 0u);
-                if (C::A32) mma_ta<BN>(d, tal + kk * 8, dbh + off, 1u);
+                mma_ta<BN>(d, tah + kk * 8, db + W_LO + 2 * kk, (kt > first || kk > 0) ? 1u : 0u);
+                if (C::A32) mma_ta<BN>(d, tal + kk * 8, db + 2 * kk, 1u);
               }
 #pragma unroll
-              for (int kk = 0; kk < BK / 8; ++kk) mma_ta<BN>(d, tah + kk * 8, dbh + (uint64_t)((kk * 32) >> 4), 1u);
-              // the stage and the A slot are free once these MMAs have completed
-              commit(smem_u32(&empty[s]));
-              commit(smem_u32(&a_free[slot]));
+              for (int kk = 0; kk < BK / 8; ++kk) mma_ta<BN>(d, tah + kk * 8, db + 2 * kk, 1u);
+              commit(smem_u32(&a_free[as]));  // the A slot is free once these MMAs have completed
             }
-            if (ok) commit(smem_u32(&acc_full[b]));
+            a_ready = __all_sync(0xffffffffu, peek_a);
+            acc_ready = __all_sync(0xffffffffu, peek_acc);
+            as = as_next;
+            a_phase = ph_next;
           }
+          if (ok && elect_one()) {
+            commit(smem_u32(&acc_full[ab]));
+            if (through) commit(smem_u32(&w_free[slot]));
+          }
+          __syncwarp();
+          par ^= nk & 1;
+          if (!ok) break;
+          check &= ~(1u << slot);
+          if (through) held &= ~(1u << slot);
+          ab = ab_next;
+          acc_phase = acc_next;
+        }
       }
-      commit(smem_u32(drain));  // every MMA completes before tensor memory is freed
-      drain_bar(smem_u32(drain), 0);
+      if (elect_one()) {
+        commit(smem_u32(drain));  // every MMA completes before tensor memory is freed
+        drain_bar(smem_u32(drain), 0);
+      }
+      __syncwarp();
     }
-  } else if (warp < 8) {
-    FC_SETMAXNREG_DEC(96);
+  } else if (warp < EPI_WARP0) {
     // ------------------------------------------------------------------ splitters
-    const int r = (warp & 3) * 32 + lane;  // row of the slab, lane of tensor memory
-    int64_t g = 0;
-    bool ok = true;
+    const int mine = (warp - SPLIT_WARP0) >> 2;  // this group's slabs: g = mine mod 2
+    const int r = (warp & 3) * 32 + lane;        // row of the slab, lane of tensor memory
+    // stage and lap of the ring, and slot of the A ring, of this group's next slab (every second
+    // one); `left` slabs of the current item remain, counted from the group's next one
+    int s = mine, left = -mine;
+    uint32_t lap = 0, as = (uint32_t)mine, as_lap = 0;
+    bool ok = true, full_ready = false, slot_ready = false;
     for (int q = 0; ok; ++q) {
-      const int it = next_item(q);
+      const int it = item_warp(q);
       if (it < 0) break;
-      const Item w = item_of<MODE>(a, it);
-      const int64_t end = g + (int64_t)substeps(w) * segments(w) * a.nk;
-      for (; g < end; ++g) {
-        const int s = (int)(g % S);
-        if (!wait_warp(smem_u32(&full[s]), (uint32_t)((g / S) & 1), abort_flag, a.status)) {
-          ok = false;
-          break;
-        }
-        const int slot = (int)(g % C::A_RING);
-        if (g >= C::A_RING &&
-            !wait_warp(smem_u32(&a_free[slot]), (uint32_t)((g / C::A_RING - 1) & 1), abort_flag, a.status)) {
-          ok = false;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;");
-        const uint8_t* slab = smem + s * C::STAGE;
-        const uint32_t ta = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(slot * C::A_STAGE);
+      left += passes_of(item_of(a, it)) * nk;
+      for (; left > 0; left -= 2) {
+        if (!full_ready) ok = wait_warp(smem_u32(&full[s]), lap & 1u, abort_flag);
+        if (!ok) break;
+        const uint8_t* slab = ring + s * C::TILE_A;
+        const uint32_t ta = tmem + ((uint32_t)((warp & 3) * 32) << 16) + as * (uint32_t)C::A_STAGE;
+        uint32_t x[32];
         if constexpr (C::A32) {
-          float x[32];
 #pragma unroll
           for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<float4*>(&x[4 * c]) = *reinterpret_cast<const float4*>(slab + chunk_at<float>(r, c));
-          store_parts<true>(ta, x);
-        } else {
-          uint32_t h[32];  // bfloat16 is a tf32 value: its bits are the high half
+            *reinterpret_cast<uint4*>(&x[4 * c]) = *reinterpret_cast<const uint4*>(slab + chunk_at<float>(r, c));
+        } else {  // bfloat16 is a tf32 value: its bits are the high half
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint4 v = *reinterpret_cast<const uint4*>(slab + chunk_at<bf16_t>(r, c));
             const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              h[8 * c + 2 * e] = vs[e] << 16;
-              h[8 * c + 2 * e + 1] = vs[e] & 0xFFFF0000u;
+              x[8 * c + 2 * e] = vs[e] << 16;
+              x[8 * c + 2 * e + 1] = vs[e] & 0xFFFF0000u;
             }
           }
-          tmem_st32(ta, h);
         }
+        // (the first lap's wait is for the phase before the first and succeeds at once)
+        if (!slot_ready) ok = wait_warp(smem_u32(&a_free[as]), (as_lap & 1u) ^ 1u, abort_flag);
+        if (!ok) break;
+        int s_next = s + 2;
+        uint32_t lap_next = lap;
+        if (s_next >= S) {
+          s_next -= S;
+          ++lap_next;
+        }
+        uint32_t as_next = as + 2, as_lap_next = as_lap;
+        if (as_next >= (uint32_t)C::A_RING) {
+          as_next -= (uint32_t)C::A_RING;
+          ++as_lap_next;
+        }
+        const bool peek_full = peek_parity(smem_u32(&full[s_next]), lap_next & 1u);
+        const bool peek_slot = peek_parity(smem_u32(&a_free[as_next]), (as_lap_next & 1u) ^ 1u);
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        if constexpr (C::A32) {
+          // hi: the upper 19 bits (tf32); lo: the rest, exact in float, rounded where tf32 ends
+          // (its lower 13 bits do not reach the product). Three operations an element: the
+          // kernel is short of issue slots before anything else.
+          uint32_t p[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) p[e] = x[e] & 0xFFFFE000u;
+          tmem_st32(ta, p);
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            p[e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xFFFFE000u)) + 0x1000u;
+          tmem_st32(ta + BK, p);
+        } else {
+          tmem_st32(ta, x);
+        }
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&empty[s]));  // the slab is in registers: its stage may be refilled
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        arrive(smem_u32(&split[s]));
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&a_full[as]));
+        full_ready = __all_sync(0xffffffffu, peek_full);
+        slot_ready = __all_sync(0xffffffffu, peek_slot);
+        s = s_next;
+        lap = lap_next;
+        as = as_next;
+        as_lap = as_lap_next;
       }
     }
   } else {
-    FC_SETMAXNREG_INC(184);
+    FC_SETMAXNREG_INC(120);
     // ------------------------------------------------------------------ epilogue
-    const int quarter = warp & 3, half = (warp - 8) >> 2;
-    uint8_t* stage0 = epi + (warp - 8) * 2 * EPI_BUF;
-    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(A_COLS + half * 64);
+    // one warp per lane quarter and 32 columns; a thread holds its row's 32 columns
+    const int quarter = warp & 3, half = (warp - EPI_WARP0) >> 2;
+    uint8_t* boxes = epi + (warp - EPI_WARP0) * C::BUFS * EPI_BUF;
+    uint64_t* landed = aux + (warp - EPI_WARP0) * C::BUFS;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(A_COLS + half * 32);
     const float sa = MODE == DX ? 0.f : __ldg(a.act_scale);
-    int64_t u = 0;
-    int nbuf = 0;
-    uint32_t aux_phase = 0;
+    const int col = ct * BN + half * 32;
+    const bool live = col < a.N;  // the warp has columns to write
+    uint32_t ab = 0, acc_phase = 0;  // the accumulator in turn
+    uint32_t par = 0;                // parity of the pass's first slab
     bool ok = true;
-    // units u .. u+count-1 are complete (their accumulators are read and then given back)
-    auto wait_unit = [&](int64_t v) {
-      const bool done = wait_warp(smem_u32(&acc_full[v % NACC]), (uint32_t)((v / NACC) & 1), abort_flag, a.status);
+    auto wait_acc = [&]() {
+      const bool done = wait_warp(smem_u32(&acc_full[ab]), acc_phase, abort_flag);
       asm volatile("tcgen05.fence::after_thread_sync;");
       return done;
     };
-    auto free_unit = [&](int64_t v) {
+    auto free_acc = [&]() {
       asm volatile("tcgen05.fence::before_thread_sync;");
       __syncwarp();
-      if (lane == 0) arrive(smem_u32(&acc_empty[v % NACC]));
+      if (lane == 0) arrive(smem_u32(&acc_empty[ab]));
+      par ^= (uint32_t)nk & 1u;
+      if (++ab == NACC) {
+        ab = 0;
+        acc_phase ^= 1u;
+      }
     };
-    // 32 columns of this warp's rows from the staging buffer to memory
-    auto send = [&](const CUtensorMap* map, uint8_t* buf, int col, int row, int z) {
+    // columns c0 .. c0+15 of the row: both halves of the accumulator (a single slab fills the
+    // half of its parity)
+    auto load16 = [&](int c0, float* f) {
+      const uint32_t t = lane_base + ab * (uint32_t)ACC_W + (uint32_t)c0;
+      if (nk > 1) tmem_ld_sum<16>(t, t + BN, f);
+      else tmem_ld<16>(t + par * BN, f);
+    };
+    // this warp's 32 x 32 box from staging to memory
+    auto send = [&](const CUtensorMap* map, uint8_t* buf, int row, int z) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) {
+      if (elect_one()) {
         tma_store_3d(map, smem_u32(buf), col, row, z);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
+      __syncwarp();
     };
+    // earlier stores have read their boxes (the elected lane is the same every time)
+    auto boxes_free = [&]() {
+      if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      __syncwarp();
+    };
+    uint32_t box = 0, box_phase = 0;  // PRE: the box in turn; bit b: parity of landed[b]'s next completion
     for (int q = 0; ok; ++q) {
-      const int it = next_item(q);
+      const int it = item_warp(q);
       if (it < 0) break;
-      const Item w = item_of<MODE>(a, it);
-      const int col0 = w.ct * BN + half * 64, row0 = w.tile * BM + quarter * 32;
-      const int nch = max(0, min(2, (a.N - col0 + 31) / 32));
+      const Item w = item_of(a, it);
+      const int row0 = w.tile * BM + quarter * 32;
       if constexpr (MODE == DX) {
-        float acc[64];
+        float acc[32];
+        const bool sums = w.k0 == 0;
+        const int passes = passes_of(w);
+        for (int p = 0; p < passes; ++p) {
+          if (!(ok = wait_acc())) break;
 #pragma unroll
-        for (int c = 0; c < 64; ++c) acc[c] = 0.f;
-        const int units = segments(w) * a.nu;
-        for (int j = 0; j < units && ok; ++j, ++u) {
-          if (!(ok = wait_unit(u))) break;
+          for (int h = 0; h < 2; ++h) {
+            float f[16];
+            load16(h * 16, f);
 #pragma unroll
-          for (int cb = 0; cb < 2; ++cb) {
-            float f[32];
-            tmem_ld<32>(lane_base + (uint32_t)((u % NACC) * BN + cb * 32), f);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) acc[cb * 32 + c] += f[c];
+            for (int c = 0; c < 16; ++c) acc[h * 16 + c] = (sums && p > 0) ? acc[h * 16 + c] + f[c] : f[c];
           }
-          free_unit(u);
+          free_acc();
+          if (live && (!sums || p + 1 == passes)) {
+            boxes_free();
+            put_row<T>(boxes, lane, acc);
+            send(&mp.o, boxes, row0, sums ? 0 : w.k0 + p);
+          }
         }
-        if (!ok) break;
-#pragma unroll
-        for (int cb = 0; cb < 2; ++cb)
-          if (cb < nch) {
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-            __syncwarp();
-            uint8_t* buf = stage0 + nbuf * EPI_BUF;
-            put_row<T>(buf, lane, acc + cb * 32);
-            send(&mp.o, buf, col0 + cb * 32, row0, w.k0);
-            nbuf ^= 1;
-          }
       } else {
-        // the gate: pre-activations of this thread's row and 64 columns
-        float z[64];
-#pragma unroll
-        for (int c = 0; c < 64; ++c) z[c] = 0.f;
-        for (int j = 0; j < a.nu && ok; ++j, ++u) {
-          if (!(ok = wait_unit(u))) break;
-#pragma unroll
-          for (int cb = 0; cb < 2; ++cb) {
-            float f[32];
-            tmem_ld<32>(lane_base + (uint32_t)((u % NACC) * BN + cb * 32), f);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) z[cb * 32 + c] += f[c];
+        // ask for component m's box of g
+        int asked = 0, got = 0;
+        auto ask = [&](int m, uint32_t b) {
+          asked = m + 1;
+          if (elect_one()) {
+            const uint32_t fb = smem_u32(&landed[b]);
+            arrive_tx(fb, 32 * 32 * sizeof(T));
+            tma_load_3d(smem_u32(boxes + b * EPI_BUF), &mp.g, col, row0, w.k0 + m, fb);
           }
-          free_unit(u);
+          __syncwarp();
+        };
+        if (MODE == PRE && live) {
+          boxes_free();
+          ask(0, box);
         }
-        if (!ok) break;
-        if (a.bias) {
+        float z[32];  // pre-activations of this thread's row
+        ok = wait_acc();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load16(h * 16, z + h * 16);
+        free_acc();
+        if (a.bias && live) {
           const T* b = (const T*)a.bias + (int64_t)w.l * a.N;
 #pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (col0 + c < a.N) z[c] += Io<T>::get(b[col0 + c]);
+          for (int c = 0; c < 32; ++c)
+            if (col + c < a.N) z[c] += Io<T>::get(b[col + c]);
         }
         if constexpr (MODE == FWD) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) z[c] = sa * gated_act<float>(a.act, z[c]);
+          for (int c = 0; c < 32; ++c) z[c] = sa * fast_act(a.act, z[c]);
           for (int m = 0; m < w.nm && ok; ++m) {
-            float acc[64];
+            if (!(ok = wait_acc())) break;
+            float f[32];
 #pragma unroll
-            for (int c = 0; c < 64; ++c) acc[c] = 0.f;
-            for (int j = 0; j < a.nu; ++j, ++u) {
-              if (!(ok = wait_unit(u))) break;
+            for (int h = 0; h < 2; ++h) load16(h * 16, f + h * 16);
+            free_acc();
+            if (live) {
 #pragma unroll
-              for (int cb = 0; cb < 2; ++cb) {
-                float f[32];
-                tmem_ld<32>(lane_base + (uint32_t)((u % NACC) * BN + cb * 32), f);
-#pragma unroll
-                for (int c = 0; c < 32; ++c) acc[cb * 32 + c] += f[c];
-              }
-              free_unit(u);
+              for (int c = 0; c < 32; ++c) f[c] *= z[c];
+              boxes_free();
+              put_row<T>(boxes, lane, f);
+              send(&mp.o, boxes, row0, w.k0 + m);
             }
-            if (!ok) break;
-#pragma unroll
-            for (int c = 0; c < 64; ++c) acc[c] *= z[c];
-#pragma unroll
-            for (int cb = 0; cb < 2; ++cb)
-              if (cb < nch) {
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-                __syncwarp();
-                uint8_t* buf = stage0 + nbuf * EPI_BUF;
-                put_row<T>(buf, lane, acc + cb * 32);
-                send(&mp.o, buf, col0 + cb * 32, row0, w.k0 + m);
-                nbuf ^= 1;
-              }
           }
         } else {
-          float sum[64];  // over m of g v
+          // the pre-activations wait in tensor memory until the rank is done; the gates stay here
+          const uint32_t z_at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(C::Z_COL + half * 32);
+          tmem_st32(z_at, reinterpret_cast<const uint32_t*>(z));
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 #pragma unroll
-          for (int c = 0; c < 64; ++c) sum[c] = 0.f;
+          for (int c = 0; c < 32; ++c) z[c] = sa * fast_act(a.act, z[c]);
+          float sum[32];  // over m of g v
+#pragma unroll
+          for (int c = 0; c < 32; ++c) sum[c] = 0.f;
           for (int m = 0; m < w.nm && ok; ++m) {
-            // the output gradient's boxes come in while the products are computed
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            __syncwarp();
-            if (lane == 0)
-              for (int cb = 0; cb < nch; ++cb) {
-                const uint32_t ab = smem_u32(&aux[(warp - 8) * 2 + cb]);
-                arrive_tx(ab, 32 * 32 * sizeof(T));
-                tma_load_3d(smem_u32(stage0 + cb * EPI_BUF), &mp.g, col0 + cb * 32, row0, w.k0 + m, ab);
+            if (!wait_acc()) ok = false;
+            if (got < asked) {
+              ++got;
+              const uint32_t par = (box_phase >> box) & 1u;
+              box_phase ^= 1u << box;
+              if (!wait_warp(smem_u32(&landed[box]), par, abort_flag)) {
+                drain_bar(smem_u32(&landed[box]), par);  // the copy may still land: let it
+                __syncwarp();
+                ok = false;
               }
-            for (int j = 0; j < a.nu; ++j)
-              if (!wait_unit(u + j)) ok = false;
+              uint8_t* buf = boxes + box * EPI_BUF;
+              uint4 raw[sizeof(T) == 2 ? 4 : 1];
+              if constexpr (sizeof(T) == 2) {  // rows of g and of dv differ in width: all of g first
 #pragma unroll
-            for (int cb = 0; cb < 2; ++cb)
-              if (cb < nch) {
-                const uint32_t ab = smem_u32(&aux[(warp - 8) * 2 + cb]);
-                const uint32_t par = (aux_phase >> cb) & 1u;
-                aux_phase ^= 1u << cb;
-                if (!wait_warp(ab, par, abort_flag, a.status)) {
-                  drain_bar(ab, par);  // the copy may still land: let it, before the buffer goes
-                  __syncwarp();
-                  ok = false;
-                }
-                uint8_t* buf = stage0 + cb * EPI_BUF;
-                uint4 raw[sizeof(T) == 2 ? 4 : 1];
-                if constexpr (sizeof(T) == 2) {  // rows of g and of dv differ in width: all of g first
-#pragma unroll
-                  for (int c = 0; c < 4; ++c) raw[c] = *reinterpret_cast<const uint4*>(buf + chunk_at<T>(lane, c));
-                  __syncwarp();
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  float v[16];
-                  tmem_ld<16>(lane_base + (uint32_t)((u % NACC) * BN + cb * 32 + h * 16), v);
-                  for (int j = 1; j < a.nu; ++j) {
-                    float v2[16];
-                    tmem_ld<16>(lane_base + (uint32_t)(((u + j) % NACC) * BN + cb * 32 + h * 16), v2);
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) v[c] += v2[c];
-                  }
-#pragma unroll
-                  for (int c4 = 0; c4 < 4; ++c4) {
-                    float4* at = reinterpret_cast<float4*>(buf + chunk_at<float>(lane, h * 4 + c4));
-                    float gv[4];
-                    if constexpr (sizeof(T) == 4) {
-                      const float4 t = *at;
-                      gv[0] = t.x, gv[1] = t.y, gv[2] = t.z, gv[3] = t.w;
-                    } else {
-                      const int e0 = h * 16 + c4 * 4;  // element of the row
-                      const uint4 t = raw[e0 / 8];
-                      const uint32_t lo = (e0 % 8) ? t.z : t.x, hi = (e0 % 8) ? t.w : t.y;
-                      gv[0] = __uint_as_float(lo << 16), gv[1] = __uint_as_float(lo & 0xFFFF0000u);
-                      gv[2] = __uint_as_float(hi << 16), gv[3] = __uint_as_float(hi & 0xFFFF0000u);
-                    }
-                    float o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                      const int c = cb * 32 + h * 16 + c4 * 4 + e;
-                      sum[c] += gv[e] * v[c4 * 4 + e];
-                      o[e] = gv[e] * (sa * gated_act<float>(a.act, z[c]));
-                    }
-                    *at = make_float4(o[0], o[1], o[2], o[3]);
-                  }
-                }
-                send(&mp.o, buf, col0 + cb * 32, row0, w.k0 + m);
+                for (int c = 0; c < 4; ++c) raw[c] = *reinterpret_cast<const uint4*>(buf + chunk_at<T>(lane, c));
+                __syncwarp();
               }
-            for (int j = 0; j < a.nu; ++j, ++u) free_unit(u);
-          }
-          if (!ok) break;
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          __syncwarp();
 #pragma unroll
-          for (int cb = 0; cb < 2; ++cb)
-            if (cb < nch) {
+              for (int h = 0; h < 2; ++h) {
+                float v[16];
+                load16(h * 16, v);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) sum[cb * 32 + c] *= sa * gated_dact<float>(a.act, z[cb * 32 + c]);
-              uint8_t* buf = stage0 + cb * EPI_BUF;
-              put_row<float>(buf, lane, sum + cb * 32);
-              send(&mp.o2, buf, col0 + cb * 32, row0, w.l);
+                for (int c4 = 0; c4 < 4; ++c4) {
+                  float4* at = reinterpret_cast<float4*>(buf + chunk_at<float>(lane, h * 4 + c4));
+                  float gv[4];
+                  if constexpr (sizeof(T) == 4) {
+                    const float4 t = *at;
+                    gv[0] = t.x, gv[1] = t.y, gv[2] = t.z, gv[3] = t.w;
+                  } else {
+                    const int e0 = h * 16 + c4 * 4;  // element of the row
+                    const uint4 t = raw[e0 / 8];
+                    const uint32_t lo = (e0 % 8) ? t.z : t.x, hi = (e0 % 8) ? t.w : t.y;
+                    gv[0] = __uint_as_float(lo << 16), gv[1] = __uint_as_float(lo & 0xFFFF0000u);
+                    gv[2] = __uint_as_float(hi << 16), gv[3] = __uint_as_float(hi & 0xFFFF0000u);
+                  }
+                  float o[4];
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) {
+                    const int c = h * 16 + c4 * 4 + e;
+                    sum[c] += gv[e] * v[c4 * 4 + e];
+                    o[e] = gv[e] * z[c];
+                  }
+                  *at = make_float4(o[0], o[1], o[2], o[3]);
+                }
+              }
+              if (m + 1 < w.nm && ok) {
+                boxes_free();  // the other box: its store is a component old
+                ask(m + 1, box ^ 1u);
+              }
+              send(&mp.o, buf, row0, w.k0 + m);
+              box ^= 1u;
             }
+            free_acc();
+          }
+          if (got < asked) {  // gave up: the box asked for may still land
+            drain_bar(smem_u32(&landed[box]), (box_phase >> box) & 1u);
+            __syncwarp();
+          }
+          if (ok && live) {
+            boxes_free();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float zz[16];
+              tmem_ld<16>(z_at + h * 16, zz);
+#pragma unroll
+              for (int c = 0; c < 16; ++c) sum[h * 16 + c] *= sa * fast_dact(a.act, zz[c]);
+            }
+            put_row<float>(boxes + box * EPI_BUF, lane, sum);
+            send(&mp.o2, boxes + box * EPI_BUF, row0, w.l);
+            box ^= 1u;
+          }
         }
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (elect_one()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
   }
   asm volatile("tcgen05.fence::before_thread_sync;");
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) fc_flag(a.status, FC_DEV_TIMEOUT);
   if (warp == 0) {
     asm volatile("tcgen05.fence::after_thread_sync;");
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
   }
-}
-
-// ---------------------------------------------------------------------------- weight gradients
-
-// Matrices 0 .. ranks-1: dWv_l (reduction over the 2l+1 components of n rows), ranks .. 2
-// ranks - 1: dWg_l (n rows). Each is cut into 128 x 128 output tiles ("jobs"), a job's
-// reduction into 32-row slabs; all slabs of all jobs form one line that the CTAs share out
-// equally. CTA i's part of job j has the partial matrix i + j of the workspace.
-struct WArgs {
-  int ranks, H, Cn;
-  int n_ht, n_ct;
-  int64_t blocks;      // 32-row blocks
-  int64_t width[8];    // slabs per job of a matrix
-  int skip;            // bit per matrix that is not wanted: its slabs keep their place on the
-                       // line, so what is wanted does not depend on what else is
-  int64_t total;       // slabs in all
-  int ctas;
-  float* part;         // partial matrices, 128 x 128 each
-  float* bias_part;    // partial bias gradients, 128 each (ct = 0 jobs of the gates), or null
-  int* status;
-};
-
-struct WMaps {
-  CUtensorMap dv, dz, x;  // (channel, row, component / rank), boxes of 128 channels x 32 rows
-};
-
-struct Job {
-  int mat, ht, ct;
-  int64_t index;        // job number
-  int64_t first, last;  // its slabs on the line
-};
-
-__host__ __device__ inline Job job_at(const WArgs& a, int64_t slab) {
-  Job j{0, 0, 0, 0, 0, 0};
-  const int tiles = a.n_ht * a.n_ct;
-  int64_t at = 0;
-  for (int mat = 0; mat < 2 * a.ranks; ++mat) {
-    const int64_t len = a.width[mat] * tiles;
-    if (slab < at + len) {
-      const int64_t t = (slab - at) / a.width[mat];
-      j.mat = mat;
-      j.ht = (int)(t / a.n_ct);
-      j.ct = (int)(t - (int64_t)j.ht * a.n_ct);
-      j.index = (int64_t)mat * tiles + t;
-      j.first = at + t * a.width[mat];
-      j.last = j.first + a.width[mat];
-      return j;
-    }
-    at += len;
-  }
-  return j;
-}
-__host__ __device__ inline int64_t cta_begin(const WArgs& a, int64_t i) { return i * a.total / a.ctas; }
-
-template <typename T>
-struct WCfg {
-  static constexpr bool X32 = sizeof(T) == 4;
-  static constexpr int TILE_D = 32 * BM * 4;         // raw dv / dz slab
-  static constexpr int TILE_X = 32 * BN * sizeof(T); // raw x slab
-  static constexpr int STAGE = TILE_D + TILE_X + (X32 ? 2 : 1) * TILE_B;
-  static constexpr int STAGES = X32 ? 3 : 4;
-  static constexpr int SMEM = STAGES * STAGE + BAR_BYTES + 1024;
-  static constexpr int NACC = 2, A_COLS = STAGES * 2 * BK;  // every stage has its A slot
-  static_assert(A_COLS + NACC * BN <= 512, "tensor memory");
-  static_assert(SMEM <= 227 * 1024, "shared memory per CTA");
-};
-
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 1) wgrad_kernel(const __grid_constant__ WMaps mp, const WArgs a) {
-  using C = WCfg<T>;
-  constexpr int S = C::STAGES, NACC = C::NACC, A_COLS = C::A_COLS;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * C::STAGE);
-  uint64_t* split = full + S;
-  uint64_t* empty = split + S;
-  uint64_t* acc_full = empty + S;
-  uint64_t* acc_empty = acc_full + NACC;
-  uint64_t* drain = acc_empty + NACC;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  // within a stage: the K-major B parts first (1024-byte aligned), then the raw slabs
-  constexpr int D_OFF = (C::X32 ? 2 : 1) * TILE_B, X_OFF = D_OFF + C::TILE_D;
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(512));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  if (threadIdx.x == 32) {
-    auto init = [](uint64_t* b, int n) {
-      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n));
-    };
-    for (int s = 0; s < S; ++s) {
-      init(&full[s], 1);
-      init(&split[s], 256);
-      init(&empty[s], 1);
-    }
-    for (int b = 0; b < NACC; ++b) {
-      init(&acc_full[b], 1);
-      init(&acc_empty[b], 4);
-    }
-    init(drain, 1);
-    *abort_flag = 0;
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;");
-  __syncthreads();
-  asm volatile("tcgen05.fence::after_thread_sync;");
-  const uint32_t tmem = *tmem_slot;
-  const int64_t begin = cta_begin(a, blockIdx.x), end = cta_begin(a, blockIdx.x + 1);
-
-  if (warp < 4) {
-    FC_SETMAXNREG_DEC(56);
-    if (warp == 0 && lane == 0) {
-      // ---------------------------------------------------------------- TMA producer
-      int64_t g = 0;
-      bool ok = true;
-      for (int64_t p = begin; p < end && ok;) {
-        const Job j = job_at(a, p);
-        const bool gates = j.mat >= a.ranks;
-        const int l = gates ? j.mat - a.ranks : j.mat, w = gates ? 1 : 2 * l + 1;
-        const int64_t stop = min(end, j.last);
-        if (a.skip >> j.mat & 1) {
-          p = stop;
-          continue;
-        }
-        for (; p < stop; ++p, ++g) {
-          const int s = (int)(g % S);
-          if (g >= S && !wait_parity(smem_u32(&empty[s]), (uint32_t)(((g / S) - 1) & 1), abort_flag, a.status)) {
-            ok = false;
-            break;
-          }
-          // rows of a node block one component after the other: they share DRAM pages
-          const int64_t r = p - j.first, nb = r / w;
-          const int m = (int)(r - nb * w);
-          uint8_t* st = smem + s * C::STAGE;
-          const uint32_t fb = smem_u32(&full[s]);
-          arrive_tx(fb, C::TILE_D + C::TILE_X);
-          tma_load_3d(smem_u32(st + D_OFF), gates ? &mp.dz : &mp.dv, j.ht * BM, (int)(nb * 32), gates ? l : l * l + m,
-                      fb);
-          tma_load_3d(smem_u32(st + X_OFF), &mp.x, j.ct * BN, (int)(nb * 32), gates ? 0 : l * l + m, fb);
-        }
-      }
-      for (int s = 0; s < S; ++s) {
-        const int64_t uses = g > s ? (g - 1 - s) / S + 1 : 0;
-        if (uses > 0) drain_bar(smem_u32(&full[s]), (uint32_t)((uses - 1) & 1));
-      }
-    } else if (warp == 1 && lane == 0) {
-      // ---------------------------------------------------------------- MMA issue
-      int64_t g = 0, u = 0;
-      bool ok = true;
-      for (int64_t p = begin; p < end && ok;) {
-        const Job j = job_at(a, p);
-        const int64_t stop = min(end, j.last);
-        if (a.skip >> j.mat & 1) p = stop;
-        while (p < stop && ok) {
-          const int b = (int)(u % NACC);
-          const int64_t v = u / NACC;
-          if (v >= 1 && !wait_parity(smem_u32(&acc_empty[b]), (uint32_t)((v - 1) & 1), abort_flag, a.status)) {
-            ok = false;
-            break;
-          }
-          asm volatile("tcgen05.fence::after_thread_sync;");
-          const uint32_t d = tmem + (uint32_t)(A_COLS + b * BN);
-          const int64_t unit = min(stop, p + KG);
-          bool fresh = true;
-          for (; p < unit; ++p, ++g) {
-            const int s = (int)(g % S);
-            if (!wait_parity(smem_u32(&split[s]), (uint32_t)((g / S) & 1), abort_flag, a.status)) {
-              ok = false;
-              break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;");
-            uint8_t* st = smem + s * C::STAGE;
-            const uint64_t dbh = make_desc(smem_u32(st)), dbl = make_desc(smem_u32(st + TILE_B));
-            const uint32_t tah = tmem + (uint32_t)(s * 2 * BK), tal = tah + (uint32_t)BK;
-#pragma unroll
-            for (int kk = 0; kk < BK / 8; ++kk) {
-              const uint64_t off = (uint64_t)((kk * 32) >> 4);
-              mma_ta<BN>(d, tal + kk * 8, dbh + off, fresh && kk == 0 ? 0u : 1u);
-              if (C::X32) mma_ta<BN>(d, tah + kk * 8, dbl + off, 1u);
-            }
-#pragma unroll
-            for (int kk = 0; kk < BK / 8; ++kk) mma_ta<BN>(d, tah + kk * 8, dbh + (uint64_t)((kk * 32) >> 4), 1u);
-            fresh = false;
-            commit(smem_u32(&empty[s]));
-          }
-          if (ok) {
-            commit(smem_u32(&acc_full[b]));
-            ++u;
-          }
-        }
-      }
-      commit(smem_u32(drain));
-      drain_bar(smem_u32(drain), 0);
-    }
-  } else if (warp < 12) {
-    FC_SETMAXNREG_DEC(112);
-    // ------------------------------------------------------------------ splitters
-    const bool of_d = warp < 8;               // dv / dz into tensor memory, or x into K-major rows
-    const int c = (warp & 3) * 32 + lane;     // channel: lane of tensor memory, or row of the B tile
-    int64_t g = 0;
-    bool ok = true;
-    for (int64_t p = begin; p < end && ok;) {
-      const Job j = job_at(a, p);
-      const int64_t stop = min(end, j.last);
-      if (a.skip >> j.mat & 1) {
-        p = stop;
-        continue;
-      }
-      const bool bias = of_d && a.bias_part && j.mat >= a.ranks && j.ct == 0;
-      float bsum = 0.f;
-      for (; p < stop; ++p, ++g) {
-        const int s = (int)(g % S);
-        if (!wait_warp(smem_u32(&full[s]), (uint32_t)((g / S) & 1), abort_flag, a.status)) {
-          ok = false;
-          break;
-        }
-        uint8_t* st = smem + s * C::STAGE;
-        float x[32];
-        if (of_d) {
-          const float* raw = reinterpret_cast<const float*>(st + D_OFF) + c;
-#pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = raw[k * BM];
-          if (bias) {
-            float t = 0.f;  // a slab's sum first: fewer roundings against the running sum
-#pragma unroll
-            for (int k = 0; k < 32; ++k) t += x[k];
-            bsum += t;
-          }
-          store_parts<true>(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(s * 2 * BK), x);
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        } else {
-          const T* raw = reinterpret_cast<const T*>(st + X_OFF) + c;
-#pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = Io<T>::get(raw[k * BN]);
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            float h[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = C::X32 ? round_tf32(x[4 * q + e]) : x[4 * q + e];
-            *reinterpret_cast<float4*>(st + chunk_at<float>(c, q)) = make_float4(h[0], h[1], h[2], h[3]);
-            if (C::X32) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) h[e] = round_tf32(x[4 * q + e] - h[e]);
-              *reinterpret_cast<float4*>(st + TILE_B + chunk_at<float>(c, q)) = make_float4(h[0], h[1], h[2], h[3]);
-            }
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        }
-        arrive(smem_u32(&split[s]));
-      }
-      if (bias && ok) a.bias_part[(blockIdx.x + j.index) * BM + c] = bsum;
-    }
-  } else {
-    FC_SETMAXNREG_INC(216);
-    // ------------------------------------------------------------------ epilogue: unit sums
-    const int quarter = warp & 3;
-    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)A_COLS;
-    int64_t u = 0;
-    bool ok = true;
-    for (int64_t p = begin; p < end && ok;) {
-      const Job j = job_at(a, p);
-      const int64_t stop = min(end, j.last);
-      if (a.skip >> j.mat & 1) {
-        p = stop;
-        continue;
-      }
-      float acc[BN];
-#pragma unroll
-      for (int c = 0; c < BN; ++c) acc[c] = 0.f;
-      for (; p < stop; p += KG, ++u) {
-        const int b = (int)(u % NACC);
-        if (!wait_warp(smem_u32(&acc_full[b]), (uint32_t)((u / NACC) & 1), abort_flag, a.status)) {
-          ok = false;
-          break;
-        }
-        asm volatile("tcgen05.fence::after_thread_sync;");
-#pragma unroll
-        for (int cb = 0; cb < BN / 32; ++cb) {
-          float f[32];
-          tmem_ld<32>(lane_base + (uint32_t)(b * BN + cb * 32), f);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) acc[cb * 32 + c] += f[c];
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;");
-        __syncwarp();
-        if (lane == 0) arrive(smem_u32(&acc_empty[b]));
-      }
-      p = stop;
-      if (!ok) break;
-      float4* out = reinterpret_cast<float4*>(a.part + ((blockIdx.x + j.index) * BM + quarter * 32 + lane) * BN);
-#pragma unroll
-      for (int c = 0; c < BN / 4; ++c)
-        out[c] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
-    }
-  }
-  asm volatile("tcgen05.fence::before_thread_sync;");
-  __syncthreads();
-  if (warp == 0) {
-    asm volatile("tcgen05.fence::after_thread_sync;");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
-  }
-}
-
-struct WOut {
-  void* w[8];     // gradient of each matrix (gates: rows l H .. of one matrix), or null
-  void* bias;     // ((ranks) H) or null
-  const float* scales;
-};
-
-// Partial matrices added in the order of the CTAs. One block per 8 rows of a job's tile; the
-// bias by the blocks of the ct = 0 gate jobs.
-template <typename T>
-__global__ void __launch_bounds__(256) wgrad_sum_kernel(const WArgs a, const WOut o) {
-  const int tiles = a.n_ht * a.n_ct;
-  const int64_t job = blockIdx.x / (BM / 8);
-  const int row = (int)(blockIdx.x % (BM / 8)) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int mat = (int)(job / tiles), t = (int)(job % tiles);
-  const int64_t width = a.width[mat];
-  const int h = (t / a.n_ct) * BM + row, c = (t % a.n_ct) * BN + lane * 4;
-  const bool gates = mat >= a.ranks;
-  const bool bias = gates && o.bias && t % a.n_ct == 0 && (threadIdx.x & 31) == 0;
-  if (h >= a.H || (!o.w[mat] && !bias)) return;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  float bsum = 0.f;
-  if (width > 0 && a.total > 0) {
-    int64_t first = 0;
-    for (int m = 0; m < mat; ++m) first += a.width[m] * tiles;
-    first += t * width;
-    int64_t i0 = first * a.ctas / a.total;
-    while (i0 > 0 && cta_begin(a, i0) > first) --i0;
-    while (i0 + 1 < a.ctas && cta_begin(a, i0 + 1) <= first) ++i0;
-#pragma unroll 4
-    for (int64_t i = i0; i < a.ctas; ++i) {
-      if (cta_begin(a, i) >= first + width) break;
-      const float4 v = *reinterpret_cast<const float4*>(a.part + ((i + job) * BM + row) * BN + lane * 4);
-      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-      if (bias) bsum += a.bias_part[(i + job) * BM + row];
-    }
-  }
-  const int l = gates ? mat - a.ranks : mat;
-  const float sc = o.scales[gates ? a.ranks : l];
-  if (o.w[mat]) {
-    T* out = (T*)o.w[mat] + ((int64_t)(gates ? l * a.H : 0) + h) * a.Cn + c;
-    const float v[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (c + e < a.Cn) out[e] = Io<T>::put(sc * v[e]);
-  }
-  if (bias) ((T*)o.bias)[(int64_t)l * a.H + h] = Io<T>::put(bsum);
 }
 
 // ---------------------------------------------------------------------------- operand layouts
+
+constexpr int MAX_LISTS = 160;  // work lists of a launch: one per 64 output channels
 
 // Scaled weights as tf32 hi | lo parts: matrix q (values 0 .. ranks-1, then gates) at q, its
 // low part 2 ranks matrices behind; (out, k) rows of kp elements, zero behind K. fwd: out =
@@ -1014,7 +686,8 @@ struct PrepArgs {
 
 template <typename T>
 __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs p) {
-  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 4) p.counters[threadIdx.x] = 0;
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < 2 * MAX_LISTS; i += 256) p.counters[i] = 0;
   const int ranks = p.g.L + 1, q = blockIdx.y, l = q < ranks ? q : q - ranks, C = p.g.C, H = p.g.H;
   const T* w = q < ranks ? (const T*)p.g.wv[l] : (const T*)p.g.wg + (int64_t)l * H * C;
   const float sc = ((const float*)p.g.scales)[q < ranks ? l : ranks];
@@ -1059,10 +732,8 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// (channel, row, component) map of a tensor of rows [comps][ld]; box_c channels x box_r rows.
-// swizzled: 32-channel boxes with the 128- or 64-byte swizzle of their row width.
 template <typename E>
-static bool encode_rows(CUtensorMap* map, const void* base, int64_t channels, int64_t rows, int64_t comps, int64_t ld,
+bool encode_rows(CUtensorMap* map, const void* base, int64_t channels, int64_t rows, int64_t comps, int64_t ld,
                         int box_c, int box_r) {
   const cuuint64_t dims[3] = {(cuuint64_t)channels, (cuuint64_t)rows, (cuuint64_t)comps};
   const cuuint64_t strides[2] = {(cuuint64_t)(comps * ld) * sizeof(E), (cuuint64_t)ld * sizeof(E)};
@@ -1076,10 +747,13 @@ static bool encode_rows(CUtensorMap* map, const void* base, int64_t channels, in
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static bool encode_weights(CUtensorMap* map, const float* base, int kp, int out, int mats) {
+template bool encode_rows<float>(CUtensorMap*, const void*, int64_t, int64_t, int64_t, int64_t, int, int);
+template bool encode_rows<bf16_t>(CUtensorMap*, const void*, int64_t, int64_t, int64_t, int64_t, int, int);
+
+static bool encode_weights(CUtensorMap* map, const float* base, int kp, int out, int mats, int box_rows) {
   const cuuint64_t dims[3] = {(cuuint64_t)kp, (cuuint64_t)out, (cuuint64_t)mats};
   const cuuint64_t strides[2] = {(cuuint64_t)kp * 4, (cuuint64_t)kp * out * 4};
-  const cuuint32_t box[3] = {32, BN, 1};
+  const cuuint32_t box[3] = {32, (cuuint32_t)box_rows, 1};
   const cuuint32_t unit[3] = {1, 1, 1};
   return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims, strides, box, unit,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -1094,32 +768,18 @@ static int sm_count() {
   return sms[dev];
 }
 
-// Shared-memory size, and the registers that setmaxnreg shares out: the block must be launched
-// with 128 per thread (its roles' shares add up to exactly that).
-struct Ready {
-  bool done[64] = {};
-};
-template <typename K>
-static int ready(K kernel, int smem, Ready& r) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return FC_ERR_LAUNCH;
-  if (r.done[dev]) return 0;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return FC_ERR_LAUNCH;
-  cudaFuncAttributes at;
-  if (cudaFuncGetAttributes(&at, kernel) != cudaSuccess) return FC_ERR_LAUNCH;
-  if (at.numRegs != 128) return FC_ERR_UNSUPPORTED;
-  r.done[dev] = true;
-  return 0;
-}
+// Whether the products of a reduction over K into N columns keep their weights in shared memory.
+static bool resident(int K, int N, int sms) { return K <= MAX_NK * BK && (N + BN - 1) / BN <= std::min(sms, MAX_LISTS); }
 
 template <int MODE, typename T>
-static int run_products(const Maps& mp, const Args& args, cudaStream_t s) {
-  constexpr int smem = Cfg<MODE, T>::SMEM;
+static int run_products(const Maps& mp, Args a, int K, int sms, cudaStream_t s) {
+  if (!resident(K, a.N, sms)) return run_stream<MODE, T>(mp, a, sms, s);
+  using C = Cfg<MODE, T>;
+  a.stages = C::stages(a.nk);
   static Ready state;
-  if (int rc = ready(gated_tc_kernel<MODE, T>, smem, state)) return rc;
-  const int grid = (int)std::min<int64_t>(args.items, sm_count());
-  gated_tc_kernel<MODE, T><<<grid, THREADS, smem, s>>>(mp, args);
+  if (int rc = ready(gated_tc_kernel<MODE, T>, SMEM_MAX, state, TC_REGS)) return rc;
+  const int lists = (int)std::min<int64_t>(a.items, sms / a.n_ct);
+  gated_tc_kernel<MODE, T><<<lists * a.n_ct, TC_THREADS, C::smem(a.nk, a.stages), s>>>(mp, a);
   return fc_check_launch();
 }
 
@@ -1139,15 +799,15 @@ static Ws layout(int L, int C, int H, int64_t n, int esize, bool backward, int s
     at += (bytes + 127) / 128 * 128;
     return p;
   };
-  w.counters = take(16);
+  w.counters = take(2 * MAX_LISTS * 4);
   w.fwd = take(4 * ranks * H * cp * 4);
   if (backward) {
-    const int64_t jobs = 2 * ranks * ((H + BM - 1) / BM) * ((C + BN - 1) / BN);
+    const int64_t parts = wgrad_part_count((int)ranks, C, H, sms);
     w.dx = take(4 * ranks * C * hp * 4);
     w.dv = take(n * comps * hp * 4);
     w.dz = take(n * ranks * hp * 4);
-    w.part = take((sms + jobs) * BM * BN * 4);
-    w.bias = take((sms + jobs) * BM * 4);
+    w.part = take(parts * BM * BM * 4);
+    w.bias = take(parts * BM * 4);
   }
   // copies with 16-byte rows, used where the caller's rows are not (or are misaligned)
   w.x = take(n * comps * ce * esize);
@@ -1179,32 +839,37 @@ static int repitch(const T* src, int64_t src_ld, T* dst, int64_t dst_ld, int wid
   return fc_check_launch();
 }
 
-static Args product_args(const GatedArgs& g, int N, int K, int n_items_cols, int mode, int sms) {
+static Args product_args(const GatedArgs& g, int N, int K, int mode, int sms) {
   Args a{};
   a.L = g.L;
   a.ranks = g.L + 1;
   a.comps = a.ranks * a.ranks;
   a.N = N;
   a.nk = (K + BK - 1) / BK;
-  // PRE holds a component's accumulators until its epilogue is done, so all its units have to
-  // fit the ring; the others add units of 64 products in registers
-  a.kg = mode == PRE ? std::max(KG, (a.nk + NACC - 1) / NACC) : KG;
-  a.nu = (a.nk + a.kg - 1) / a.kg;
-  a.n_ct = n_items_cols;
   a.tiles = (int)((g.n + BM - 1) / BM);
+  const bool res = resident(K, N, sms);
+  a.n_ct = res ? (N + BN - 1) / BN : (N + STREAM_BN - 1) / STREAM_BN;
   // with fewer (tile, rank) groups than SMs the components are items of their own (the gate is
   // computed again for each); PRE needs a rank's components together
-  const int64_t groups = (int64_t)a.tiles * a.ranks * a.n_ct;
-  a.per_comp = mode == DX || (mode == FWD && groups < sms);
-  a.items = (int64_t)a.tiles * a.n_ct * (a.per_comp ? a.comps : a.ranks);
-  const int tail = (2 * sms + a.ranks * a.n_ct - 1) / (a.ranks * a.n_ct);
-  a.main_tiles = std::max(0, a.tiles - tail);
+  a.per_comp = (mode == DX && !res) || (mode != PRE && (int64_t)a.tiles * a.ranks * a.n_ct < sms);
+  a.items = (int64_t)a.tiles * (a.per_comp ? a.comps : a.ranks);
+  if (!res) {
+    a.items *= a.n_ct;
+    // PRE holds a component's accumulators until its epilogue is done, so all its units have
+    // to fit the ring; the others add units of 64 products in registers
+    a.kg = mode == PRE ? std::max(STREAM_KG, (a.nk + STREAM_NACC - 1) / STREAM_NACC) : STREAM_KG;
+    a.nu = (a.nk + a.kg - 1) / a.kg;
+    const int tail = (2 * sms + a.ranks * a.n_ct - 1) / (a.ranks * a.n_ct);
+    a.main_tiles = std::max(0, a.tiles - tail);
+  }
   a.act = g.act;
   a.bias = g.bias;
   a.act_scale = (const float*)g.scales + a.ranks + 1;
   a.status = g.status;
   return a;
 }
+
+static int weight_rows(int K, int N, int sms) { return resident(K, N, sms) ? BN : STREAM_BN; }
 
 template <typename T>
 static int run_prep(const GatedArgs& g, float* fwd, float* dx, int* counters, cudaStream_t s) {
@@ -1235,15 +900,15 @@ int gated_tc_fwd(const GatedArgs& a, cudaStream_t s) {
   int* counters = (int*)(ws + w.counters);
   float* weights = (float*)(ws + w.fwd);
   if (int rc = run_prep<T>(a, weights, nullptr, counters, s)) return rc;
-  Args args = product_args(a, a.H, a.C, (a.H + BN - 1) / BN, FWD, sms);
+  Args args = product_args(a, a.H, a.C, FWD, sms);
   args.counter = counters;
   Maps mp;
   if (!encode_rows<T>(&mp.a, x.p, a.C, a.n, comps, x.ld, BK, BM) ||
-      !encode_weights(&mp.b, weights, (a.C + 3) & ~3, a.H, 4 * ranks) ||
+      !encode_weights(&mp.b, weights, (a.C + 3) & ~3, a.H, 4 * ranks, weight_rows(a.C, a.H, sms)) ||
       !encode_rows<T>(&mp.o, y.p, a.H, a.n, comps, y.ld, 32, 32))
     return FC_ERR_UNSUPPORTED;
-  mp.a2 = mp.g = mp.o2 = mp.o;  // not used
-  if (int rc = run_products<FWD, T>(mp, args, s)) return rc;
+  mp.a2 = mp.ap = mp.g = mp.gp = mp.o2 = mp.o;  // not used
+  if (int rc = run_products<FWD, T>(mp, args, a.C, sms, s)) return rc;
   if (y.copied) return repitch<T>(y.p, y.ld, (T*)a.y, a.H, a.H, a.n * comps, s);
   return 0;
 }
@@ -1261,24 +926,7 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
   int* counters = (int*)(ws + w.counters);
   float *fwd = (float*)(ws + w.fwd), *dx = (float*)(ws + w.dx), *dv = (float*)(ws + w.dv), *dz = (float*)(ws + w.dz);
   bool any = a.gwg || a.gbias;
-  WArgs wa{};
-  wa.ranks = ranks;
-  wa.H = a.H;
-  wa.Cn = a.C;
-  wa.n_ht = (a.H + BM - 1) / BM;
-  wa.n_ct = (a.C + BN - 1) / BN;
-  wa.blocks = (a.n + 31) / 32;
-  for (int l = 0; l < ranks; ++l) {
-    wa.width[l] = wa.blocks * (2 * l + 1);
-    wa.width[ranks + l] = wa.blocks;
-    if (!a.gwv[l]) wa.skip |= 1 << l;
-    if (!a.gwg && !a.gbias) wa.skip |= 1 << (ranks + l);
-    wa.total += (wa.width[l] + wa.width[ranks + l]) * wa.n_ht * wa.n_ct;
-    any = any || a.gwv[l];
-  }
-  wa.part = (float*)(ws + w.part);
-  wa.bias_part = a.gbias ? (float*)(ws + w.bias) : nullptr;
-  wa.status = a.status;
+  for (int l = 0; l < ranks; ++l) any = any || a.gwv[l];
   if (a.n > 0) {
     if (x.copied)
       if (int rc = repitch<T>((const T*)a.x, a.C, const_cast<T*>(x.p), x.ld, a.C, a.n * comps, s)) return rc;
@@ -1287,46 +935,34 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
     if (int rc = run_prep<T>(a, fwd, a.gx ? dx : nullptr, counters, s)) return rc;
     Maps mp;
     if (!encode_rows<T>(&mp.a, x.p, a.C, a.n, comps, x.ld, BK, BM) ||
-        !encode_weights(&mp.b, fwd, (a.C + 3) & ~3, a.H, 4 * ranks) ||
+        !encode_weights(&mp.b, fwd, (a.C + 3) & ~3, a.H, 4 * ranks, weight_rows(a.C, a.H, sms)) ||
         !encode_rows<float>(&mp.o, dv, a.H, a.n, comps, hp, 32, 32) ||
         !encode_rows<T>(&mp.g, gy.p, a.H, a.n, comps, gy.ld, 32, 32) ||
+        !encode_rows<T>(&mp.gp, gy.p, a.H, a.n, comps, gy.ld, BN, BM) ||
+        !encode_rows<T>(&mp.ap, x.p, a.C, a.n, comps, x.ld, MAX_NK * BK, BM) ||
         !encode_rows<float>(&mp.o2, dz, a.H, a.n, ranks, hp, 32, 32))
       return FC_ERR_UNSUPPORTED;
     mp.a2 = mp.o2;  // not used
-    Args args = product_args(a, a.H, a.C, (a.H + BN - 1) / BN, PRE, sms);
+    Args args = product_args(a, a.H, a.C, PRE, sms);
     args.counter = counters;
-    if (int rc = run_products<PRE, T>(mp, args, s)) return rc;
+    if (int rc = run_products<PRE, T>(mp, args, a.C, sms, s)) return rc;
     if (a.gx) {
       const Rows<T> gx = rows_of<T>(a.gx, a.C, ws + w.gx);
       Maps md;
       if (!encode_rows<float>(&md.a, dv, a.H, a.n, comps, hp, BK, BM) ||
           !encode_rows<float>(&md.a2, dz, a.H, a.n, ranks, hp, BK, BM) ||
-          !encode_weights(&md.b, dx, (int)hp, a.C, 4 * ranks) ||
+          !encode_weights(&md.b, dx, (int)hp, a.C, 4 * ranks, weight_rows(a.H, a.C, sms)) ||
           !encode_rows<T>(&md.o, gx.p, a.C, a.n, comps, gx.ld, 32, 32))
         return FC_ERR_UNSUPPORTED;
-      md.g = md.o2 = md.o;  // not used
-      Args dargs = product_args(a, a.C, a.H, (a.C + BN - 1) / BN, DX, sms);
-      dargs.counter = counters + 1;
-      if (int rc = run_products<DX, T>(md, dargs, s)) return rc;
+      md.ap = md.g = md.gp = md.o2 = md.o;  // not used
+      Args dargs = product_args(a, a.C, a.H, DX, sms);
+      dargs.counter = counters + MAX_LISTS;
+      if (int rc = run_products<DX, T>(md, dargs, a.H, sms, s)) return rc;
       if (gx.copied)
         if (int rc = repitch<T>(gx.p, gx.ld, (T*)a.gx, a.C, a.C, a.n * comps, s)) return rc;
     }
   }
   if (!any) return 0;
-  if (wa.total > 0) {
-    // at least four slabs per CTA: a partial matrix costs 128 KB of traffic
-    wa.ctas = (int)std::min<int64_t>(sms, (wa.total + 3) / 4);
-    WMaps wm;
-    if (!encode_rows<float>(&wm.dv, dv, a.H, a.n, comps, hp, BM, 32) ||
-        !encode_rows<float>(&wm.dz, dz, a.H, a.n, ranks, hp, BM, 32) ||
-        !encode_rows<T>(&wm.x, x.p, a.C, a.n, comps, x.ld, BN, 32))
-      return FC_ERR_UNSUPPORTED;
-    constexpr int smem = WCfg<T>::SMEM;
-    static Ready state;
-    if (int rc = ready(wgrad_kernel<T>, smem, state)) return rc;
-    wgrad_kernel<T><<<wa.ctas, THREADS, smem, s>>>(wm, wa);
-    if (int rc = fc_check_launch()) return rc;
-  }
   WOut o{};
   for (int l = 0; l < ranks; ++l) {
     o.w[l] = a.gwv[l];
@@ -1334,9 +970,8 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
   }
   o.bias = a.gbias;
   o.scales = (const float*)a.scales;
-  if (wa.ctas == 0) wa.ctas = 1;
-  wgrad_sum_kernel<T><<<(unsigned)(2 * ranks * wa.n_ht * wa.n_ct * (BM / 8)), 256, 0, s>>>(wa, o);
-  return fc_check_launch();
+  return run_wgrad<T>(ranks, a.C, a.H, a.n, dv, dz, hp, x.p, x.ld, (float*)(ws + w.part), (float*)(ws + w.bias), o,
+                      a.status, sms, s);
 }
 
 template int gated_tc_fwd<float>(const GatedArgs&, cudaStream_t);
