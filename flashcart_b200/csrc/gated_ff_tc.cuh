@@ -196,13 +196,13 @@ __device__ __forceinline__ void put_row(uint8_t* buf, int r, const float* f) {
 
 // sigma(z) by the hardware's base-2 exponential and reciprocal. The exponent -z log2(e) is
 // formed as a float and its remainder, 2^(t + r) = 2^t (1 + r ln 2), so its rounding does not
-// grow with |z|; 0 and 1 beyond the exponential's range.
+// grow with |z|; the power stays finite (the reciprocal of 2^127 is taken as 0). NaN stays NaN.
 __device__ __forceinline__ float fast_sigmoid(float z) {
   const float hi = 1.44269502f, lo = 1.92596303e-8f;  // log2(e)
   const float t = -z * hi;
   const float r = fmaf(-z, hi, -t) - z * lo;
   float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t > 127.f ? 127.f : t));
   e = fabsf(z) < 1e30f ? fmaf(e, r * 0.693147181f, e) : e;  // (r is NaN for infinite z)
   return __fdividef(1.f, 1.f + e);
 }
