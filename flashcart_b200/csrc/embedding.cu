@@ -431,9 +431,10 @@ static SumPlan sum_plan(int64_t R, int64_t D, bool vec) {
   p.lanes = 1;
   while (p.lanes < 32 && (int64_t)p.lanes * p.per < D) p.lanes *= 2;
   p.col_tiles = (int)((D + (int64_t)p.lanes * p.per - 1) / ((int64_t)p.lanes * p.per));
-  // chunks just long enough that all lane groups together fill the GPU (148 SMs x 2048
-  // threads) once: shorter ones write and re-read more partial sums, longer ones idle lanes
-  const int64_t fill = R * p.lanes * p.col_tiles / (148 * 2048);
+  // chunks just long enough that the lane groups together are 512 threads per SM, which with
+  // eight rows in flight each cover the memory latency: shorter chunks write and re-read more
+  // partial sums, longer ones leave too few loads in flight
+  const int64_t fill = R * p.lanes * p.col_tiles / (148 * 512);
   p.Lc = (int)(fill < 16 ? 16 : fill > 256 ? 256 : (fill + 7) / 8 * 8);
   p.chunks = (R + p.Lc - 1) / p.Lc;
   p.Dp = (D + 7) / 8 * 8;

@@ -322,37 +322,57 @@ __global__ void __launch_bounds__(THREADS, 1) wgrad_kernel(const __grid_constant
   }
 }
 
-// Partial matrices added in the order of the CTAs. One block per 8 rows of a job's tile; the
-// bias by the blocks of the ct = 0 gate jobs.
+// Partial matrices added in the order of the CTAs. A block takes four rows of a job's tile: its
+// warps 4 r + p add every fourth partial of row r from the p-th on, and the four sums are added
+// in order. The bias goes with the ct = 0 gate jobs.
+constexpr int SUM_ROWS = 4, SUM_PARTS = 4;
 template <typename T>
-__global__ void __launch_bounds__(256) wgrad_sum_kernel(const WArgs a, const WOut o) {
+__global__ void __launch_bounds__(SUM_ROWS * SUM_PARTS * 32) wgrad_sum_kernel(const WArgs a, const WOut o) {
+  __shared__ float4 red[SUM_ROWS][SUM_PARTS][32];
+  __shared__ float bred[SUM_ROWS][SUM_PARTS];
   const int tiles = a.n_ht * a.n_ct;
-  const int64_t job = blockIdx.x / (BM / 8);
-  const int row = (int)(blockIdx.x % (BM / 8)) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int mat = (int)(job / tiles), t = (int)(job % tiles);
-  const int64_t width = a.width[mat];
-  const int h = (t / a.n_ct) * BM + row, c = (t % a.n_ct) * BN + lane * 4;
+  const int job = (int)(blockIdx.x / (BM / SUM_ROWS)), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int rr = warp / SUM_PARTS, part = warp % SUM_PARTS;
+  const int row = (int)(blockIdx.x % (BM / SUM_ROWS)) * SUM_ROWS + rr;
+  const int mat = job / tiles, t = job - mat * tiles, ht = t / a.n_ct, ct = t - ht * a.n_ct;
   const bool gates = mat >= a.ranks;
-  const bool bias = gates && o.bias && t % a.n_ct == 0 && (threadIdx.x & 31) == 0;
-  if (h >= a.H || (!o.w[mat] && !bias)) return;
+  const int l = gates ? mat - a.ranks : mat;
+  const int h = ht * BM + row, c = ct * BN + lane * 4;
+  const bool bias = gates && o.bias && ct == 0;
+  if (ht * BM + (int)(blockIdx.x % (BM / SUM_ROWS)) * SUM_ROWS >= a.H || (!o.w[mat] && !bias)) return;  // whole block
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
   float bsum = 0.f;
-  if (width > 0 && a.total > 0) {
+  if (a.total > 0) {
+    // the CTAs whose share [i total / ctas, (i + 1) total / ctas) meets the job's slabs
     int64_t first = 0;
     for (int m = 0; m < mat; ++m) first += a.width[m] * tiles;
-    first += t * width;
-    int64_t i0 = first * a.ctas / a.total;
+    const int64_t last = first + (t + 1) * a.width[mat];
+    first += t * a.width[mat];
+    int64_t i0 = first * a.ctas / a.total, i1 = last * a.ctas / a.total;
     while (i0 > 0 && cta_begin(a, i0) > first) --i0;
     while (i0 + 1 < a.ctas && cta_begin(a, i0 + 1) <= first) ++i0;
-#pragma unroll 4
-    for (int64_t i = i0; i < a.ctas; ++i) {
-      if (cta_begin(a, i) >= first + width) break;
-      const float4 v = *reinterpret_cast<const float4*>(a.part + ((i + job) * BM + row) * BN + lane * 4);
+    while (i1 > i0 && cta_begin(a, i1) >= last) --i1;
+    if (i1 >= a.ctas) i1 = a.ctas - 1;
+    const float* p = a.part + ((i0 + part + job) * BM + row) * BN + lane * 4;
+    const float* q = a.bias_part + (i0 + part + job) * BM + row;
+    const int n = (int)(i1 - i0) - part;
+#pragma unroll 8
+    for (int i = 0; i <= n; i += SUM_PARTS) {
+      const float4 v = *reinterpret_cast<const float4*>(p + (int64_t)i * BM * BN);
       sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-      if (bias) bsum += a.bias_part[(i + job) * BM + row];
     }
+    if (bias && lane == 0)
+      for (int i = 0; i <= n; i += SUM_PARTS) bsum += q[(int64_t)i * BM];
   }
-  const int l = gates ? mat - a.ranks : mat;
+  red[rr][part][lane] = sum;
+  if (lane == 0) bred[rr][part] = bsum;
+  __syncthreads();
+  if (part != 0 || h >= a.H) return;
+  for (int k = 1; k < SUM_PARTS; ++k) {
+    const float4 v = red[rr][k][lane];
+    sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    bsum += bred[rr][k];
+  }
   const float sc = o.scales[gates ? a.ranks : l];
   if (o.w[mat]) {
     T* out = (T*)o.w[mat] + ((int64_t)(gates ? l * a.H : 0) + h) * a.Cn + c;
@@ -361,7 +381,7 @@ __global__ void __launch_bounds__(256) wgrad_sum_kernel(const WArgs a, const WOu
     for (int e = 0; e < 4; ++e)
       if (c + e < a.Cn) out[e] = Io<T>::put(sc * v[e]);
   }
-  if (bias) ((T*)o.bias)[(int64_t)l * a.H + h] = Io<T>::put(bsum);
+  if (bias && lane == 0) ((T*)o.bias)[(int64_t)l * a.H + h] = Io<T>::put(bsum);
 }
 
 int64_t wgrad_part_count(int ranks, int C, int H, int sms) {
@@ -404,7 +424,8 @@ int run_wgrad(int ranks, int C, int H, int64_t n, const float* dv, const float* 
     wgrad_kernel<T><<<wa.ctas, THREADS, smem, s>>>(wm, wa);
     if (int rc = fc_check_launch()) return rc;
   }
-  wgrad_sum_kernel<T><<<(unsigned)(2 * ranks * wa.n_ht * wa.n_ct * (BM / 8)), 256, 0, s>>>(wa, o);
+  wgrad_sum_kernel<T><<<(unsigned)(2 * ranks * wa.n_ht * wa.n_ct * (BM / SUM_ROWS)), SUM_ROWS * SUM_PARTS * 32, 0,
+                        s>>>(wa, o);
   return fc_check_launch();
 }
 template int run_wgrad<float>(int, int, int, int64_t, const float*, const float*, int64_t, const float*, int64_t, float*,
