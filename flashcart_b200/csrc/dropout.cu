@@ -94,6 +94,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, c
   constexpr int NV = sizeof(T) == 8 ? 2 : 4, PARTS = 4 / NV;  // a 64-bit quad is two 16-byte vectors
   for (I u0 = (I)blockIdx.x * (256 * UN) + threadIdx.x; u0 < total; u0 += (I)gridDim.x * (256 * UN)) {
     if constexpr (L == 0 && VEC) {
+      // plain rows of channels in fours are one run of quads
       Pack<T, NV> v[UN][PARTS];
 #pragma unroll
       for (int j = 0; j < UN; ++j)

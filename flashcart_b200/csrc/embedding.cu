@@ -68,34 +68,46 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
 
 // ------------------------------------------------------------------------------ forward
 
-// Rows of whole, aligned 16-byte vectors: unit = one vector, per_row of them in a row.
+// Rows of whole, aligned 16-byte vectors: unit = one vector, per_row of them in a row. Four
+// units per thread and step; the next step's indices are asked for before this step's rows are
+// (the index comes from DRAM, the row from L1 or L2).
 template <typename T, typename I>
 __global__ void __launch_bounds__(256) embed_fwd_vec(const T* __restrict__ table, int64_t V, int per_row,
                                                      const int64_t* __restrict__ idx, int64_t units,
                                                      typename Io<T>::Acc scale, typename Io<T>::Acc offset,
                                                      T* __restrict__ out, int* status) {
   constexpr int NV = Io<T>::VEC, UN = 4;
-  const I total = (I)units;
-  for (I u0 = (I)blockIdx.x * (256 * UN) + threadIdx.x; u0 < total; u0 += (I)gridDim.x * (256 * UN)) {
-    Pack<T, NV> v[UN];
-    int64_t t[UN];
-    int col[UN];
+  const I total = (I)units, step = (I)gridDim.x * (256 * UN);
+  int64_t t[UN], at[UN];
+  auto ask = [&](I u0, int64_t* tt, int64_t* cc) {
 #pragma unroll
     for (int j = 0; j < UN; ++j) {
       const I u = u0 + j * 256;
+      tt[j] = -1;
+      cc[j] = 0;
       if (u < total) {
         const I row = u / (I)per_row;
-        col[j] = (int)(u - row * (I)per_row);
-        t[j] = __ldg(idx + row);
-        if (t[j] < 0 || t[j] >= V) {
-          if (col[j] == 0) fc_flag(status, FC_DEV_BAD_INDEX);
-          t[j] = -1;
-        }
+        cc[j] = (int64_t)(u - row * (I)per_row);
+        tt[j] = __ldg(idx + row);
       }
     }
+  };
+  I u0 = (I)blockIdx.x * (256 * UN) + threadIdx.x;
+  ask(u0, t, at);
+  for (; u0 < total; u0 += step) {
+    int64_t tn[UN], an[UN];
+    ask(u0 + step, tn, an);
+    Pack<T, NV> v[UN];
 #pragma unroll
     for (int j = 0; j < UN; ++j)
-      if (u0 + j * 256 < total && t[j] >= 0) v[j].load(table + (t[j] * per_row + col[j]) * NV);
+      if (u0 + j * 256 < total) {
+        if (t[j] < 0 || t[j] >= V) {
+          if (at[j] == 0) fc_flag(status, FC_DEV_BAD_INDEX);
+          t[j] = -1;
+        } else {
+          v[j].load(table + (t[j] * per_row + at[j]) * NV);
+        }
+      }
 #pragma unroll
     for (int j = 0; j < UN; ++j)
       if (u0 + j * 256 < total) {
@@ -104,6 +116,11 @@ __global__ void __launch_bounds__(256) embed_fwd_vec(const T* __restrict__ table
           v[j].set(k, t[j] >= 0 ? embed_value<T>(v[j].at(k), scale, offset) : Io<T>::put(0));
         v[j].store(out + (int64_t)(u0 + j * 256) * NV);
       }
+#pragma unroll
+    for (int j = 0; j < UN; ++j) {
+      t[j] = tn[j];
+      at[j] = an[j];
+    }
   }
 }
 
@@ -154,8 +171,8 @@ int embed_fwd(const void* table_, int64_t V, int64_t D, const int64_t* idx, int6
   const uintptr_t at = reinterpret_cast<uintptr_t>(table), ao = reinterpret_cast<uintptr_t>(out);
   if (D % NV == 0 && D / NV <= 0x7fffffff && !((at | ao) & 15)) {
     const int64_t units = R * (D / NV), b = (units + 1023) / 1024;
-    const unsigned grid = (unsigned)(b < (1 << 20) ? b : (1 << 20));
-    if (units + (int64_t)grid * 1024 < ((int64_t)1 << 32))
+    const unsigned grid = (unsigned)(b < 148 * 4 ? b : 148 * 4);  // four blocks per SM stay and walk on
+    if (units + 2 * (int64_t)grid * 1024 < ((int64_t)1 << 32))
       embed_fwd_vec<T, uint32_t><<<grid, 256, 0, s>>>(table, V, (int)(D / NV), idx, units, (A)scale, (A)offset, out,
                                                       status);
     else
@@ -281,7 +298,8 @@ template <bool FIRST>
 __global__ void __launch_bounds__(SORT_THREADS)
     sort_scatter(const int64_t* __restrict__ idx, const int* __restrict__ keys, const int* __restrict__ order,
                  int64_t R, int64_t V, int shift, int bits, int digits, const int* __restrict__ hist,
-                 const int* __restrict__ totals, int* __restrict__ keys_out, int* __restrict__ order_out) {
+                 const int* __restrict__ totals, int* __restrict__ keys_out, int* __restrict__ order_out,
+                 int* __restrict__ start, int scanned) {
   __shared__ int counters[SORT_THREADS / 32][256];
   __shared__ int base[256];
   __shared__ int sh[8];
@@ -298,11 +316,25 @@ __global__ void __launch_bounds__(SORT_THREADS)
 #pragma unroll
   for (int j = 0; j < SORT_ITEMS; ++j)
     loc[j] = warp_rank(key[j] >= 0 ? (key[j] >> shift) & ((1 << bits) - 1) : 256, counters[warp]);
-  int all;
-  const int d0 = threadIdx.x < digits ? totals[threadIdx.x] : 0;
-  const int before = block_exclusive<8>(d0, sh, all);  // its barriers also end the ranking
+  int all, d0 = 0, ahead = 0;  // of this thread's digit: in all tiles, in the tiles before this one
   if (threadIdx.x < digits) {
-    base[threadIdx.x] = before + hist[(int64_t)threadIdx.x * gridDim.x + blockIdx.x];
+    const int* row = hist + (int64_t)threadIdx.x * gridDim.x;
+    if (scanned) {
+      d0 = totals[threadIdx.x];
+      ahead = row[blockIdx.x];
+    } else {
+      for (int t = 0; t < (int)gridDim.x; ++t) {
+        const int c = row[t];
+        d0 += c;
+        if (t < (int)blockIdx.x) ahead += c;
+      }
+    }
+  }
+  const int before = block_exclusive<8>(d0, sh, all);  // its barriers also end the ranking
+  // a sort of one pass: the digits are the tokens, and their totals place them
+  if (start && blockIdx.x == 0 && threadIdx.x < digits) start[threadIdx.x] = before;
+  if (threadIdx.x < digits) {
+    base[threadIdx.x] = before + ahead;
     int sum = 0;
     for (int w = 0; w < SORT_THREADS / 32; ++w) {
       const int t = counters[w][threadIdx.x];
@@ -326,7 +358,8 @@ __global__ void __launch_bounds__(SORT_THREADS)
 // keys and rows ping-ponged in shared memory (one launch where latency is all that counts).
 __global__ void __launch_bounds__(SMALL_THREADS) sort_small(const int64_t* __restrict__ idx, int R, int64_t V,
                                                             int passes, int bits, int* __restrict__ keys_out,
-                                                            int* __restrict__ order_out, int* status) {
+                                                            int* __restrict__ order_out, int* __restrict__ start,
+                                                            int* status) {
   extern __shared__ int sm[];
   constexpr int WARPS = SMALL_THREADS / 32;
   __shared__ int sh[WARPS];
@@ -367,6 +400,7 @@ __global__ void __launch_bounds__(SMALL_THREADS) sort_small(const int64_t* __res
     int all;
     const int before = block_exclusive<WARPS>(sum, sh, all);
     if (threadIdx.x < 256) base[threadIdx.x] = before;
+    if (passes == 1 && threadIdx.x <= V) start[threadIdx.x] = before;
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < SMALL_ROWS / SMALL_THREADS; ++j) {
@@ -394,24 +428,37 @@ __device__ __forceinline__ int lower_bound(const int* __restrict__ keys, int n, 
   return lo;
 }
 
+// Zeros in row[0 .. D) by the lanes of a warp.
+template <typename T>
+__device__ __forceinline__ void zero_row(T* row, int64_t D, bool vec, int lane, int step) {
+  if (vec) {
+    Pack<T, Io<T>::VEC> z;
+    z.raw = make_uint4(0, 0, 0, 0);
+    for (int64_t d = (int64_t)lane * Io<T>::VEC; d < D; d += (int64_t)step * Io<T>::VEC) z.store(row + d);
+  } else {
+    for (int64_t d = lane; d < D; d += step) row[d] = Io<T>::put(0);
+  }
+}
+
 // start[v] = first sorted position of token v (v <= V); zero rows for tokens without any.
 template <typename T>
 __global__ void __launch_bounds__(256) embed_bounds(const int* __restrict__ keys, int R, int64_t V, int64_t D,
-                                                    int* __restrict__ start, T* __restrict__ d_table) {
+                                                    int vec, int* __restrict__ start, T* __restrict__ d_table) {
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const int lane = threadIdx.x & 31;
   int a = 0, b = 0;
   if (v <= V) {
     a = lower_bound(keys, R, (int)v);
     start[v] = a;
-    b = v < V ? lower_bound(keys, R, (int)v + 1) : a + 1;
   }
+  // the next token's start is the next lane's own
+  b = __shfl_down_sync(0xffffffffu, a, 1);
+  if (lane == 31 && v < V) b = lower_bound(keys, R, (int)v + 1);
   unsigned none = __ballot_sync(0xffffffffu, v < V && a == b);
   while (none) {
     const int l = __ffs(none) - 1;
     none &= none - 1;
-    T* row = d_table + (v - lane + l) * D;
-    for (int64_t d = lane; d < D; d += 32) row[d] = Io<T>::put(0);
+    zero_row<T>(d_table + (v - lane + l) * D, D, vec, lane, 32);
   }
 }
 
@@ -488,15 +535,24 @@ __global__ void __launch_bounds__(256)
     }
   };
   int cur = __ldg(keys + p0), from = p0;
-  for (int p = p0; p < p1; p += U) {
-    int key[U], row[U];
-    Pack<T, VECT ? PER : 1> v[U][VECT ? 1 : PER];
+  int key[U], row[U], key_next[U], row_next[U];
+  auto ask = [&](int p, int* k, int* r) {  // the next rows' numbers come while this batch is added
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int q = min(p + u, p1 - 1);
-      key[u] = __ldg(keys + q);
-      row[u] = __ldg(order + q);
+      k[u] = __ldg(keys + q);
+      r[u] = __ldg(order + q);
     }
+  };
+  ask(p0, key_next, row_next);
+  for (int p = p0; p < p1; p += U) {
+    Pack<T, VECT ? PER : 1> v[U][VECT ? 1 : PER];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      key[u] = key_next[u];
+      row[u] = row_next[u];
+    }
+    if (p + U < p1) ask(p + U, key_next, row_next);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const T* g = grad + (int64_t)row[u] * D;
@@ -526,21 +582,24 @@ __global__ void __launch_bounds__(256)
   flush(cur, from, p1);
 }
 
-constexpr int COMBINE_THREADS = 512;
+constexpr int MAX_SLICES = 16;
 
 // Tokens that span chunks: their partial sums added, a token at a time per block. The block
 // looks at `per_block` candidates (tokens, or chunks in which such a token ends, whichever
-// are fewer) and adds each one's partial rows with fixed strides and a fixed tree.
-template <typename T>
-__global__ void __launch_bounds__(COMBINE_THREADS)
+// are fewer) and adds each one's partial rows with fixed strides and a fixed tree. With few
+// types (slices > 1, one candidate per block) blockIdx.z takes a slice of the chunks and leaves
+// its sum to embed_finish. Candidates without any row get their zeros here when they are tokens.
+template <typename T, int THREADS>
+__global__ void __launch_bounds__(THREADS)
     embed_combine(const typename Io<T>::Acc* __restrict__ partial, const int* __restrict__ keys,
                   const int* __restrict__ start, int R, int64_t V, int64_t D, int64_t Dp, int Lc, int64_t chunks,
-                  int by_token, int per_block, int lanes, typename Io<T>::Acc scale, T* __restrict__ d_table) {
+                  int by_token, int per_block, int lanes, int slices, int vec, typename Io<T>::Acc scale,
+                  typename Io<T>::Acc* __restrict__ sums, T* __restrict__ d_table) {
   using A = typename Io<T>::Acc;
   constexpr int PC = 16 / sizeof(A);
-  __shared__ int list[COMBINE_THREADS][3];
+  __shared__ int list[THREADS][3];
   __shared__ int count;
-  __shared__ A red[COMBINE_THREADS][PC];
+  __shared__ A red[THREADS][PC];
   if (threadIdx.x == 0) count = 0;
   __syncthreads();
   const int64_t cand = (int64_t)blockIdx.x * per_block + threadIdx.x;
@@ -556,21 +615,33 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
           list[at][1] = cf;
           list[at][2] = cl;
         }
+      } else if (by_token) {
+        const int at = atomicAdd(&count, 1);
+        list[at][0] = (int)v;
+        list[at][1] = 0;
+        list[at][2] = -1;
       }
     }
   }
   __syncthreads();
-  const int n = count, lane = threadIdx.x & (lanes - 1), g = threadIdx.x / lanes, groups = COMBINE_THREADS / lanes;
+  const int n = count, lane = threadIdx.x & (lanes - 1), g = threadIdx.x / lanes, groups = THREADS / lanes;
   const int64_t col = ((int64_t)blockIdx.y * lanes + lane) * PC;
   for (int e = 0; e < n; ++e) {
     const int64_t v = list[e][0];
     const int cf = list[e][1], cl = list[e][2];
+    if (cl < 0) {
+      if (blockIdx.y == 0 && blockIdx.z == 0)
+        zero_row<T>(d_table + v * D, D, vec, threadIdx.x, THREADS);
+      continue;
+    }
+    const int len = cl - cf + 1, c0 = cf + (int)((int64_t)len * blockIdx.z / slices),
+              c1 = cf + (int)((int64_t)len * (blockIdx.z + 1) / slices);
     A acc[PC];
 #pragma unroll
     for (int k = 0; k < PC; ++k) acc[k] = A(0);
     if (col < Dp) {
 #pragma unroll 8
-      for (int c = cf + g; c <= cl; c += groups) {
+      for (int c = c0 + g; c < c1; c += groups) {
         Pack<A, PC> q;
         q.load(partial + ((int64_t)c * 2 + (c == cf ? 1 : 0)) * Dp + col);
 #pragma unroll
@@ -589,16 +660,42 @@ __global__ void __launch_bounds__(COMBINE_THREADS)
     if (g == 0)
 #pragma unroll
       for (int k = 0; k < PC; ++k)
-        if (col + k < D) d_table[v * D + col + k] = Io<T>::put(scale * red[threadIdx.x][k]);
+        if (col + k < D) {
+          if (slices > 1) sums[(v * slices + blockIdx.z) * Dp + col + k] = red[threadIdx.x][k];
+          else d_table[v * D + col + k] = Io<T>::put(scale * red[threadIdx.x][k]);
+        }
     __syncthreads();
   }
+}
+
+// The slices of tokens that span chunks, added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) embed_finish(const typename Io<T>::Acc* __restrict__ sums,
+                                                    const int* __restrict__ start, int64_t V, int64_t D, int64_t Dp,
+                                                    int Lc, int slices, typename Io<T>::Acc scale,
+                                                    T* __restrict__ d_table) {
+  const int64_t v = blockIdx.x, col = (int64_t)blockIdx.y * 256 + threadIdx.x;
+  const int a = start[v], b = start[v + 1];
+  if (col >= D || b <= a || a / Lc == (b - 1) / Lc) return;
+  typename Io<T>::Acc t = 0;
+  for (int z = 0; z < slices; ++z) t += sums[(v * slices + z) * Dp + col];
+  d_table[v * D + col] = Io<T>::put(scale * t);
 }
 
 // ------------------------------------------------------------------------------ host
 
 struct EmbedWs {
-  int64_t keys[2], order[2], hist, totals, start, partial, bytes;
+  int64_t keys[2], order[2], hist, totals, start, partial, sums, bytes;
 };
+
+// Blocks that share a token's chunks: several where the types alone would leave SMs idle, but
+// at least 64 chunks each.
+static int combine_slices(int64_t V, const SumPlan& sp) {
+  if (V > sp.chunks) return 1;
+  const int64_t blocks = V * ((sp.Dp + 127) / 128), most = sp.chunks / (V * 64);
+  const int64_t z = 148 * 2 / blocks < most ? 148 * 2 / blocks : most;
+  return (int)(z < 1 ? 1 : z > MAX_SLICES ? MAX_SLICES : z);
+}
 
 static int64_t up16(int64_t b) { return (b + 15) & ~(int64_t)15; }
 
@@ -621,6 +718,7 @@ static EmbedWs embed_ws(int64_t R, int64_t V, int64_t D, const SumPlan& sp) {
   w.totals = take(so.digits * 4);
   w.start = take((V + 1) * 4);
   w.partial = take(sp.chunks * 2 * sp.Dp * (int64_t)sizeof(typename Io<T>::Acc));
+  w.sums = take(combine_slices(V, sp) > 1 ? V * MAX_SLICES * sp.Dp * (int64_t)sizeof(typename Io<T>::Acc) : 0);
   w.bytes = at;
   return w;
 }
@@ -659,7 +757,7 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
     const int bytes = (4 * cap + (SMALL_THREADS / 32) * 256) * 4;
     if (cudaFuncSetAttribute(sort_small, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
       return FC_ERR_LAUNCH;
-    sort_small<<<1, SMALL_THREADS, bytes, s>>>(idx, (int)R, V, so.passes, so.bits, keys[0], order[0], status);
+    sort_small<<<1, SMALL_THREADS, bytes, s>>>(idx, (int)R, V, so.passes, so.bits, keys[0], order[0], start, status);
   } else if (R > 0) {
     const unsigned tiles = (unsigned)((R + SORT_TILE - 1) / SORT_TILE);
     for (int pass = 0; pass < so.passes; ++pass) {
@@ -669,21 +767,25 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
       else
         sort_count<false><<<tiles, SORT_THREADS, 0, s>>>(idx, keys[from], R, V, shift, so.bits, so.digits, hist,
                                                          status);
-      sort_scan<<<so.digits, 256, 0, s>>>(hist, (int)tiles, totals);
+      // few tiles: every scatter block adds their counts itself (a launch less)
+      const int scanned = tiles > 64;
+      if (scanned) sort_scan<<<so.digits, 256, 0, s>>>(hist, (int)tiles, totals);
       if (pass == 0)
         sort_scatter<true><<<tiles, SORT_THREADS, 0, s>>>(idx, nullptr, nullptr, R, V, shift, so.bits, so.digits, hist,
-                                                          totals, keys[to], order[to]);
+                                                          totals, keys[to], order[to], so.passes == 1 ? start : nullptr, scanned);
       else
         sort_scatter<false><<<tiles, SORT_THREADS, 0, s>>>(idx, keys[from], order[from], R, V, shift, so.bits,
-                                                           so.digits, hist, totals, keys[to], order[to]);
+                                                           so.digits, hist, totals, keys[to], order[to], nullptr, scanned);
       at = to;
     }
   }
   if (fc_check_launch()) return FC_ERR_LAUNCH;
-  embed_bounds<T><<<(unsigned)((V + 1 + 255) / 256), 256, 0, s>>>(keys[at], (int)R, V, D, start, d_table);
+  // with one pass the sort has placed the tokens, and embed_combine writes the empty rows
+  const int by_token = V <= sp.chunks;
+  if (R == 0 || so.passes > 1 || !by_token || sp.chunks == 1)
+    embed_bounds<T><<<(unsigned)((V + 1 + 255) / 256), 256, 0, s>>>(keys[at], (int)R, V, D, vec, start, d_table);
   if (R > 0) {
-    const int64_t threads = sp.chunks * sp.col_tiles * sp.lanes;
-    const unsigned grid = (unsigned)((threads + 255) / 256);
+    const unsigned grid = (unsigned)((sp.chunks * sp.col_tiles * sp.lanes + 255) / 256);
     if (vec)
       embed_sum<T, Io<T>::VEC, true><<<grid, 256, 0, s>>>(grad, keys[at], order[at], start, (int)R, V, D, sp.Lc,
                                                           sp.chunks, sp.lanes, sp.col_tiles, (A)scale, partial, sp.Dp,
@@ -695,15 +797,21 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
       constexpr int PC = 16 / (int)sizeof(A);
       int lanes = 1;
       while (lanes < 32 && (int64_t)lanes * PC < sp.Dp) lanes *= 2;
-      const int by_token = V <= sp.chunks;
+      const int slices = combine_slices(V, sp);
       const int64_t cands = by_token ? V : sp.chunks;
       int64_t per_block = (cands + 148 * 4 - 1) / (148 * 4);
-      if (per_block > COMBINE_THREADS) per_block = COMBINE_THREADS;
+      // few types: long spans, large blocks; else most spans are a few chunks
+      const int threads = by_token ? 512 : 256;
+      if (per_block > threads) per_block = threads;
+      A* sums = (A*)(p + w.sums);
       const dim3 cgrid((unsigned)((cands + per_block - 1) / per_block),
-                       (unsigned)((sp.Dp + (int64_t)lanes * PC - 1) / ((int64_t)lanes * PC)));
-      embed_combine<T><<<cgrid, COMBINE_THREADS, 0, s>>>(partial, keys[at], start, (int)R, V, D, sp.Dp, sp.Lc,
-                                                         sp.chunks, by_token, (int)per_block, lanes, (A)scale,
-                                                         d_table);
+                       (unsigned)((sp.Dp + (int64_t)lanes * PC - 1) / ((int64_t)lanes * PC)), (unsigned)slices);
+      const auto combine = by_token ? embed_combine<T, 512> : embed_combine<T, 256>;
+      combine<<<cgrid, threads, 0, s>>>(partial, keys[at], start, (int)R, V, D, sp.Dp, sp.Lc, sp.chunks, by_token,
+                                        (int)per_block, lanes, slices, vec, (A)scale, sums, d_table);
+      if (slices > 1)
+        embed_finish<T><<<dim3((unsigned)V, (unsigned)((D + 255) / 256)), 256, 0, s>>>(
+            sums, start, V, D, sp.Dp, sp.Lc, slices, (A)scale, d_table);
     }
   }
   return fc_check_launch();
