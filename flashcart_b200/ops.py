@@ -1594,14 +1594,43 @@ def _grad_needed(*tensors: Optional[Tensor]) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+# The host's share of a call decides small sizes, so these calls pass plain integers and look
+# up a device's stream and status word directly.
+_STATUS_PTR: Dict[int, int] = {}
+
+
+def _launch_on(device: torch.device) -> Tuple[int, int]:
+    """(status word, current stream) of a device as integers for the C ABI."""
+    idx = device.index
+    st = _STATUS_PTR.get(idx)
+    if st is None:
+        st = _STATUS_PTR[idx] = status_word(device).data_ptr()
+    return st, torch._C._cuda_getCurrentRawStream(idx)
+
+
+def _run(what: str, kernels: int, tensors, device: torch.device, fn, *args) -> None:
+    if _TIMER is None:
+        rc = fn(*args)
+    else:
+        with _timed(what[3:], kernels, _nbytes(*tensors)):
+            rc = fn(*args)
+    if rc or _DEBUG_CHECK:
+        _after(N.lib(), rc, what, device)
+
+
+def _addr(t: Optional[Tensor]) -> Optional[int]:
+    return None if t is None else t.data_ptr()
+
+
 def _same_device(what: str, ref: Tensor, *tensors: Optional[Tensor]) -> None:
+    _require_cuda(ref, *tensors)
+    dev = ref.device
     for t in tensors:
-        if t is not None and t.device != ref.device:
-            raise ValueError(f"{what}: tensors on different devices ({ref.device}, {t.device})")
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on different devices ({dev}, {t.device})")
 
 
 def _embedding_args(table: Tensor, index: Tensor) -> None:
-    _require_cuda(table, index)
     _same_device("embedding", table, index)
     if table.dim() != 2:
         raise ValueError(f"embedding: table must be (n_types, features), got shape {tuple(table.shape)}")
@@ -1614,16 +1643,14 @@ def _embedding_fwd(table: Tensor, index: Tensor, scale: float, offset: float) ->
     code = _block_code(table.dtype, "embedding")
     t, idx = table.contiguous(), _idx(index)
     out = t.new_empty(tuple(idx.shape) + (t.shape[1],))
-    lib = N.lib()
-    with _timed("embedding_fwd", 1, _nbytes(t, idx, out)):
-        rc = lib.fc_embedding_fwd(_p(t), t.shape[0], t.shape[1], code, _p(idx), idx.numel(), float(scale),
-                                  float(offset), _p(out), _p(status_word(t.device)), _stream(t.device))
-    _after(lib, rc, "fc_embedding_fwd", t.device)
+    dev = t.device
+    status, stream = _launch_on(dev)
+    _run("fc_embedding_fwd", 1, (t, idx, out), dev, N.lib().fc_embedding_fwd, _addr(t), t.shape[0], t.shape[1], code,
+         _addr(idx), idx.numel(), scale, offset, _addr(out), status, stream)
     return out
 
 
 def _embedding_bwd(grad_out: Tensor, index: Tensor, n_types: int, scale: float) -> Tensor:
-    _require_cuda(grad_out, index)
     _same_device("embedding", grad_out, index)
     code = _block_code(grad_out.dtype, "embedding")
     if grad_out.dim() < 1 or tuple(grad_out.shape[:-1]) != tuple(index.shape):
@@ -1637,10 +1664,9 @@ def _embedding_bwd(grad_out: Tensor, index: Tensor, n_types: int, scale: float) 
     if nb < 0:
         N.check(lib, int(nb), "fc_embedding_bwd_workspace_bytes")
     ws = torch.empty(int(nb), dtype=torch.uint8, device=g.device)
-    with _timed("embedding_bwd", 4, _nbytes(g, idx, out)):
-        rc = lib.fc_embedding_bwd(_p(g), _p(idx), idx.numel(), int(n_types), d, code, float(scale), _p(ws), _p(out),
-                                  _p(status_word(g.device)), _stream(g.device))
-    _after(lib, rc, "fc_embedding_bwd", g.device)
+    status, stream = _launch_on(g.device)
+    _run("fc_embedding_bwd", 4, (g, idx, out), g.device, lib.fc_embedding_bwd, _addr(g), _addr(idx), idx.numel(),
+         int(n_types), d, code, scale, _addr(ws), _addr(out), status, stream)
     return out
 
 
@@ -1692,7 +1718,6 @@ def embedding(table: Tensor, index: Tensor, scale: float = 1.0, offset: float = 
 
 
 def _dropout_args(x: Tensor, rng: Tensor, p: float, l_max: int) -> int:
-    _require_cuda(x, rng)
     _same_device("irreps_dropout", x, rng)
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"irreps_dropout: p must lie in [0, 1], got {p}")
@@ -1710,11 +1735,9 @@ def _irreps_dropout(x: Tensor, rng: Tensor, p: float, l_max: int) -> Tensor:
     code = _block_code(x.dtype, "irreps_dropout")
     x, rng = x.contiguous(), rng.contiguous()
     y = torch.empty_like(x)
-    lib = N.lib()
-    with _timed("irreps_dropout", 1, _nbytes(x, y)):
-        rc = lib.fc_irreps_dropout(int(l_max), features, code, _p(x), _p(rng), float(p), x.shape[0], _p(y),
-                                   _stream(x.device))
-    _after(lib, rc, "fc_irreps_dropout", x.device)
+    _, stream = _launch_on(x.device)
+    _run("fc_irreps_dropout", 1, (x, y), x.device, N.lib().fc_irreps_dropout, l_max, features, code, _addr(x),
+         _addr(rng), p, x.shape[0], _addr(y), stream)
     return y
 
 
@@ -1753,7 +1776,6 @@ _GATE_ACTS = {"silu": N.FC_GATE_SILU, "sigmoid": N.FC_GATE_SIGMOID}
 def _gated_args(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor, gate_bias: Optional[Tensor],
                 scales: Tensor, l_max: int, activation: str) -> N.GatedFfDesc:
     what = "gated_feed_forward"
-    _require_cuda(x, gate_weight, gate_bias, scales, *value_weights)
     _same_device(what, x, gate_weight, gate_bias, scales, *value_weights)
     if activation not in _GATE_ACTS:
         raise ValueError(f"{what}: activation must be 'silu' or 'sigmoid', got {activation!r}")
@@ -1799,10 +1821,9 @@ def _gated_ff_fwd(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tenso
     y = x.new_empty((x.shape[0], (l_max + 1) ** 2 * d.hidden_features))
     lib = N.lib()
     ws = _gated_workspace(lib, d, x.shape[0], False, x.device)
-    with _timed("gated_ff_fwd", 2, _nbytes(x, y, wg, b, *wv)):
-        rc = lib.fc_gated_ff_fwd(ctypes.byref(d), _p(x), _ptr_array(wv), _p(wg), _p(b), _p(sc), x.shape[0], _p(ws),
-                                 _p(y), _p(status_word(x.device)), _stream(x.device))
-    _after(lib, rc, "fc_gated_ff_fwd", x.device)
+    status, stream = _launch_on(x.device)
+    _run("fc_gated_ff_fwd", 2, (x, y, wg, b, *wv), x.device, lib.fc_gated_ff_fwd, ctypes.byref(d), _addr(x),
+         _ptr_array(wv), _addr(wg), _addr(b), _addr(sc), x.shape[0], _addr(ws), _addr(y), status, stream)
     return y
 
 
@@ -1814,7 +1835,6 @@ def _gated_ff_bwd(grad_y: Tensor, x: Tensor, value_weights: Sequence[Tensor], ga
     if tuple(grad_y.shape) != (x.shape[0], (l_max + 1) ** 2 * d.hidden_features) or grad_y.dtype != x.dtype:
         raise ValueError(f"gated_feed_forward: grad_y must be {(x.shape[0], (l_max + 1) ** 2 * d.hidden_features)} of "
                          f"{x.dtype}, got {tuple(grad_y.shape)} of {grad_y.dtype}")
-    _require_cuda(grad_y)
     _same_device("gated_feed_forward", x, grad_y)
     g, x, wg, sc = grad_y.contiguous(), x.contiguous(), gate_weight.contiguous(), scales.contiguous()
     wv = [w.contiguous() for w in value_weights]
@@ -1825,11 +1845,12 @@ def _gated_ff_bwd(grad_y: Tensor, x: Tensor, value_weights: Sequence[Tensor], ga
         return outs
     lib = N.lib()
     ws = _gated_workspace(lib, d, x.shape[0], True, x.device)
-    with _timed("gated_ff_bwd", 8, _nbytes(g, *ins, *outs)):
-        rc = lib.fc_gated_ff_bwd(ctypes.byref(d), _p(g), _p(x), _ptr_array(wv), _p(wg), _p(b), _p(sc), x.shape[0],
-                                 _p(ws), _p(outs[0]), _ptr_array(outs[3:]), _p(outs[1]), _p(outs[2]),
-                                 _p(status_word(x.device)), _stream(x.device))
-    _after(lib, rc, "fc_gated_ff_bwd", x.device)
+    status, stream = _launch_on(x.device)
+    # an empty x still has its place: what is null is not wanted
+    gx = None if outs[0] is None or x.shape[0] == 0 else _addr(outs[0])
+    _run("fc_gated_ff_bwd", 5, (g, *ins, *outs), x.device, lib.fc_gated_ff_bwd, ctypes.byref(d), _addr(g), _addr(x),
+         _ptr_array(wv), _addr(wg), _addr(b), _addr(sc), x.shape[0], _addr(ws), gx, _ptr_array(outs[3:]),
+         _addr(outs[1]), _addr(outs[2]), status, stream)
     return outs
 
 
