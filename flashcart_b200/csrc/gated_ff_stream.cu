@@ -96,7 +96,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   static_assert((3 * S + C::A_RING + 2 * NACC + 2 * SCHED + 1 + 2 * EPI_WARPS) * 8 + SCHED * 4 + 8 <= BAR_BYTES, "barriers");
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512));
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
 
   if (warp < 4) {
     FC_SETMAXNREG_DEC(48);
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
       // ---------------------------------------------------------------- TMA producer
       constexpr uint32_t bytes = C::TILE_A + 2 * TILE_B;
       int next = (int)blockIdx.x;
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
         const int64_t uses = g > s ? (g - 1 - s) / S + 1 : 0;
         if (uses > 0) drain_bar(smem_u32(&full[s]), (uint32_t)((uses - 1) & 1));
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 && elect_one()) {
       // ---------------------------------------------------------------- MMA issue
       int64_t g = 0, u = 0;
       bool ok = true;
@@ -276,11 +276,11 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
         const uint8_t* slab = smem + s * C::STAGE;
         const uint32_t ta = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(slot * C::A_STAGE);
         if constexpr (C::A32) {
-          float x[32];
+          uint32_t x[32];
 #pragma unroll
           for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<float4*>(&x[4 * c]) = *reinterpret_cast<const float4*>(slab + chunk_at<float>(r, c));
-          store_parts<true>(ta, x);
+            *reinterpret_cast<uint4*>(&x[4 * c]) = *reinterpret_cast<const uint4*>(slab + chunk_at<float>(r, c));
+          store_parts(ta, x);
         } else {
           uint32_t h[32];  // bfloat16 is a tf32 value: its bits are the high half
 #pragma unroll
@@ -327,10 +327,11 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
     auto send = [&](const CUtensorMap* map, uint8_t* buf, int col, int row, int z) {
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
-      if (lane == 0) {
+      if (elect_one()) {
         tma_store_3d(map, smem_u32(buf), col, row, z);
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       }
+      __syncwarp();
     };
     for (int q = 0; ok; ++q) {
       const int it = next_item(q);
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
           if (cb < nch) {
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
             __syncwarp();
             uint8_t* buf = stage0 + nbuf * EPI_BUF;
             put_row<T>(buf, lane, acc + cb * 32);
@@ -412,7 +413,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb)
               if (cb < nch) {
-                if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
                 __syncwarp();
                 uint8_t* buf = stage0 + nbuf * EPI_BUF;
                 put_row<T>(buf, lane, acc + cb * 32);
@@ -426,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
           for (int c = 0; c < 64; ++c) sum[c] = 0.f;
           for (int m = 0; m < w.nm && ok; ++m) {
             // the output gradient's boxes come in while the products are computed
-            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
             if (lane == 0)
               for (int cb = 0; cb < nch; ++cb) {
@@ -493,7 +494,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
             for (int j = 0; j < a.nu; ++j, ++u) free_unit(u);
           }
           if (!ok) break;
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
           __syncwarp();
 #pragma unroll
           for (int cb = 0; cb < 2; ++cb)
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
         }
       }
     }
-    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    if (elect_one()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     __syncwarp();
   }
   asm volatile("tcgen05.fence::before_thread_sync;");

@@ -63,7 +63,7 @@ struct Cfg {
   static constexpr int TILE_A = BM * BK * (A32 ? 4 : 2);
   static constexpr int A_STAGE = A32 ? 2 * BK : BK;  // tensor-memory columns
   // Slots of the A ring. Even, so that a slot belongs to one splitter group and one MMA warp,
-  // whose waits miss none of its barriers' phases. PRE keeps pre-activations behind them.
+  // whose waits miss none of its barriers' phases. PRE keeps the gates' slopes behind them.
   static constexpr int A_RING = MODE == PRE && A32 ? 2 : 4, Z_COL = 192;
   static constexpr int BUFS = MODE == PRE ? 2 : 1;   // staging boxes per epilogue warp
   static constexpr int FIXED = EPI_WARPS * BUFS * EPI_BUF + BAR_BYTES + 1024;
@@ -214,10 +214,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
           const bool gates = MODE == DX && w.k0 == 0 && p > 0;
           const CUtensorMap* ma = gates ? &mp.a2 : &mp.a;
           const int z = gates ? p - 1 : MODE == DX ? w.k0 + p : (p == 0 ? 0 : w.k0 + p - 1);
-          if (MODE == PRE && p + 1 < passes) {
-            // two A stages are too few to cover DRAM: have the next pass's operands in L2
-            tma_prefetch_3d(&mp.ap, 0, w.tile * BM, w.k0 + p);
-            tma_prefetch_3d(&mp.gp, ct * BN, w.tile * BM, w.k0 + p);
+          // have the next pass's operands in L2: the ring's stages alone do not cover DRAM
+          if (p + 1 < passes && (MODE != DX || w.k0 > 0)) {
+            const int zn = w.k0 + p + (MODE == DX ? 1 : 0);
+            tma_prefetch_3d(&mp.ap, 0, w.tile * BM, zn);
+            if (MODE == PRE) tma_prefetch_3d(&mp.gp, ct * BN, w.tile * BM, zn);
+          } else if (p + 1 == passes && next < a.items) {
+            const Item wn = item_of(a, next);
+            tma_prefetch_3d(&mp.ap, 0, wn.tile * BM, MODE == DX ? wn.k0 : 0);
           }
           for (int kt = 0; kt < nk; ++kt, ++g) {
             if (lap > 0 && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
@@ -406,6 +410,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
             }
           }
         }
+        // the slab is in registers: its stage may be refilled
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&empty[s]));
         // (the first lap's wait is for the phase before the first and succeeds at once)
         if (!slot_ready) ok = wait_warp(smem_u32(&a_free[as]), (as_lap & 1u) ^ 1u, abort_flag);
         if (!ok) break;
@@ -424,22 +431,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
         const bool peek_slot = peek_parity(smem_u32(&a_free[as_next]), (as_lap_next & 1u) ^ 1u);
         asm volatile("tcgen05.fence::after_thread_sync;");
         if constexpr (C::A32) {
-          // hi: the upper 19 bits (tf32); lo: the rest, exact in float, rounded where tf32 ends
-          // (its lower 13 bits do not reach the product). Three operations an element: the
-          // kernel is short of issue slots before anything else.
-          uint32_t p[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) p[e] = x[e] & 0xFFFFE000u;
-          tmem_st32(ta, p);
-#pragma unroll
-          for (int e = 0; e < 32; ++e)
-            p[e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xFFFFE000u)) + 0x1000u;
-          tmem_st32(ta + BK, p);
+          store_parts(ta, x);  // three operations an element: issue slots are short here
         } else {
           tmem_st32(ta, x);
         }
-        __syncwarp();
-        if (lane == 0) arrive(smem_u32(&empty[s]));  // the slab is in registers: its stage may be refilled
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -503,6 +498,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
       if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
       __syncwarp();
     };
+    // PRE: the box in turn is free (the boxes send by turns, so at most the other one's store is
+    // still reading)
+    auto box_free = [&]() {
+      if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+      __syncwarp();
+    };
     uint32_t box = 0, box_phase = 0;  // PRE: the box in turn; bit b: parity of landed[b]'s next completion
     for (int q = 0; ok; ++q) {
       const int it = item_warp(q);
@@ -542,7 +543,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
           __syncwarp();
         };
         if (MODE == PRE && live) {
-          boxes_free();
+          box_free();
           ask(0, box);
         }
         float z[32];  // pre-activations of this thread's row
@@ -574,12 +575,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
             }
           }
         } else {
-          // the pre-activations wait in tensor memory until the rank is done; the gates stay here
+          // the gates stay here, their slopes wait in tensor memory until the rank is done
           const uint32_t z_at = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(C::Z_COL + half * 32);
-          tmem_st32(z_at, reinterpret_cast<const uint32_t*>(z));
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          {
+            float slope[32];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) z[c] = sa * fast_act(a.act, z[c]);
+            for (int c = 0; c < 32; ++c) {
+              const float sg = fast_sigmoid(z[c]), q = 1.f - sg;
+              slope[c] = sa * (a.act == FC_GATE_SIGMOID ? sg * q : sg * fmaf(z[c], q, 1.f));
+              z[c] = sa * (a.act == FC_GATE_SIGMOID ? sg : z[c] * sg);
+            }
+            tmem_st32(z_at, reinterpret_cast<const uint32_t*>(slope));
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          }
           float sum[32];  // over m of g v
 #pragma unroll
           for (int c = 0; c < 32; ++c) sum[c] = 0.f;
@@ -643,13 +651,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
             __syncwarp();
           }
           if (ok && live) {
-            boxes_free();
+            box_free();
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float zz[16];
               tmem_ld<16>(z_at + h * 16, zz);
 #pragma unroll
-              for (int c = 0; c < 16; ++c) sum[h * 16 + c] *= sa * fast_dact(a.act, zz[c]);
+              for (int c = 0; c < 16; ++c) sum[h * 16 + c] *= zz[c];
             }
             put_row<float>(boxes + box * EPI_BUF, lane, sum);
             send(&mp.o2, boxes + box * EPI_BUF, row0, w.l);
@@ -807,7 +815,7 @@ static Ws layout(int L, int C, int H, int64_t n, int esize, bool backward, int s
     w.dv = take(n * comps * hp * 4);
     w.dz = take(n * ranks * hp * 4);
     w.part = take(parts * BM * BM * 4);
-    w.bias = take(parts * BM * 4);
+    w.bias = take(parts * 2 * BM * 4);
   }
   // copies with 16-byte rows, used where the caller's rows are not (or are misaligned)
   w.x = take(n * comps * ce * esize);
@@ -905,9 +913,10 @@ int gated_tc_fwd(const GatedArgs& a, cudaStream_t s) {
   Maps mp;
   if (!encode_rows<T>(&mp.a, x.p, a.C, a.n, comps, x.ld, BK, BM) ||
       !encode_weights(&mp.b, weights, (a.C + 3) & ~3, a.H, 4 * ranks, weight_rows(a.C, a.H, sms)) ||
+      !encode_rows<T>(&mp.ap, x.p, a.C, a.n, comps, x.ld, MAX_NK * BK, BM) ||
       !encode_rows<T>(&mp.o, y.p, a.H, a.n, comps, y.ld, 32, 32))
     return FC_ERR_UNSUPPORTED;
-  mp.a2 = mp.ap = mp.g = mp.gp = mp.o2 = mp.o;  // not used
+  mp.a2 = mp.g = mp.gp = mp.o2 = mp.o;  // not used
   if (int rc = run_products<FWD, T>(mp, args, a.C, sms, s)) return rc;
   if (y.copied) return repitch<T>(y.p, y.ld, (T*)a.y, a.H, a.H, a.n * comps, s);
   return 0;
@@ -950,11 +959,12 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
       const Rows<T> gx = rows_of<T>(a.gx, a.C, ws + w.gx);
       Maps md;
       if (!encode_rows<float>(&md.a, dv, a.H, a.n, comps, hp, BK, BM) ||
+          !encode_rows<float>(&md.ap, dv, a.H, a.n, comps, hp, MAX_NK * BK, BM) ||
           !encode_rows<float>(&md.a2, dz, a.H, a.n, ranks, hp, BK, BM) ||
           !encode_weights(&md.b, dx, (int)hp, a.C, 4 * ranks, weight_rows(a.H, a.C, sms)) ||
           !encode_rows<T>(&md.o, gx.p, a.C, a.n, comps, gx.ld, 32, 32))
         return FC_ERR_UNSUPPORTED;
-      md.ap = md.g = md.gp = md.o2 = md.o;  // not used
+      md.g = md.gp = md.o2 = md.o;  // not used
       Args dargs = product_args(a, a.C, a.H, DX, sms);
       dargs.counter = counters + MAX_LISTS;
       if (int rc = run_products<DX, T>(md, dargs, a.H, sms, s)) return rc;

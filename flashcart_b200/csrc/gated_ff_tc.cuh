@@ -104,18 +104,28 @@ __device__ __forceinline__ void tmem_ld_sum<32>(uint32_t ta, uint32_t tb, float*
   for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(v[c]) + __uint_as_float(w[c]);
 }
 
-// 32 floats -> the tf32 parts of a lane's 32 columns
-template <bool LO>
-__device__ __forceinline__ void store_parts(uint32_t ta, const float* x) {
+// 16 consecutive tensor-memory columns of this thread's lane (warp-collective).
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+
+// 32 floats -> the tf32 parts of a lane's 32 columns: hi, the upper 19 bits, and lo, the rest,
+// exact in float and rounded where tf32 ends (its lower 13 bits do not reach the product). The
+// other operand's hi is rounded, so that the left-out product of both lo parts averages out.
+__device__ __forceinline__ void store_parts(uint32_t ta, const uint32_t* x) {
   uint32_t p[32];
 #pragma unroll
-  for (int e = 0; e < 32; ++e) p[e] = __float_as_uint(round_tf32(x[e]));
+  for (int e = 0; e < 32; ++e) p[e] = x[e] & 0xFFFFE000u;
   tmem_st32(ta, p);
-  if (LO) {
 #pragma unroll
-    for (int e = 0; e < 32; ++e) p[e] = __float_as_uint(round_tf32(x[e] - round_tf32(x[e])));
-    tmem_st32(ta + BK, p);
-  }
+  for (int e = 0; e < 32; ++e)
+    p[e] = __float_as_uint(__uint_as_float(x[e]) - __uint_as_float(x[e] & 0xFFFFE000u)) + 0x1000u;
+  tmem_st32(ta + BK, p);
 }
 
 // One lane of a converged warp. tcgen05 and TMA instructions take their operands from uniform
@@ -158,7 +168,7 @@ __device__ __forceinline__ bool wait_phase(uint32_t mbar, uint32_t parity, volat
 #pragma unroll 1
   do {
     done = test_parity(mbar, parity);
-  } while (!done && ++round < WAIT_ROUNDS && !*abort_flag);
+  } while (!done && ++round < WAIT_ROUNDS && !((round & 31) == 0 && *abort_flag));
   if (!done) *abort_flag = 1;
   return done;
 }

@@ -18,6 +18,7 @@ namespace fc {
 namespace gtc {
 
 constexpr int BN = 128, TILE_B = BN * BK * 4;
+constexpr int PF = 6;  // slabs between the L2 prefetches and the copies
 constexpr int KG = 2;  // slabs per accumulation unit (see gated_ff_tc.cu)
 
 struct WArgs {
@@ -30,7 +31,7 @@ struct WArgs {
   int64_t total;       // slabs in all
   int ctas;
   float* part;         // partial matrices, 128 x 128 each
-  float* bias_part;    // partial bias gradients, 128 each (ct = 0 jobs of the gates), or null
+  float* bias_part;    // partial bias gradients, 2 x 128 each (ct = 0 jobs of the gates), or null
   int* status;
 };
 
@@ -66,37 +67,46 @@ __host__ __device__ inline Job job_at(const WArgs& a, int64_t slab) {
 }
 __host__ __device__ inline int64_t cta_begin(const WArgs& a, int64_t i) { return i * a.total / a.ctas; }
 
+constexpr int W_SPLIT0 = 4, W_EPI0 = 20, W_THREADS = 28 * 32;
+constexpr int W_REGS = 72;  // per thread at launch: 896 x 72 = 128 x 40 + 512 x 56 + 256 x 120
+constexpr int RAW = 4, OPS = 2;  // stages of raw slabs, slots of split operands; even: each belongs
+                                 // to one splitter group, which so sees every phase of its barriers
+
 template <typename T>
 struct WCfg {
   static constexpr bool X32 = sizeof(T) == 4;
-  static constexpr int TILE_D = 32 * BM * 4;         // raw dv / dz slab
-  static constexpr int TILE_X = 32 * BN * sizeof(T); // raw x slab
-  static constexpr int STAGE = TILE_D + TILE_X + (X32 ? 2 : 1) * TILE_B;
-  static constexpr int STAGES = X32 ? 3 : 4;
-  static constexpr int SMEM = STAGES * STAGE + BAR_BYTES + 1024;
-  static constexpr int NACC = 2, A_COLS = STAGES * 2 * BK;  // every stage has its A slot
+  static constexpr int TILE_D = 32 * BM * 4;          // raw dv / dz slab
+  static constexpr int TILE_X = 32 * BN * sizeof(T);  // raw x slab
+  static constexpr int OPERAND = (X32 ? 2 : 1) * TILE_B;
+  static constexpr int SMEM = OPS * OPERAND + RAW * (TILE_D + TILE_X) + BAR_BYTES + 1024;
+  static constexpr int NACC = 2, A_COLS = OPS * 2 * BK;
   static_assert(A_COLS + NACC * BN <= 512, "tensor memory");
   static_assert(SMEM <= 227 * 1024, "shared memory per CTA");
 };
 
+// Roles of the 28 warps: 0 TMA producer, 1 MMA issue, 4-19 splitters (two groups that take the
+// slabs in turn, each four warps for dv / dz and four for x), 20-27 epilogue (unit sums, two
+// warps per lane quarter). Measured before the second group, the raw ring of its own and the
+// early answers: 130 us for 27,648 x 16 rows of 128 -> 128 channels, a slab waiting for its
+// splitters most of the time.
 template <typename T>
-__global__ void __launch_bounds__(THREADS, 1) wgrad_kernel(const __grid_constant__ WMaps mp, const WArgs a) {
+__global__ void __launch_bounds__(W_THREADS, 1) wgrad_kernel(const __grid_constant__ WMaps mp, const WArgs a) {
   using C = WCfg<T>;
-  constexpr int S = C::STAGES, NACC = C::NACC, A_COLS = C::A_COLS;
+  constexpr int NACC = C::NACC, A_COLS = C::A_COLS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * C::STAGE);
-  uint64_t* split = full + S;
-  uint64_t* empty = split + S;
-  uint64_t* acc_full = empty + S;
+  uint8_t* raw = smem + OPS * C::OPERAND;
+  uint64_t* full = reinterpret_cast<uint64_t*>(raw + RAW * (C::TILE_D + C::TILE_X));
+  uint64_t* empty = full + RAW;
+  uint64_t* op_full = empty + RAW;
+  uint64_t* op_free = op_full + OPS;
+  uint64_t* acc_full = op_free + OPS;
   uint64_t* acc_empty = acc_full + NACC;
   uint64_t* drain = acc_empty + NACC;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  // within a stage: the K-major B parts first (1024-byte aligned), then the raw slabs
-  constexpr int D_OFF = (C::X32 ? 2 : 1) * TILE_B, X_OFF = D_OFF + C::TILE_D;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if (warp == 0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(512));
@@ -106,14 +116,17 @@ __global__ void __launch_bounds__(THREADS, 1) wgrad_kernel(const __grid_constant
     auto init = [](uint64_t* b, int n) {
       asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n));
     };
-    for (int s = 0; s < S; ++s) {
+    for (int s = 0; s < RAW; ++s) {
       init(&full[s], 1);
-      init(&split[s], 8);
-      init(&empty[s], 1);
+      init(&empty[s], 8);
+    }
+    for (int s = 0; s < OPS; ++s) {
+      init(&op_full[s], 8);
+      init(&op_free[s], 1);
     }
     for (int b = 0; b < NACC; ++b) {
       init(&acc_full[b], 1);
-      init(&acc_empty[b], 4);
+      init(&acc_empty[b], 8);
     }
     init(drain, 1);
     *abort_flag = 0;
@@ -125,11 +138,12 @@ __global__ void __launch_bounds__(THREADS, 1) wgrad_kernel(const __grid_constant
   const uint32_t tmem = *tmem_slot;
   const int64_t begin = cta_begin(a, blockIdx.x), end = cta_begin(a, blockIdx.x + 1);
 
-  if (warp < 4) {
-    FC_SETMAXNREG_DEC(56);
-    if (warp == 0 && lane == 0) {
+  if (warp < W_SPLIT0) {
+    FC_SETMAXNREG_DEC(40);
+    if (warp == 0 && elect_one()) {
       // ---------------------------------------------------------------- TMA producer
       int64_t g = 0;
+      uint32_t s = 0, lap = 0;
       bool ok = true;
       for (int64_t p = begin; p < end && ok;) {
         const Job j = job_at(a, p);
@@ -140,176 +154,228 @@ __global__ void __launch_bounds__(THREADS, 1) wgrad_kernel(const __grid_constant
           p = stop;
           continue;
         }
+        const CUtensorMap* md = gates ? &mp.dz : &mp.dv;
+        const int zd = gates ? l : l * l, zx = gates ? 0 : l * l;
+        // rows of a node block one component after the other: they share DRAM pages
+        int nb = (int)((p - j.first) / w), m = (int)((p - j.first) - (int64_t)nb * w);
+        int nbf = nb + PF / w, mf = m + PF % w;  // PF slabs on
+        if (mf >= w) {
+          mf -= w;
+          ++nbf;
+        }
         for (; p < stop; ++p, ++g) {
-          const int s = (int)(g % S);
-          if (g >= S && !wait_phase(smem_u32(&empty[s]), (uint32_t)(((g / S) - 1) & 1), abort_flag)) {
+          if (lap > 0 && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
             ok = false;
             break;
           }
-          // rows of a node block one component after the other: they share DRAM pages
-          const int64_t r = p - j.first, nb = r / w;
-          const int m = (int)(r - nb * w);
-          uint8_t* st = smem + s * C::STAGE;
+          if (p + PF < stop) {  // the ring's stages alone do not cover DRAM
+            tma_prefetch_3d(md, j.ht * BM, nbf * 32, zd + mf);
+            tma_prefetch_3d(&mp.x, j.ct * BN, nbf * 32, zx + mf);
+            if (++mf == w) {
+              mf = 0;
+              ++nbf;
+            }
+          }
+          uint8_t* st = raw + s * (C::TILE_D + C::TILE_X);
           const uint32_t fb = smem_u32(&full[s]);
           arrive_tx(fb, C::TILE_D + C::TILE_X);
-          tma_load_3d(smem_u32(st + D_OFF), gates ? &mp.dz : &mp.dv, j.ht * BM, (int)(nb * 32), gates ? l : l * l + m,
-                      fb);
-          tma_load_3d(smem_u32(st + X_OFF), &mp.x, j.ct * BN, (int)(nb * 32), gates ? 0 : l * l + m, fb);
+          tma_load_3d(smem_u32(st), md, j.ht * BM, nb * 32, zd + m, fb);
+          tma_load_3d(smem_u32(st + C::TILE_D), &mp.x, j.ct * BN, nb * 32, zx + m, fb);
+          if (++m == w) {
+            m = 0;
+            ++nb;
+          }
+          if (++s == RAW) {
+            s = 0;
+            ++lap;
+          }
         }
       }
-      for (int s = 0; s < S; ++s) {
-        const int64_t uses = g > s ? (g - 1 - s) / S + 1 : 0;
-        if (uses > 0) drain_bar(smem_u32(&full[s]), (uint32_t)((uses - 1) & 1));
+      for (int t = 0; t < RAW; ++t) {
+        const int64_t uses = g > t ? (g - 1 - t) / RAW + 1 : 0;
+        if (uses > 0) drain_bar(smem_u32(&full[t]), (uint32_t)((uses - 1) & 1));
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issue
-      int64_t g = 0, u = 0;
-      bool ok = true;
+      const uint64_t desc = make_desc(smem_u32(smem));
+      uint32_t os = 0, op_phase = 0, ab = 0, acc_phase = 0;
+      bool ok = true, op_ready = false, acc_ready = false;
       for (int64_t p = begin; p < end && ok;) {
         const Job j = job_at(a, p);
-        const int64_t stop = min(end, j.last);
-        if (a.skip >> j.mat & 1) p = stop;
-        while (p < stop && ok) {
-          const int b = (int)(u % NACC);
-          const int64_t v = u / NACC;
-          if (v >= 1 && !wait_phase(smem_u32(&acc_empty[b]), (uint32_t)((v - 1) & 1), abort_flag)) {
-            ok = false;
-            break;
-          }
+        const int slabs = (int)(min(end, j.last) - p);
+        p += slabs;
+        if (a.skip >> j.mat & 1) continue;
+#pragma unroll 1
+        for (int t = 0; t < slabs; ++t) {
+          const bool first = t % KG == 0, last = t % KG == KG - 1 || t + 1 == slabs;  // of its unit
+          if (first && !acc_ready) ok = wait_warp(smem_u32(&acc_empty[ab]), acc_phase ^ 1u, abort_flag);
+          if (!op_ready) ok = ok && wait_warp(smem_u32(&op_full[os]), op_phase, abort_flag);
+          if (!ok) break;
           asm volatile("tcgen05.fence::after_thread_sync;");
-          const uint32_t d = tmem + (uint32_t)(A_COLS + b * BN);
-          const int64_t unit = min(stop, p + KG);
-          bool fresh = true;
-          for (; p < unit; ++p, ++g) {
-            const int s = (int)(g % S);
-            if (!wait_phase(smem_u32(&split[s]), (uint32_t)((g / S) & 1), abort_flag)) {
-              ok = false;
-              break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;");
-            uint8_t* st = smem + s * C::STAGE;
-            const uint64_t dbh = make_desc(smem_u32(st)), dbl = make_desc(smem_u32(st + TILE_B));
-            const uint32_t tah = tmem + (uint32_t)(s * 2 * BK), tal = tah + (uint32_t)BK;
+          const uint32_t os_next = os ^ 1u, ph_next = op_phase ^ os, ab_next = ab ^ 1u, acc_next = acc_phase ^ ab;
+          const bool peek_op = peek_parity(smem_u32(&op_full[os_next]), ph_next);
+          const bool peek_acc = peek_parity(smem_u32(&acc_empty[ab_next]), acc_next ^ 1u);
+          const uint32_t d = tmem + (uint32_t)A_COLS + ab * (uint32_t)BN;
+          const uint32_t tah = tmem + os * (uint32_t)(2 * BK), tal = tah + (uint32_t)BK;
+          const uint64_t dbh = desc + (uint64_t)os * (C::OPERAND >> 4), dbl = dbh + (uint64_t)(TILE_B >> 4);
+          if (elect_one()) {
 #pragma unroll
             for (int kk = 0; kk < BK / 8; ++kk) {
-              const uint64_t off = (uint64_t)((kk * 32) >> 4);
-              mma_ta<BN>(d, tal + kk * 8, dbh + off, fresh && kk == 0 ? 0u : 1u);
-              if (C::X32) mma_ta<BN>(d, tah + kk * 8, dbl + off, 1u);
+              mma_ta<BN>(d, tal + kk * 8, dbh + 2 * kk, first && kk == 0 ? 0u : 1u);
+              if (C::X32) mma_ta<BN>(d, tah + kk * 8, dbl + 2 * kk, 1u);
             }
 #pragma unroll
-            for (int kk = 0; kk < BK / 8; ++kk) mma_ta<BN>(d, tah + kk * 8, dbh + (uint64_t)((kk * 32) >> 4), 1u);
-            fresh = false;
-            commit(smem_u32(&empty[s]));
+            for (int kk = 0; kk < BK / 8; ++kk) mma_ta<BN>(d, tah + kk * 8, dbh + 2 * kk, 1u);
+            commit(smem_u32(&op_free[os]));
+            if (last) commit(smem_u32(&acc_full[ab]));
           }
-          if (ok) {
-            commit(smem_u32(&acc_full[b]));
-            ++u;
+          op_ready = __all_sync(0xffffffffu, peek_op);
+          const bool acc_next_ready = __all_sync(0xffffffffu, peek_acc);
+          os = os_next;
+          op_phase = ph_next;
+          if (last) {
+            acc_ready = acc_next_ready;
+            ab = ab_next;
+            acc_phase = acc_next;
           }
         }
       }
-      commit(smem_u32(drain));
-      drain_bar(smem_u32(drain), 0);
+      if (elect_one()) {
+        commit(smem_u32(drain));
+        drain_bar(smem_u32(drain), 0);
+      }
+      __syncwarp();
     }
-  } else if (warp < 12) {
-    FC_SETMAXNREG_DEC(112);
+  } else if (warp < W_EPI0) {
+    FC_SETMAXNREG_DEC(56);
     // ------------------------------------------------------------------ splitters
-    const bool of_d = warp < 8;               // dv / dz into tensor memory, or x into K-major rows
-    const int c = (warp & 3) * 32 + lane;     // channel: lane of tensor memory, or row of the B tile
-    int64_t g = 0;
-    bool ok = true;
+    const int mine = (warp - W_SPLIT0) >> 3;           // this group's slabs: g = mine mod 2
+    const bool of_d = ((warp - W_SPLIT0) & 4) == 0;    // dv / dz into tensor memory, or x into K-major rows
+    const int c = (warp & 3) * 32 + lane;              // channel: lane of tensor memory, or row of the B tile
+    const uint32_t ta = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(mine * 2 * BK);
+    uint8_t* ops = smem + mine * C::OPERAND;
+    uint32_t s = (uint32_t)mine, lap = 0, op_phase = 1;  // own raw stage, own operand slot (free at first)
+    int left = -mine;                                    // slabs of the part from this group's next one on
+    bool ok = true, full_ready = false;
     for (int64_t p = begin; p < end && ok;) {
       const Job j = job_at(a, p);
-      const int64_t stop = min(end, j.last);
-      if (a.skip >> j.mat & 1) {
-        p = stop;
-        continue;
-      }
+      const int slabs = (int)(min(end, j.last) - p);
+      p += slabs;
+      if (a.skip >> j.mat & 1) continue;
       const bool bias = of_d && a.bias_part && j.mat >= a.ranks && j.ct == 0;
       float bsum = 0.f;
-      for (; p < stop; ++p, ++g) {
-        const int s = (int)(g % S);
-        if (!wait_warp(smem_u32(&full[s]), (uint32_t)((g / S) & 1), abort_flag)) {
-          ok = false;
-          break;
-        }
-        uint8_t* st = smem + s * C::STAGE;
-        float x[32];
+      for (left += slabs; left > 0; left -= 2) {
+        if (!full_ready) ok = wait_warp(smem_u32(&full[s]), lap & 1u, abort_flag);
+        ok = ok && wait_warp(smem_u32(&op_free[mine]), op_phase, abort_flag);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        const uint8_t* st = raw + s * (C::TILE_D + C::TILE_X);
+        const uint32_t s_next = s ^ 2u, lap_next = lap + (s >> 1);  // stages mine and mine + 2 in turn
+        const bool peek_full = peek_parity(smem_u32(&full[s_next]), lap_next & 1u);
+        // 16 rows at a time; hi = the upper 19 bits, lo = the exact rest, rounded where tf32 ends
         if (of_d) {
-          const float* raw = reinterpret_cast<const float*>(st + D_OFF) + c;
+          const uint32_t* src = reinterpret_cast<const uint32_t*>(st) + c;
+          float t = 0.f;  // a slab's sum first: fewer roundings against the running sum
 #pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = raw[k * BM];
-          if (bias) {
-            float t = 0.f;  // a slab's sum first: fewer roundings against the running sum
+          for (int h = 0; h < 2; ++h) {
+            uint32_t x[16], q[16];
 #pragma unroll
-            for (int k = 0; k < 32; ++k) t += x[k];
-            bsum += t;
+            for (int k = 0; k < 16; ++k) x[k] = src[(h * 16 + k) * BM];
+            if (bias)
+#pragma unroll
+              for (int k = 0; k < 16; ++k) t += __uint_as_float(x[k]);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) q[k] = x[k] & 0xFFFFE000u;
+            tmem_st16(ta + h * 16, q);
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              q[k] = __float_as_uint(__uint_as_float(x[k]) - __uint_as_float(x[k] & 0xFFFFE000u)) + 0x1000u;
+            tmem_st16(ta + BK + h * 16, q);
           }
-          store_parts<true>(tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(s * 2 * BK), x);
+          bsum += t;
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         } else {
-          const T* raw = reinterpret_cast<const T*>(st + X_OFF) + c;
+          // hi rounded here: were both operands' lo parts of their values' sign, the product of
+          // the two that is left out would not average out (2.4e-7 of the sum)
+          const uint32_t r0 = C::X32 ? 0x1000u : 0u;
+          const T* src = reinterpret_cast<const T*>(st + C::TILE_D) + c;
 #pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = Io<T>::get(raw[k * BN]);
+          for (int h = 0; h < 2; ++h) {
+            uint32_t x[16];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            float h[4];
+            for (int k = 0; k < 16; ++k) x[k] = __float_as_uint(Io<T>::get(src[(h * 16 + k) * BN]));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) h[e] = C::X32 ? round_tf32(x[4 * q + e]) : x[4 * q + e];
-            *reinterpret_cast<float4*>(st + chunk_at<float>(c, q)) = make_float4(h[0], h[1], h[2], h[3]);
-            if (C::X32) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) h[e] = round_tf32(x[4 * q + e] - h[e]);
-              *reinterpret_cast<float4*>(st + TILE_B + chunk_at<float>(c, q)) = make_float4(h[0], h[1], h[2], h[3]);
+            for (int q = 0; q < 4; ++q) {
+              uint4 v;
+              v.x = (x[4 * q] + r0) & 0xFFFFE000u, v.y = (x[4 * q + 1] + r0) & 0xFFFFE000u;
+              v.z = (x[4 * q + 2] + r0) & 0xFFFFE000u, v.w = (x[4 * q + 3] + r0) & 0xFFFFE000u;
+              *reinterpret_cast<uint4*>(ops + chunk_at<float>(c, h * 4 + q)) = v;
+              if (C::X32) {
+                uint4 r;
+                r.x = __float_as_uint(__uint_as_float(x[4 * q]) - __uint_as_float(v.x)) + 0x1000u;
+                r.y = __float_as_uint(__uint_as_float(x[4 * q + 1]) - __uint_as_float(v.y)) + 0x1000u;
+                r.z = __float_as_uint(__uint_as_float(x[4 * q + 2]) - __uint_as_float(v.z)) + 0x1000u;
+                r.w = __float_as_uint(__uint_as_float(x[4 * q + 3]) - __uint_as_float(v.w)) + 0x1000u;
+                *reinterpret_cast<uint4*>(ops + TILE_B + chunk_at<float>(c, h * 4 + q)) = r;
+              }
             }
           }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         }
         __syncwarp();
-        if (lane == 0) arrive(smem_u32(&split[s]));
+        if (lane == 0) {
+          arrive(smem_u32(&empty[s]));
+          arrive(smem_u32(&op_full[mine]));
+        }
+        full_ready = __all_sync(0xffffffffu, peek_full);
+        s = s_next;
+        lap = lap_next;
+        op_phase ^= 1u;
       }
-      if (bias && ok) a.bias_part[(blockIdx.x + j.index) * BM + c] = bsum;
+      // both groups' sums of the bias channel: the first group's in the first half of the slot
+      if (bias && ok) a.bias_part[((blockIdx.x + j.index) * 2 + mine) * BM + c] = bsum;
     }
   } else {
-    FC_SETMAXNREG_INC(216);
+    FC_SETMAXNREG_INC(120);
     // ------------------------------------------------------------------ epilogue: unit sums
-    const int quarter = warp & 3;
-    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)A_COLS;
-    int64_t u = 0;
+    const int quarter = warp & 3, half = (warp - W_EPI0) >> 2;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(A_COLS + half * 64);
+    uint32_t ab = 0, acc_phase = 0;
     bool ok = true;
     for (int64_t p = begin; p < end && ok;) {
       const Job j = job_at(a, p);
-      const int64_t stop = min(end, j.last);
-      if (a.skip >> j.mat & 1) {
-        p = stop;
-        continue;
-      }
-      float acc[BN];
+      const int slabs = (int)(min(end, j.last) - p);
+      p += slabs;
+      if (a.skip >> j.mat & 1) continue;
+      float acc[64];
 #pragma unroll
-      for (int c = 0; c < BN; ++c) acc[c] = 0.f;
-      for (; p < stop; p += KG, ++u) {
-        const int b = (int)(u % NACC);
-        if (!wait_warp(smem_u32(&acc_full[b]), (uint32_t)((u / NACC) & 1), abort_flag)) {
+      for (int c = 0; c < 64; ++c) acc[c] = 0.f;
+#pragma unroll 1
+      for (int t = 0; t < slabs; t += KG) {
+        if (!wait_warp(smem_u32(&acc_full[ab]), acc_phase, abort_flag)) {
           ok = false;
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;");
 #pragma unroll
-        for (int cb = 0; cb < BN / 32; ++cb) {
-          float f[32];
-          tmem_ld<32>(lane_base + (uint32_t)(b * BN + cb * 32), f);
+        for (int cb = 0; cb < 4; ++cb) {
+          float f[16];
+          tmem_ld<16>(lane_base + ab * (uint32_t)BN + (uint32_t)(cb * 16), f);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) acc[cb * 32 + c] += f[c];
+          for (int c = 0; c < 16; ++c) acc[cb * 16 + c] += f[c];
         }
         asm volatile("tcgen05.fence::before_thread_sync;");
         __syncwarp();
-        if (lane == 0) arrive(smem_u32(&acc_empty[b]));
+        if (lane == 0) arrive(smem_u32(&acc_empty[ab]));
+        acc_phase ^= ab;
+        ab ^= 1u;
       }
-      p = stop;
       if (!ok) break;
-      float4* out = reinterpret_cast<float4*>(a.part + ((blockIdx.x + j.index) * BM + quarter * 32 + lane) * BN);
+      float4* out =
+          reinterpret_cast<float4*>(a.part + ((blockIdx.x + j.index) * BM + quarter * 32 + lane) * BN + half * 64);
 #pragma unroll
-      for (int c = 0; c < BN / 4; ++c)
+      for (int c = 0; c < 16; ++c)
         out[c] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
     }
   }
@@ -354,7 +420,7 @@ __global__ void __launch_bounds__(SUM_ROWS * SUM_PARTS * 32) wgrad_sum_kernel(co
     while (i1 > i0 && cta_begin(a, i1) >= last) --i1;
     if (i1 >= a.ctas) i1 = a.ctas - 1;
     const float* p = a.part + ((i0 + part + job) * BM + row) * BN + lane * 4;
-    const float* q = a.bias_part + (i0 + part + job) * BM + row;
+    const float* q = a.bias_part + (i0 + part + job) * 2 * BM + row;
     const int n = (int)(i1 - i0) - part;
 #pragma unroll 8
     for (int i = 0; i <= n; i += SUM_PARTS) {
@@ -362,7 +428,7 @@ __global__ void __launch_bounds__(SUM_ROWS * SUM_PARTS * 32) wgrad_sum_kernel(co
       sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
     if (bias && lane == 0)
-      for (int i = 0; i <= n; i += SUM_PARTS) bsum += q[(int64_t)i * BM];
+      for (int i = 0; i <= n; i += SUM_PARTS) bsum += q[(int64_t)i * 2 * BM] + q[(int64_t)i * 2 * BM + BM];
   }
   red[rr][part][lane] = sum;
   if (lane == 0) bred[rr][part] = bsum;
@@ -420,8 +486,8 @@ int run_wgrad(int ranks, int C, int H, int64_t n, const float* dv, const float* 
       return FC_ERR_UNSUPPORTED;
     constexpr int smem = WCfg<T>::SMEM;
     static Ready state;
-    if (int rc = ready(wgrad_kernel<T>, smem, state)) return rc;
-    wgrad_kernel<T><<<wa.ctas, THREADS, smem, s>>>(wm, wa);
+    if (int rc = ready(wgrad_kernel<T>, smem, state, W_REGS)) return rc;
+    wgrad_kernel<T><<<wa.ctas, W_THREADS, smem, s>>>(wm, wa);
     if (int rc = fc_check_launch()) return rc;
   }
   wgrad_sum_kernel<T><<<(unsigned)(2 * ranks * wa.n_ht * wa.n_ct * (BM / SUM_ROWS)), SUM_ROWS * SUM_PARTS * 32, 0,
