@@ -1,0 +1,139 @@
+"""Training blocks: element embedding, gated feed-forward and irreps dropout as modules.
+
+They hold the parameters of the layers they stand for under the same names, so a checkpoint of
+one loads into the other; :func:`use_training_blocks` puts them into a potential.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+
+from flashcart_b200 import ops
+from flashcart_b200.nn.layers import EquivariantGatedLayer, ProductPathWeights, _NoSpecialParameters
+
+
+class ScaledEmbedding(nn.Module):
+    """``offset + scale * weight[index]`` (parameter ``weight``, as ``nn.Embedding``); the
+    gradient is summed over sorted tokens, so equal batches give equal gradients."""
+
+    def __init__(self, n_types: int, features: int, scale: float = 1.0, offset: float = 0.0,
+                 weight: Optional[nn.Parameter] = None):
+        super().__init__()
+        if n_types <= 0 or features <= 0:
+            raise ValueError(f"n_types and features must be positive. Provided: {n_types}, {features}.")
+        if weight is not None and tuple(weight.shape) != (n_types, features):
+            raise ValueError(f"weight must be ({n_types}, {features}), got {tuple(weight.shape)}.")
+        self.n_types, self.features = n_types, features
+        self.scale, self.offset = float(scale), float(offset)
+        self.weight = nn.Parameter(torch.randn(n_types, features)) if weight is None else weight
+
+    @classmethod
+    def from_embedding(cls, emb: nn.Embedding, scale: float = 1.0, offset: float = 0.0) -> "ScaledEmbedding":
+        """The same table (shared, not copied)."""
+        return cls(emb.num_embeddings, emb.embedding_dim, scale, offset, weight=emb.weight)
+
+    def forward(self, index: torch.Tensor) -> torch.Tensor:
+        return ops.embedding(self.weight, index, self.scale, self.offset)
+
+    def extra_repr(self) -> str:
+        return f"{self.n_types}, {self.features}, scale={self.scale}, offset={self.offset}"
+
+
+class IrrepsDropout(_NoSpecialParameters, nn.Module):
+    """Dropout of whole irreps: one decision per (row, rank, channel), shared by the rank's
+    components, so the layer commutes with rotations. Every training call takes the next
+    offset of the seed's stream (device buffer ``rng`` = (seed, offset)); identity in
+    evaluation."""
+
+    def __init__(self, p: float, l_max: int = 0, seed: int = 0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError(f"p must lie in [0, 1]. Provided: {p}.")
+        self.p, self.l_max = float(p), int(l_max)
+        self.register_buffer("rng", torch.tensor([int(seed), 0], dtype=torch.int64), persistent=False)
+        self.register_buffer("advance", torch.tensor([0, 1], dtype=torch.int64), persistent=False)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if not self.training or self.p == 0.0:
+            return x
+        state = self.rng.clone()  # the gradient regenerates the mask from these two numbers
+        self.rng.add_(self.advance)
+        return ops.irreps_dropout(x, state, self.p, self.l_max)
+
+    def extra_repr(self) -> str:
+        return f"p={self.p}, l_max={self.l_max}"
+
+
+class GatedFeedForward(EquivariantGatedLayer):
+    """``EquivariantGatedLayer`` (reference ``nn/layers.py:543-648``: same constructor,
+    parameters and result) whose gate map, value map, activation and product are one kernel,
+    with one fused backward for all gradients; optionally dropout of the hidden irreps."""
+
+    def __init__(self, l_max: int, in_features: int, hidden_features: Optional[int] = None,
+                 gate_activation: str = "silu", gate_bias: bool = True, use_triton: bool = False,
+                 dropout: float = 0.0, seed: int = 0):
+        super().__init__(l_max, in_features, hidden_features, gate_activation, gate_bias, use_triton)
+        self.dropout = IrrepsDropout(dropout, l_max, seed)
+        self.register_buffer("scales", torch.cat([self.value_linear.scale.reshape(-1),
+                                                  self.gate_linear.scale.reshape(1),
+                                                  self.gate_activation.scale.reshape(1)]), persistent=False)
+
+    @classmethod
+    def from_layer(cls, layer: EquivariantGatedLayer, dropout: float = 0.0, seed: int = 0) -> "GatedFeedForward":
+        """The same parameters (shared, not copied)."""
+        with torch.random.fork_rng(devices=[]):  # the initial weights drawn here are thrown away
+            new = cls(layer.l_max, layer.in_features, layer.hidden_features, layer.gate_activation_name,
+                      layer.gate_bias, dropout=dropout, seed=seed)
+        new.value_linear, new.gate_linear = layer.value_linear, layer.gate_linear
+        new.output_linear, new.gate_activation = layer.output_linear, layer.gate_activation
+        new.scales = torch.cat([layer.value_linear.scale.reshape(-1), layer.gate_linear.scale.reshape(1),
+                                layer.gate_activation.scale.reshape(1)])
+        new.dropout.to(new.scales.device)
+        new.train(layer.training)
+        return new
+
+    def forward(self, node_feats: torch.Tensor) -> torch.Tensor:
+        if node_feats.shape[-1] != self.in_dim:
+            raise RuntimeError(f"Incorrect last dimension for node_feats. Expected {self.in_dim}, "
+                               f"got {node_feats.shape[-1]}.")
+        dtype = node_feats.dtype
+        cast = lambda w: w if w is None or w.dtype == dtype else w.to(dtype)
+        acc = torch.float64 if dtype == torch.float64 else torch.float32
+        hidden = ops.gated_feed_forward(node_feats, [cast(w) for w in self.value_linear.weight],
+                                        cast(self.gate_linear.weight), cast(self.gate_linear.bias),
+                                        self.scales.to(acc), self.l_max, self.gate_activation_name)
+        return self.output_linear(self.dropout(hidden), residual=node_feats)
+
+
+class _FusedPathWeights(ProductPathWeights):
+    """Element-dependent path weights ``1 + delta[type]`` in one lookup."""
+
+    def forward(self, atom_types=None):
+        if atom_types is None:
+            raise ValueError("atom_types required when n_elements is set.")
+        return ops.embedding(self.delta.weight, atom_types, 1.0, 1.0)
+
+
+def use_training_blocks(model: nn.Module, dropout: float = 0.0, seed: int = 0) -> nn.Module:
+    """Put the training blocks into a :class:`~flashcart_b200.model.flashcart.FlashCartPotential`
+    (in place; returned for convenience): the element embeddings, the element-dependent path
+    weights and the gated layers. Parameters, their names and the model's results stay the
+    same, up to rounding; ``dropout`` > 0 drops hidden irreps of the gated layers in training
+    mode (each layer has its own stream of ``seed``)."""
+    if isinstance(model.embedding, nn.Embedding):
+        model.embedding = ScaledEmbedding.from_embedding(model.embedding)
+    for inter in model.interactions:
+        if isinstance(inter.emb_i, nn.Embedding):
+            inter.emb_i = ScaledEmbedding.from_embedding(inter.emb_i)
+            inter.emb_j = ScaledEmbedding.from_embedding(inter.emb_j)
+    for product in model.products:
+        for weights in product.path_weights:
+            if weights.element_dependent:
+                weights.__class__ = _FusedPathWeights  # same attributes, another lookup
+    if model.nonlinearity:
+        for k, layer in enumerate(model.nonlinearities):
+            model.nonlinearities[k] = GatedFeedForward.from_layer(layer, dropout, seed + k)
+    return model
