@@ -410,7 +410,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
             }
           }
         }
-        // the slab is in registers: its stage may be refilled
+        // the slab is in registers once these loads are done: then its stage may be refilled. The
+        // arrival alone does not hold the copy that refills it behind loads still on their way (the
+        // last 16 bytes of some rows came from the next slab, in one product of 10^5).
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) arrive(smem_u32(&empty[s]));
         // (the first lap's wait is for the phase before the first and succeeds at once)

@@ -273,6 +273,22 @@ def test_gated_water_box_size(cuda_device, dtype):
         assert _rel(a, w) <= _gated_tol(dtype, c, 7 * n)
 
 
+@pytest.mark.parametrize("dtype,n,l_max,c,h", [(F32, 27648, 3, 128, 128), (BF16, 27648, 3, 128, 128),
+                                               (F32, 9001, 2, 200, 136), (BF16, 100003, 0, 96, 200)])
+def test_gated_large_passes_repeat_their_bits(cuda_device, dtype, n, l_max, c, h):
+    # one ring stage refilled while a few of its values are still being read shows in one product of
+    # 10^5: about one pass of three at these sizes, so a hundred passes show it
+    x, wv, wg, _, scales, g = R.gated_inputs(n, l_max, c, h, False, dtype, "cuda", seed=3)
+    for t in (x, wg, *wv):
+        t.requires_grad_(True)
+    want = None
+    for _ in range(100):
+        y = ops.gated_feed_forward(x, wv, wg, None, scales, l_max, "silu")
+        got = [y.detach(), *torch.autograd.grad(y, [x, wg, *wv], g)]
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_gated_subsets_of_gradients(cuda_device):
     x, wv, wg, b, sc, g = R.gated_inputs(300, 2, 64, 64, True, F32, "cuda")
     every = [x, wg, b, *wv]
