@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
     const int quarter = warp & 3, half = (warp - 8) >> 2;
     uint8_t* stage0 = epi + (warp - 8) * 2 * EPI_BUF;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(A_COLS + half * 64);
-    const float sa = MODE == DX ? 0.f : __ldg(a.act_scale);
+    const float sa = MODE == DX ? 0.f : __ldg(a.scales + a.ranks + 1);
     int64_t u = 0;
     int nbuf = 0;
     uint32_t aux_phase = 0;

@@ -1,5 +1,5 @@
 // Gated feed-forward block on tcgen05 tensor cores, fed by TMA (sm_100a): float32 rows as
-// 3xTF32 products, bfloat16 rows (exact in tf32) times weights in two tf32 parts.
+// 3xTF32 products (bfloat16 rows: gated_ff_bf16.cu, but for the input gradient).
 //
 // Mathematics and row layout: gated_ff.cu. The scales s_l, s_g are folded into the split
 // weights, so the accumulators hold v_k and z_l - b_l themselves.
@@ -59,12 +59,11 @@ constexpr int TC_REGS = 96;  // per thread at launch; the epilogue takes what th
 
 template <int MODE, typename T>
 struct Cfg {
-  static constexpr bool A32 = MODE == DX || sizeof(T) == 4;  // A in float32: hi and lo parts
-  static constexpr int TILE_A = BM * BK * (A32 ? 4 : 2);
-  static constexpr int A_STAGE = A32 ? 2 * BK : BK;  // tensor-memory columns
+  static constexpr int TILE_A = BM * BK * 4;
+  static constexpr int A_STAGE = 2 * BK;  // tensor-memory columns: hi and lo parts
   // Slots of the A ring. Even, so that a slot belongs to one splitter group and one MMA warp,
   // whose waits miss none of its barriers' phases. PRE keeps the gates' slopes behind them.
-  static constexpr int A_RING = MODE == PRE && A32 ? 2 : 4, Z_COL = 192;
+  static constexpr int A_RING = MODE == PRE ? 2 : 4, Z_COL = 192;
   static constexpr int BUFS = MODE == PRE ? 2 : 1;   // staging boxes per epilogue warp
   static constexpr int FIXED = EPI_WARPS * BUFS * EPI_BUF + BAR_BYTES + 1024;
   static_assert(A_RING * A_STAGE <= (MODE == PRE ? Z_COL : A_COLS) && A_COLS + NACC * ACC_W <= 512, "tensor memory");
@@ -73,28 +72,6 @@ struct Cfg {
   static int stages(int nk) { return std::min(MAX_STAGES, (SMEM_MAX - FIXED - 2 * nk * W_SLAB) / TILE_A) & ~1; }
   static int smem(int nk, int st) { return FIXED + 2 * nk * W_SLAB + st * TILE_A; }
 };
-
-// Work item: 128 rows, and rank l's components k0 .. k0+nm-1.
-struct Item {
-  int tile, l, k0, nm;
-};
-
-// Lists run through the ranks (high ones first: most work), all tiles of one before the next.
-__device__ __forceinline__ Item item_of(const Args& a, int it) {
-  Item w;
-  const int q = it / a.tiles;
-  w.tile = it - q * a.tiles;
-  if (a.per_comp) {
-    w.k0 = a.comps - 1 - q;
-    w.l = gated_rank_of(w.k0);
-    w.nm = 1;
-  } else {
-    w.l = a.L - q;
-    w.k0 = w.l * w.l;
-    w.nm = 2 * w.l + 1;
-  }
-  return w;
-}
 
 // An item's product passes: FWD, PRE the gate, then a value product per component, by the
 // rank's gate matrix (weight slot 0) and value matrix (slot 1), which stay until the rank
@@ -186,7 +163,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
     if (lane == 0) arrive(smem_u32(&sched_empty[s]));
     return it;
   };
-  auto passes_of = [&](const Item& w) { return MODE == DX ? (w.k0 == 0 ? a.ranks + 1 : w.nm) : 1 + w.nm; };
+  auto passes_of = [&](const WorkItem& w) { return MODE == DX ? (w.k0 == 0 ? a.ranks + 1 : w.nm) : 1 + w.nm; };
 
   if (warp < SPLIT_WARP0) {
     FC_SETMAXNREG_DEC(40);
@@ -208,7 +185,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
         arrive(smem_u32(&sched_full[s4]));
         if (it < 0) break;
         next = group + atomicAdd(a.counter + ct, 1);
-        const Item w = item_of(a, it);
+        const WorkItem w = work_item(a, it);
         const int passes = passes_of(w);
         for (int p = 0; p < passes && ok; ++p) {
           const bool gates = MODE == DX && w.k0 == 0 && p > 0;
@@ -220,7 +197,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
             tma_prefetch_3d(&mp.ap, 0, w.tile * BM, zn);
             if (MODE == PRE) tma_prefetch_3d(&mp.gp, ct * BN, w.tile * BM, zn);
           } else if (p + 1 == passes && next < a.items) {
-            const Item wn = item_of(a, next);
+            const WorkItem wn = work_item(a, next);
             tma_prefetch_3d(&mp.ap, 0, wn.tile * BM, MODE == DX ? wn.k0 : 0);
           }
           for (int kt = 0; kt < nk; ++kt, ++g) {
@@ -264,7 +241,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
       for (int q = 0; ok; ++q) {
         const int it = item_one(q);
         if (it < 0) break;
-        const Item w = item_of(a, it);
+        const WorkItem w = work_item(a, it);
         if (cycle && w.k0 == 0) {
           for (int p = 0; p <= a.ranks && ok; ++p) {
             const int mat = p == 0 ? 0 : a.ranks + p - 1;
@@ -307,7 +284,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
       for (int q = 0; ok; ++q) {
         const int it = item_warp(q);
         if (it < 0) break;
-        const Item w = item_of(a, it);
+        const WorkItem w = work_item(a, it);
         const int passes = passes_of(w);
         const bool through = cycle && w.k0 == 0;
         if (through) {
@@ -345,7 +322,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
 #pragma unroll
               for (int kk = 0; kk < BK / 8; ++kk) {
                 mma_ta<BN>(d, tah + kk * 8, db + W_LO + 2 * kk, (kt > first || kk > 0) ? 1u : 0u);
-                if (C::A32) mma_ta<BN>(d, tal + kk * 8, db + 2 * kk, 1u);
+                mma_ta<BN>(d, tal + kk * 8, db + 2 * kk, 1u);
               }
 #pragma unroll
               for (int kk = 0; kk < BK / 8; ++kk) mma_ta<BN>(d, tah + kk * 8, db + 2 * kk, 1u);
@@ -387,29 +364,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
     for (int q = 0; ok; ++q) {
       const int it = item_warp(q);
       if (it < 0) break;
-      left += passes_of(item_of(a, it)) * nk;
+      left += passes_of(work_item(a, it)) * nk;
       for (; left > 0; left -= 2) {
         if (!full_ready) ok = wait_warp(smem_u32(&full[s]), lap & 1u, abort_flag);
         if (!ok) break;
         const uint8_t* slab = ring + s * C::TILE_A;
         const uint32_t ta = tmem + ((uint32_t)((warp & 3) * 32) << 16) + as * (uint32_t)C::A_STAGE;
         uint32_t x[32];
-        if constexpr (C::A32) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            *reinterpret_cast<uint4*>(&x[4 * c]) = *reinterpret_cast<const uint4*>(slab + chunk_at<float>(r, c));
-        } else {  // bfloat16 is a tf32 value: its bits are the high half
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint4 v = *reinterpret_cast<const uint4*>(slab + chunk_at<bf16_t>(r, c));
-            const uint32_t vs[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[8 * c + 2 * e] = vs[e] << 16;
-              x[8 * c + 2 * e + 1] = vs[e] & 0xFFFF0000u;
-            }
-          }
-        }
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(&x[4 * c]) = *reinterpret_cast<const uint4*>(slab + chunk_at<float>(r, c));
         // the slab is in registers once these loads are done: then its stage may be refilled. The
         // arrival alone does not hold the copy that refills it behind loads still on their way (the
         // last 16 bytes of some rows came from the next slab, in one product of 10^5).
@@ -433,11 +397,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
         const bool peek_full = peek_parity(smem_u32(&full[s_next]), lap_next & 1u);
         const bool peek_slot = peek_parity(smem_u32(&a_free[as_next]), (as_lap_next & 1u) ^ 1u);
         asm volatile("tcgen05.fence::after_thread_sync;");
-        if constexpr (C::A32) {
-          store_parts(ta, x);  // three operations an element: issue slots are short here
-        } else {
-          tmem_st32(ta, x);
-        }
+        store_parts(ta, x);  // three operations an element: issue slots are short here
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
@@ -458,7 +418,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
     uint8_t* boxes = epi + (warp - EPI_WARP0) * C::BUFS * EPI_BUF;
     uint64_t* landed = aux + (warp - EPI_WARP0) * C::BUFS;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(A_COLS + half * 32);
-    const float sa = MODE == DX ? 0.f : __ldg(a.act_scale);
+    const float sa = MODE == DX ? 0.f : __ldg(a.scales + a.ranks + 1);
     const int col = ct * BN + half * 32;
     const bool live = col < a.N;  // the warp has columns to write
     uint32_t ab = 0, acc_phase = 0;  // the accumulator in turn
@@ -511,7 +471,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
     for (int q = 0; ok; ++q) {
       const int it = item_warp(q);
       if (it < 0) break;
-      const Item w = item_of(a, it);
+      const WorkItem w = work_item(a, it);
       const int row0 = w.tile * BM + quarter * 32;
       if constexpr (MODE == DX) {
         float acc[32];
@@ -606,12 +566,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
                 ok = false;
               }
               uint8_t* buf = boxes + box * EPI_BUF;
-              uint4 raw[sizeof(T) == 2 ? 4 : 1];
-              if constexpr (sizeof(T) == 2) {  // rows of g and of dv differ in width: all of g first
-#pragma unroll
-                for (int c = 0; c < 4; ++c) raw[c] = *reinterpret_cast<const uint4*>(buf + chunk_at<T>(lane, c));
-                __syncwarp();
-              }
 #pragma unroll
               for (int h = 0; h < 2; ++h) {
                 float v[16];
@@ -619,17 +573,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
 #pragma unroll
                 for (int c4 = 0; c4 < 4; ++c4) {
                   float4* at = reinterpret_cast<float4*>(buf + chunk_at<float>(lane, h * 4 + c4));
-                  float gv[4];
-                  if constexpr (sizeof(T) == 4) {
-                    const float4 t = *at;
-                    gv[0] = t.x, gv[1] = t.y, gv[2] = t.z, gv[3] = t.w;
-                  } else {
-                    const int e0 = h * 16 + c4 * 4;  // element of the row
-                    const uint4 t = raw[e0 / 8];
-                    const uint32_t lo = (e0 % 8) ? t.z : t.x, hi = (e0 % 8) ? t.w : t.y;
-                    gv[0] = __uint_as_float(lo << 16), gv[1] = __uint_as_float(lo & 0xFFFF0000u);
-                    gv[2] = __uint_as_float(hi << 16), gv[3] = __uint_as_float(hi & 0xFFFF0000u);
-                  }
+                  const float4 t = *at;
+                  const float gv[4] = {t.x, t.y, t.z, t.w};
                   float o[4];
 #pragma unroll
                   for (int e = 0; e < 4; ++e) {
@@ -690,8 +635,9 @@ constexpr int MAX_LISTS = 160;  // work lists of a launch: one per 64 output cha
 // hidden, k = input channel; dx: the transpose. Also zeroes the work lists' counters.
 struct PrepArgs {
   GatedArgs g;
-  float* fwd;  // or null
-  float* dx;   // or null
+  float* fwd;      // or null
+  bf16_t* direct;  // or null: in place of fwd, the weights as they are, in rows padded with zeros
+  float* dx;       // or null
   int* counters;
 };
 
@@ -703,11 +649,16 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs p) {
   const T* w = q < ranks ? (const T*)p.g.wv[l] : (const T*)p.g.wg + (int64_t)l * H * C;
   const float sc = ((const float*)p.g.scales)[q < ranks ? l : ranks];
   const int cp = (C + 3) & ~3, hp = (H + 3) & ~3;
-  const int64_t nf = p.fwd ? (int64_t)H * cp : 0, nd = p.dx ? (int64_t)C * hp : 0;
+  const int c8 = (C + 7) & ~7;
+  const int64_t nf = p.direct ? (int64_t)H * c8 : p.fwd ? (int64_t)H * cp : 0, nd = p.dx ? (int64_t)C * hp : 0;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < nf + nd; i += (int64_t)gridDim.x * 256) {
     const bool f = i < nf;
     const int64_t e = f ? i : i - nf, size = f ? nf : nd;
-    const int kp = f ? cp : hp, r = (int)(e / kp), k = (int)(e - (int64_t)r * kp);
+    const int kp = f ? (p.direct ? c8 : cp) : hp, r = (int)(e / kp), k = (int)(e - (int64_t)r * kp);
+    if (f && p.direct) {
+      p.direct[q * size + e] = k < C ? Io<bf16_t>::put(Io<T>::get(w[(int64_t)r * C + k])) : Io<bf16_t>::put(0.f);
+      continue;
+    }
     float x = 0.f;
     if (k < (f ? C : H)) x = sc * Io<T>::get(f ? w[(int64_t)r * C + k] : w[(int64_t)k * C + r]);
     const float hi = round_tf32(x);
@@ -752,22 +703,25 @@ bool encode_rows(CUtensorMap* map, const void* base, int64_t channels, int64_t r
   const cuuint32_t unit[3] = {1, 1, 1};
   return encode_fn()(map, sizeof(E) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                      const_cast<void*>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     box_c != 32        ? CU_TENSOR_MAP_SWIZZLE_NONE
-                     : sizeof(E) == 4 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                      : CU_TENSOR_MAP_SWIZZLE_64B,
+                     box_c * sizeof(E) == 128  ? CU_TENSOR_MAP_SWIZZLE_128B
+                     : box_c * sizeof(E) == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                               : CU_TENSOR_MAP_SWIZZLE_NONE,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template bool encode_rows<float>(CUtensorMap*, const void*, int64_t, int64_t, int64_t, int64_t, int, int);
 template bool encode_rows<bf16_t>(CUtensorMap*, const void*, int64_t, int64_t, int64_t, int64_t, int, int);
 
-static bool encode_weights(CUtensorMap* map, const float* base, int kp, int out, int mats, int box_rows) {
+// (k, output channel, matrix) map of weights in 128-byte boxes.
+template <typename E>
+static bool encode_weights(CUtensorMap* map, const E* base, int kp, int out, int mats, int box_rows) {
   const cuuint64_t dims[3] = {(cuuint64_t)kp, (cuuint64_t)out, (cuuint64_t)mats};
-  const cuuint64_t strides[2] = {(cuuint64_t)kp * 4, (cuuint64_t)kp * out * 4};
-  const cuuint32_t box[3] = {32, (cuuint32_t)box_rows, 1};
+  const cuuint64_t strides[2] = {(cuuint64_t)kp * sizeof(E), (cuuint64_t)kp * out * sizeof(E)};
+  const cuuint32_t box[3] = {128 / sizeof(E), (cuuint32_t)box_rows, 1};
   const cuuint32_t unit[3] = {1, 1, 1};
-  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, const_cast<float*>(base), dims, strides, box, unit,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return encode_fn()(map, sizeof(E) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                     const_cast<E*>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -779,12 +733,8 @@ static int sm_count() {
   return sms[dev];
 }
 
-// Whether the products of a reduction over K into N columns keep their weights in shared memory.
-static bool resident(int K, int N, int sms) { return K <= MAX_NK * BK && (N + BN - 1) / BN <= std::min(sms, MAX_LISTS); }
-
 template <int MODE, typename T>
-static int run_products(const Maps& mp, Args a, int K, int sms, cudaStream_t s) {
-  if (!resident(K, a.N, sms)) return run_stream<MODE, T>(mp, a, sms, s);
+static int run_resident(const Maps& mp, Args a, int sms, cudaStream_t s) {
   using C = Cfg<MODE, T>;
   a.stages = C::stages(a.nk);
   static Ready state;
@@ -792,6 +742,27 @@ static int run_products(const Maps& mp, Args a, int K, int sms, cudaStream_t s) 
   const int lists = (int)std::min<int64_t>(a.items, sms / a.n_ct);
   gated_tc_kernel<MODE, T><<<lists * a.n_ct, TC_THREADS, C::smem(a.nk, a.stages), s>>>(mp, a);
   return fc_check_launch();
+}
+
+// A column tile has its work list, and every list some CTAs.
+static bool one_list_each(int N, int sms) { return (N + BN - 1) / BN <= std::min(sms, MAX_LISTS); }
+
+// Whether the products of a reduction over K into N columns keep their weights in shared memory.
+static bool resident(int K, int N, int sms) { return K <= MAX_NK * BK && one_list_each(N, sms); }
+
+// Whether the forward (and the backward's first half) multiplies bfloat16 as it is.
+template <typename T>
+static bool direct(int K, int N, int sms) {
+  return sizeof(T) == 2 && K <= DIRECT_K && one_list_each(N, sms);
+}
+
+template <int MODE, typename T>
+static int run_products(const Maps& mp, const Args& a, int K, int sms, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2 && MODE != DX) {
+    return direct<T>(K, a.N, sms) ? run_direct<MODE>(mp, a, sms, s) : run_stream<MODE, T>(mp, a, sms, s);
+  } else {
+    return resident(K, a.N, sms) ? run_resident<MODE, T>(mp, a, sms, s) : run_stream<MODE, T>(mp, a, sms, s);
+  }
 }
 
 // Layout of the workspace (bytes), the same for the size query and the call.
@@ -850,15 +821,17 @@ static int repitch(const T* src, int64_t src_ld, T* dst, int64_t dst_ld, int wid
   return fc_check_launch();
 }
 
+template <typename T>
 static Args product_args(const GatedArgs& g, int N, int K, int mode, int sms) {
   Args a{};
   a.L = g.L;
   a.ranks = g.L + 1;
   a.comps = a.ranks * a.ranks;
   a.N = N;
-  a.nk = (K + BK - 1) / BK;
+  const bool dir = mode != DX && direct<T>(K, N, sms);
+  a.nk = dir ? (K + DIRECT_BK - 1) / DIRECT_BK : (K + BK - 1) / BK;
   a.tiles = (int)((g.n + BM - 1) / BM);
-  const bool res = resident(K, N, sms);
+  const bool res = dir || (resident(K, N, sms) && (sizeof(T) == 4 || mode == DX));
   a.n_ct = res ? (N + BN - 1) / BN : (N + STREAM_BN - 1) / STREAM_BN;
   // with fewer (tile, rank) groups than SMs the components are items of their own (the gate is
   // computed again for each); PRE needs a rank's components together
@@ -875,20 +848,33 @@ static Args product_args(const GatedArgs& g, int N, int K, int mode, int sms) {
   }
   a.act = g.act;
   a.bias = g.bias;
-  a.act_scale = (const float*)g.scales + a.ranks + 1;
+  a.scales = (const float*)g.scales;
   a.status = g.status;
   return a;
 }
 
-static int weight_rows(int K, int N, int sms) { return resident(K, N, sms) ? BN : STREAM_BN; }
-
 template <typename T>
-static int run_prep(const GatedArgs& g, float* fwd, float* dx, int* counters, cudaStream_t s) {
-  const int64_t cp = (g.C + 3) & ~3, hp = (g.H + 3) & ~3;
-  const int64_t each = (fwd ? g.H * cp : 0) + (dx ? g.C * hp : 0);
-  const PrepArgs p{g, fwd, dx, counters};
+static int run_prep(const GatedArgs& g, void* fwd, float* dx, int* counters, int sms, cudaStream_t s) {
+  const int64_t cp = (g.C + 3) & ~3, c8 = (g.C + 7) & ~7, hp = (g.H + 3) & ~3;
+  const bool dir = direct<T>(g.C, g.H, sms);
+  const int64_t each = g.H * (dir ? c8 : cp) + (dx ? g.C * hp : 0);
+  const PrepArgs p{g, dir ? nullptr : (float*)fwd, dir ? (bf16_t*)fwd : nullptr, dx, counters};
   prep_kernel<T><<<dim3((unsigned)std::min<int64_t>((each + 255) / 256, 256), 2 * (g.L + 1)), 256, 0, s>>>(p);
   return fc_check_launch();
+}
+
+// The maps of x and of the weights that the forward products read.
+template <typename T>
+static bool encode_forward(Maps& mp, const GatedArgs& g, const Rows<T>& x, const void* weights, int sms) {
+  const int ranks = g.L + 1, comps = ranks * ranks;
+  if (direct<T>(g.C, g.H, sms))
+    return encode_rows<T>(&mp.a, x.p, g.C, g.n, comps, x.ld, DIRECT_BK, BM) &&
+           encode_rows<T>(&mp.ap, x.p, g.C, g.n, comps, x.ld, DIRECT_K, BM) &&
+           encode_weights<bf16_t>(&mp.b, (const bf16_t*)weights, (g.C + 7) & ~7, g.H, 2 * ranks, BN);
+  return encode_rows<T>(&mp.a, x.p, g.C, g.n, comps, x.ld, BK, BM) &&
+         encode_rows<T>(&mp.ap, x.p, g.C, g.n, comps, x.ld, MAX_NK * BK, BM) &&
+         encode_weights<float>(&mp.b, (const float*)weights, (g.C + 3) & ~3, g.H, 4 * ranks,
+                               sizeof(T) == 4 && resident(g.C, g.H, sms) ? BN : STREAM_BN);
 }
 
 }  // namespace gtc
@@ -909,15 +895,11 @@ int gated_tc_fwd(const GatedArgs& a, cudaStream_t s) {
   if (x.copied)
     if (int rc = repitch<T>((const T*)a.x, a.C, const_cast<T*>(x.p), x.ld, a.C, a.n * comps, s)) return rc;
   int* counters = (int*)(ws + w.counters);
-  float* weights = (float*)(ws + w.fwd);
-  if (int rc = run_prep<T>(a, weights, nullptr, counters, s)) return rc;
-  Args args = product_args(a, a.H, a.C, FWD, sms);
+  if (int rc = run_prep<T>(a, ws + w.fwd, nullptr, counters, sms, s)) return rc;
+  Args args = product_args<T>(a, a.H, a.C, FWD, sms);
   args.counter = counters;
   Maps mp;
-  if (!encode_rows<T>(&mp.a, x.p, a.C, a.n, comps, x.ld, BK, BM) ||
-      !encode_weights(&mp.b, weights, (a.C + 3) & ~3, a.H, 4 * ranks, weight_rows(a.C, a.H, sms)) ||
-      !encode_rows<T>(&mp.ap, x.p, a.C, a.n, comps, x.ld, MAX_NK * BK, BM) ||
-      !encode_rows<T>(&mp.o, y.p, a.H, a.n, comps, y.ld, 32, 32))
+  if (!encode_forward<T>(mp, a, x, ws + w.fwd, sms) || !encode_rows<T>(&mp.o, y.p, a.H, a.n, comps, y.ld, 32, 32))
     return FC_ERR_UNSUPPORTED;
   mp.a2 = mp.g = mp.gp = mp.o2 = mp.o;  // not used
   if (int rc = run_products<FWD, T>(mp, args, a.C, sms, s)) return rc;
@@ -936,7 +918,7 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
   uint8_t* ws = (uint8_t*)a.ws;
   const Rows<T> x = rows_of<T>(a.x, a.C, ws + w.x), gy = rows_of<T>(a.gy, a.H, ws + w.y);
   int* counters = (int*)(ws + w.counters);
-  float *fwd = (float*)(ws + w.fwd), *dx = (float*)(ws + w.dx), *dv = (float*)(ws + w.dv), *dz = (float*)(ws + w.dz);
+  float *dx = (float*)(ws + w.dx), *dv = (float*)(ws + w.dv), *dz = (float*)(ws + w.dz);
   bool any = a.gwg || a.gbias;
   for (int l = 0; l < ranks; ++l) any = any || a.gwv[l];
   if (a.n > 0) {
@@ -944,18 +926,16 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
       if (int rc = repitch<T>((const T*)a.x, a.C, const_cast<T*>(x.p), x.ld, a.C, a.n * comps, s)) return rc;
     if (gy.copied)
       if (int rc = repitch<T>((const T*)a.gy, a.H, const_cast<T*>(gy.p), gy.ld, a.H, a.n * comps, s)) return rc;
-    if (int rc = run_prep<T>(a, fwd, a.gx ? dx : nullptr, counters, s)) return rc;
+    if (int rc = run_prep<T>(a, ws + w.fwd, a.gx ? dx : nullptr, counters, sms, s)) return rc;
     Maps mp;
-    if (!encode_rows<T>(&mp.a, x.p, a.C, a.n, comps, x.ld, BK, BM) ||
-        !encode_weights(&mp.b, fwd, (a.C + 3) & ~3, a.H, 4 * ranks, weight_rows(a.C, a.H, sms)) ||
+    if (!encode_forward<T>(mp, a, x, ws + w.fwd, sms) ||
         !encode_rows<float>(&mp.o, dv, a.H, a.n, comps, hp, 32, 32) ||
         !encode_rows<T>(&mp.g, gy.p, a.H, a.n, comps, gy.ld, 32, 32) ||
         !encode_rows<T>(&mp.gp, gy.p, a.H, a.n, comps, gy.ld, BN, BM) ||
-        !encode_rows<T>(&mp.ap, x.p, a.C, a.n, comps, x.ld, MAX_NK * BK, BM) ||
         !encode_rows<float>(&mp.o2, dz, a.H, a.n, ranks, hp, 32, 32))
       return FC_ERR_UNSUPPORTED;
     mp.a2 = mp.o2;  // not used
-    Args args = product_args(a, a.H, a.C, PRE, sms);
+    Args args = product_args<T>(a, a.H, a.C, PRE, sms);
     args.counter = counters;
     if (int rc = run_products<PRE, T>(mp, args, a.C, sms, s)) return rc;
     if (a.gx) {
@@ -964,11 +944,11 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
       if (!encode_rows<float>(&md.a, dv, a.H, a.n, comps, hp, BK, BM) ||
           !encode_rows<float>(&md.ap, dv, a.H, a.n, comps, hp, MAX_NK * BK, BM) ||
           !encode_rows<float>(&md.a2, dz, a.H, a.n, ranks, hp, BK, BM) ||
-          !encode_weights(&md.b, dx, (int)hp, a.C, 4 * ranks, weight_rows(a.H, a.C, sms)) ||
+          !encode_weights<float>(&md.b, dx, (int)hp, a.C, 4 * ranks, resident(a.H, a.C, sms) ? BN : STREAM_BN) ||
           !encode_rows<T>(&md.o, gx.p, a.C, a.n, comps, gx.ld, 32, 32))
         return FC_ERR_UNSUPPORTED;
       md.g = md.gp = md.o2 = md.o;  // not used
-      Args dargs = product_args(a, a.C, a.H, DX, sms);
+      Args dargs = product_args<T>(a, a.C, a.H, DX, sms);
       dargs.counter = counters + MAX_LISTS;
       if (int rc = run_products<DX, T>(md, dargs, a.H, sms, s)) return rc;
       if (gx.copied)

@@ -11,6 +11,8 @@ namespace gtc {
 using namespace tma;
 
 constexpr int BK = 32, THREADS = 512;
+// Reductions of bfloat16 rows and weights up to this length take the kernel without splitting.
+constexpr int DIRECT_K = 256, DIRECT_BK = 64;
 constexpr int EPI_BUF = 4096;  // a warp's 32 x 32 float staging box
 constexpr int BAR_BYTES = 640;
 constexpr int SCHED = 4;  // work items handed out ahead
@@ -26,7 +28,7 @@ struct Args {
   int stages;             // A stages (resident kernel)
   int act;
   const void* bias;       // of the rows' type, or null
-  const float* act_scale;
+  const float* scales;    // one per rank, the gate map's, the activation's
   int* counter;           // work lists, zeroed before the launch
   int* status;
 };
@@ -42,20 +44,44 @@ struct Maps {
   CUtensorMap o2;  // dz (PRE)
 };
 
+// Work item: 128 rows, and rank l's components k0 .. k0+nm-1.
+struct WorkItem {
+  int tile, l, k0, nm;
+};
+
+// Lists run through the ranks (high ones first: most work), all tiles of one before the next.
+__device__ __forceinline__ WorkItem work_item(const Args& a, int it) {
+  WorkItem w;
+  const int q = it / a.tiles;
+  w.tile = it - q * a.tiles;
+  if (a.per_comp) {
+    w.k0 = a.comps - 1 - q;
+    w.l = gated_rank_of(w.k0);
+    w.nm = 1;
+  } else {
+    w.l = a.L - q;
+    w.k0 = w.l * w.l;
+    w.nm = 2 * w.l + 1;
+  }
+  return w;
+}
+
+// N consecutive columns of this thread's lane (warp-collective), waited for in the same statement:
+// nothing that uses the values can come before the wait.
 template <int N>
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, float* f);
 template <>
 __device__ __forceinline__ void tmem_ld<32>(uint32_t taddr, float* f) {
   uint32_t v[32];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
         "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
         "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      : "r"(taddr)
+      : "memory");
 #pragma unroll
   for (int c = 0; c < 32; ++c) f[c] = __uint_as_float(v[c]);
 }
@@ -63,11 +89,12 @@ template <>
 __device__ __forceinline__ void tmem_ld<16>(uint32_t taddr, float* f) {
   uint32_t v[16];
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
         "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+      : "r"(taddr)
+      : "memory");
 #pragma unroll
   for (int c = 0; c < 16; ++c) f[c] = __uint_as_float(v[c]);
 }
@@ -253,6 +280,8 @@ static int ready(K kernel, int smem, Ready& r, int regs = 128) {
 // Launchers of the other files.
 constexpr int STREAM_BN = 128;  // output columns of a tile: streaming kernel
 constexpr int STREAM_KG = 2, STREAM_NACC = 3;
+template <int MODE>
+int run_direct(const Maps& mp, Args a, int sms, cudaStream_t s);
 template <int MODE, typename T>
 int run_stream(const Maps& mp, const Args& a, int sms, cudaStream_t s);
 
@@ -267,7 +296,7 @@ int run_wgrad(int ranks, int C, int H, int64_t n, const float* dv, const float* 
               int64_t x_ld, float* part, float* bias_part, const WOut& o, int* status, int sms, cudaStream_t s);
 
 // (channel, row, component) map of a tensor of rows [comps][ld]; box_c channels x box_r rows,
-// 32-channel boxes with the 128- or 64-byte swizzle of their row width.
+// boxes of 128- or 64-byte rows with that swizzle.
 template <typename E>
 bool encode_rows(CUtensorMap* map, const void* base, int64_t channels, int64_t rows, int64_t comps, int64_t ld,
                  int box_c, int box_r);
