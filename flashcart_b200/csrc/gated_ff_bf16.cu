@@ -76,6 +76,24 @@ __device__ __forceinline__ float brief_sigmoid(float z) {
   return s;
 }
 
+// Eight floats as two bfloat16 parts, the upper halves of their bits and the rest rounded (16
+// significant bits in a float's size), the second PART bytes behind the first: what the
+// backward's second half multiplies.
+constexpr int PART = 2048;
+__device__ __forceinline__ void put_parts(uint8_t* at, const float* f) {
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t b0 = __float_as_uint(f[2 * k]), b1 = __float_as_uint(f[2 * k + 1]);
+    const float r0 = f[2 * k] - __uint_as_float(b0 & 0xFFFF0000u);
+    const float r1 = f[2 * k + 1] - __uint_as_float(b1 & 0xFFFF0000u);
+    hi[k] = __byte_perm(b0, b1, 0x7632);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo[k]) : "f"(r1), "f"(r0));
+  }
+  *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+  *reinterpret_cast<uint4*>(at + PART) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
 template <int MODE>
 __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_constant__ Maps mp, const Args a) {
   using C = DCfg<MODE>;
@@ -140,7 +158,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
       int s = 0;
       uint32_t lap = 0;  // of the ring
       int64_t g = 0;
-      bool ok = true;
+      bool ok = true, free = true;  // (peeked: the next stage is free)
       for (int it = first; it < items && ok; it += lists) {
         const WorkItem w = work_item(a, it);
         const int lead = w.k0 == 0 ? 0 : 1;  // passes before the first component's
@@ -155,17 +173,18 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
             if (MODE == PRE) tma_prefetch_3d(&mp.gp, ct * BN, wn.tile * BM, wn.k0);
           }
           for (int kt = 0; kt < nk; ++kt, ++g) {
-            if (lap > 0 && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
+            if (!free && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
               ok = false;
               break;
             }
+            const int s_next = s + 1 == S ? 0 : s + 1;
+            const uint32_t lap_next = s_next ? lap : lap + 1;
+            free = lap_next == 0 || peek_parity(smem_u32(&empty[s_next]), (lap_next - 1) & 1u);
             const uint32_t fb = smem_u32(&full[s]);
             arrive_tx(fb, TILE_A);
             tma_load_3d(smem_u32(ring + s * TILE_A), &mp.a, kt * DIRECT_BK, w.tile * BM, z, fb);
-            if (++s == S) {
-              s = 0;
-              ++lap;
-            }
+            s = s_next;
+            lap = lap_next;
           }
         }
       }
@@ -312,6 +331,17 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
       }
       __syncwarp();
     };
+    // the same of both parts' boxes
+    auto send_parts = [&](const CUtensorMap* map, uint8_t* buf, int row, int z) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (elect_one()) {
+        tma_store_3d(map, smem_u32(buf), col, row, z);
+        tma_store_3d(map, smem_u32(buf + PART), col, row, z + 1);
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      }
+      __syncwarp();
+    };
     // earlier stores have read their boxes (box_free: all but the last one)
     auto boxes_free = [&]() {
       if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -423,38 +453,32 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
               ok = false;
             }
             uint8_t* buf = boxes + box * C::BOX;
-            uint4 raw[4];  // rows of g and of dv differ in width: all of g first
-#pragma unroll
-            for (int c = 0; c < 4; ++c) raw[c] = *reinterpret_cast<const uint4*>(buf + chunk_at<bf16_t>(lane, c));
-            __syncwarp();
+            // the rows of dv's high parts take the place of g's, chunk by chunk
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float v[16], gate[16];
               tmem_ld<16>(acc_at() + h * 16, v);
               tmem_ld<16>(gate_at + h * 16, gate);
 #pragma unroll
-              for (int c4 = 0; c4 < 4; ++c4) {
-                const int e0 = h * 16 + c4 * 4;  // element of the row
-                const uint4 t = raw[e0 / 8];
-                const uint32_t lo = (e0 % 8) ? t.z : t.x, hi = (e0 % 8) ? t.w : t.y;
-                const float gv[4] = {__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u),
-                                     __uint_as_float(hi << 16), __uint_as_float(hi & 0xFFFF0000u)};
-                float o[4];
+              for (int c8 = 0; c8 < 2; ++c8) {
+                uint8_t* at = buf + chunk_at<bf16_t>(lane, h * 2 + c8);
+                Pack<bf16_t, 8> gp;
+                gp.raw = *reinterpret_cast<const uint4*>(at);
+                float o[8];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const int c = e0 + k;
-                  sum[c] += gv[k] * v[c4 * 4 + k];
-                  o[k] = gv[k] * gate[c4 * 4 + k];
+                for (int k = 0; k < 8; ++k) {
+                  const float gv = Io<bf16_t>::get(gp.at(k));
+                  sum[h * 16 + c8 * 8 + k] += gv * v[c8 * 8 + k];
+                  o[k] = gv * gate[c8 * 8 + k];
                 }
-                *reinterpret_cast<float4*>(buf + chunk_at<float>(lane, h * 4 + c4)) =
-                    make_float4(o[0], o[1], o[2], o[3]);
+                put_parts(at, o);
               }
             }
             if (m + 1 < w.nm && ok) {
               boxes_free();  // the other box: its store is a component old
               ask(m + 1, box ^ 1u);
             }
-            send(&mp.o, buf, row0, w.k0 + m);
+            send_parts(&mp.o, buf, row0, 2 * (w.k0 + m));
             box ^= 1u;
           }
           free_acc();
@@ -471,9 +495,11 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
             tmem_ld<16>(z_at + h * 16, zz);
 #pragma unroll
             for (int c = 0; c < 16; ++c) sum[h * 16 + c] *= zz[c];
+#pragma unroll
+            for (int c8 = 0; c8 < 2; ++c8)
+              put_parts(boxes + box * C::BOX + chunk_at<bf16_t>(lane, h * 2 + c8), sum + h * 16 + c8 * 8);
           }
-          put_row<float>(boxes + box * C::BOX, lane, sum);
-          send(&mp.o2, boxes + box * C::BOX, row0, w.l);
+          send_parts(&mp.o2, boxes + box * C::BOX, row0, 2 * w.l);
           box ^= 1u;
         }
       }
@@ -490,7 +516,293 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
   }
 }
 
+// ---------------------------------------------------------------------------- input gradient
+//
+// dx_k = s_l dv_k Wv_l (+ s_g sum_l dz_l Wg_l for k = 0) from the two bfloat16 parts of dv and dz
+// and the transposed weights, a component's products all in one accumulator (the gates' in a
+// second one: their scale is another). An item is one rank of 128 rows and 128 input channels, so
+// dv and dz, twice the size of everything else, are read once up to 128 channels.
+//
+// What bounds it: DRAM (179 MB for 100,003 rows of 96 <- 200 channels, 28 us at the copy rate).
+//
+// The 12 warps: 0 TMA producer of A slabs, 1 MMA issue, 2 TMA producer of the weights, 4-11
+// epilogue (two per lane quarter, 64 columns each).
+constexpr int X_BN = DIRECT_DX_BN, X_SLAB = X_BN * 128, X_NACC = 4, X_STAGES = 4, X_THREADS = 12 * 32, X_BOX = 2048;
+constexpr int X_FIXED = 8 * 2 * X_BOX + X_STAGES * TILE_A + BAR_BYTES + 1024;
+static_assert(X_FIXED + 2 * MAX_NK * X_SLAB <= SMEM_MAX, "shared memory per CTA");
+
+// The matrix of an item's pass p and the weight slot that holds it. Slots: a matrix stays until
+// the other one has been used and a third is wanted. What a scalar item of several ranks multiplies
+// by (a value matrix, then every rank's gates) is used once and given back at once.
+struct Slots {
+  int held[2] = {-1, -1};
+  int last = 1;
+  // slot of matrix m; fresh: it has to be loaded
+  __device__ __forceinline__ int of(int m, bool& fresh) {
+    fresh = false;
+    if (held[0] == m) return last = 0;
+    if (held[1] == m) return last = 1;
+    fresh = true;
+    last ^= 1;
+    if (last) held[1] = m;
+    else held[0] = m;
+    return last;
+  }
+  __device__ __forceinline__ void drop(int slot) {
+    if (slot) held[1] = -1;
+    else held[0] = -1;
+  }
+};
+
+__global__ void __launch_bounds__(X_THREADS, 1) gated_bf16_dx_kernel(const __grid_constant__ Maps mp, const Args a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int nk = a.nk;
+  uint8_t* wmem = smem;                       // [slot][k slab]
+  uint8_t* ring = wmem + 2 * nk * X_SLAB;     // A stages
+  uint8_t* epi = ring + X_STAGES * TILE_A;    // staging boxes
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi + 8 * 2 * X_BOX);
+  uint64_t* empty = full + X_STAGES;
+  uint64_t* w_full = empty + X_STAGES;        // per slot
+  uint64_t* w_free = w_full + 2;
+  uint64_t* acc_full = w_free + 2;
+  uint64_t* acc_empty = acc_full + X_NACC;
+  uint64_t* drain = acc_empty + X_NACC;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 * X_STAGES + 4 + 2 * X_NACC + 1) * 8 + 8 <= BAR_BYTES, "barriers");
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (threadIdx.x == 32) {
+    auto init = [](uint64_t* b, int n) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n));
+    };
+    for (int s = 0; s < X_STAGES; ++s) {
+      init(&full[s], 1);
+      init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      init(&w_full[b], 1);
+      init(&w_free[b], 1);
+    }
+    for (int b = 0; b < X_NACC; ++b) {
+      init(&acc_full[b], 1);
+      init(&acc_empty[b], 8);
+    }
+    init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;");
+  const uint32_t tmem = *tmem_slot;
+  const int ct = (int)blockIdx.x % a.n_ct;
+  const int first = (int)blockIdx.x / a.n_ct, lists = (int)gridDim.x / a.n_ct, items = (int)a.items;
+  // Last rows first: what the backward's first half wrote last is in L2 still.
+  auto item_at = [&](int it) {
+    WorkItem w = work_item(a, it);
+    w.tile = a.tiles - 1 - w.tile;
+    return w;
+  };
+  auto passes_of = [&](const WorkItem& w) { return w.k0 == 0 ? a.ranks + 1 : w.nm; };
+  auto matrix_of = [&](const WorkItem& w, int p) { return w.k0 > 0 ? w.l : p == 0 ? 0 : a.ranks + p - 1; };
+
+  if (warp == 0) {
+    if (elect_one()) {
+      uint32_t s = 0, lap = 0;
+      int64_t g = 0;
+      bool ok = true, free = true;
+      for (int it = first; it < items && ok; it += lists) {
+        const WorkItem w = item_at(it);
+        const int passes = passes_of(w);
+        for (int p = 0; p < passes && ok; ++p) {
+          const bool gates = w.k0 == 0 && p > 0;
+          for (int i = 0; i < 2 * nk; ++i, ++g) {  // slab and part
+            if (!free && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
+              ok = false;
+              break;
+            }
+            const uint32_t s_next = (s + 1) % X_STAGES, lap_next = s_next ? lap : lap + 1;
+            free = lap_next == 0 || peek_parity(smem_u32(&empty[s_next]), (lap_next - 1) & 1u);
+            const uint32_t fb = smem_u32(&full[s]);
+            arrive_tx(fb, TILE_A);
+            tma_load_3d(smem_u32(ring + s * TILE_A), gates ? &mp.a2 : &mp.a, (i >> 1) * DIRECT_BK, w.tile * BM,
+                        2 * (gates ? p - 1 : w.k0 + p) + (i & 1), fb);
+            s = s_next;
+            lap = lap_next;
+          }
+        }
+      }
+      for (int t = 0; t < X_STAGES; ++t) {
+        const int64_t uses = g > t ? (g - 1 - t) / X_STAGES + 1 : 0;
+        if (uses > 0) drain_bar(smem_u32(&full[t]), (uint32_t)((uses - 1) & 1));
+      }
+    }
+  } else if (warp == 2) {
+    if (elect_one()) {
+      Slots slots;
+      int loads[2] = {0, 0};
+      bool ok = true;
+      for (int it = first; it < items && ok; it += lists) {
+        const WorkItem w = item_at(it);
+        const int passes = w.k0 == 0 ? a.ranks + 1 : 1;
+        for (int p = 0; p < passes && ok; ++p) {
+          bool fresh;
+          const int m = matrix_of(w, p), slot = slots.of(m, fresh);
+          if (fresh) {
+            const int before = slot ? loads[1] : loads[0];
+            if (before > 0 && !wait_phase(smem_u32(&w_free[slot]), (uint32_t)((before - 1) & 1), abort_flag)) {
+              ok = false;
+              break;
+            }
+            const uint32_t fb = smem_u32(&w_full[slot]);
+            arrive_tx(fb, (uint32_t)(nk * X_SLAB));
+            for (int kt = 0; kt < nk; ++kt)
+              tma_load_3d(smem_u32(wmem + (slot * nk + kt) * X_SLAB), &mp.b, kt * DIRECT_BK, ct * X_BN, m, fb);
+            if (slot) ++loads[1];
+            else ++loads[0];
+          }
+          if (w.k0 == 0 && a.ranks > 1) slots.drop(slot);
+        }
+      }
+      if (loads[0] > 0) drain_bar(smem_u32(&w_full[0]), (uint32_t)((loads[0] - 1) & 1));
+      if (loads[1] > 0) drain_bar(smem_u32(&w_full[1]), (uint32_t)((loads[1] - 1) & 1));
+    }
+  } else if (warp == 1) {
+    const uint64_t wdesc = make_desc(smem_u32(wmem)), adesc = make_desc(smem_u32(ring));
+    Slots slots;
+    uint32_t w_phase = 3u, unfreed = 0u;  // bit per slot: phase of its last load; not given back
+    uint32_t s = 0, lap = 0, n = 0;
+    bool ok = true, ready_a = false;
+    for (int it = first; it < items && ok; it += lists) {
+      const WorkItem w = item_at(it);
+      const int passes = passes_of(w);
+      for (int p = 0; p < passes && ok; ++p) {
+        bool fresh;
+        const int slot = slots.of(matrix_of(w, p), fresh);
+        const uint32_t bit = 1u << slot;
+        if (fresh) {
+          if ((unfreed & bit) && elect_one()) commit(smem_u32(&w_free[slot]));
+          __syncwarp();
+          unfreed |= bit;
+          w_phase ^= bit;
+        }
+        // all gate matrices' products add up in the accumulator behind the values'
+        const bool opens = w.k0 > 0 || p <= 1, closes = w.k0 > 0 || p == 0 || p == a.ranks;
+        if (opens) ok = wait_warp(smem_u32(&acc_empty[n % X_NACC]), (n / X_NACC & 1u) ^ 1u, abort_flag);
+        if (fresh) ok = ok && wait_warp(smem_u32(&w_full[slot]), (w_phase >> slot) & 1u, abort_flag);
+        const uint32_t d = tmem + n % X_NACC * X_BN;
+        for (int i = 0; i < 2 * nk; ++i) {
+          if (!ready_a) ok = ok && wait_warp(smem_u32(&full[s]), lap & 1u, abort_flag);
+          if (!ok) break;
+          asm volatile("tcgen05.fence::after_thread_sync;");
+          const uint32_t s_next = (s + 1) % X_STAGES, lap_next = s_next ? lap : lap + 1;
+          const bool peek = peek_parity(smem_u32(&full[s_next]), lap_next & 1u);
+          if (elect_one()) {
+            mma_slab<X_BN>(d, adesc + (uint64_t)(s * (TILE_A >> 4)),
+                           wdesc + (uint64_t)((slot * nk + (i >> 1)) * (X_SLAB >> 4)), !opens || i > 0);
+            commit(smem_u32(&empty[s]));
+          }
+          ready_a = __all_sync(0xffffffffu, peek);
+          s = s_next;
+          lap = lap_next;
+        }
+        if (ok && elect_one()) {
+          if (closes) commit(smem_u32(&acc_full[n % X_NACC]));
+          if (w.k0 == 0 && a.ranks > 1) commit(smem_u32(&w_free[slot]));
+        }
+        __syncwarp();
+        if (w.k0 == 0 && a.ranks > 1) {
+          slots.drop(slot);
+          unfreed &= ~bit;
+        }
+        if (closes) ++n;
+      }
+    }
+    if (elect_one()) {
+      commit(smem_u32(drain));
+      drain_bar(smem_u32(drain), 0);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int e = warp - 4, quarter = warp & 3, half = e >> 2;
+    uint8_t* boxes = epi + e * 2 * X_BOX;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 64);
+    const float sg = __ldg(a.scales + a.ranks);
+    const int col = ct * X_BN + half * 64;
+    uint32_t n = 0, box = 0;
+    bool ok = true;
+    for (int it = first; it < items && ok; it += lists) {
+      const WorkItem w = item_at(it);
+      const float sv = __ldg(a.scales + w.l);
+      const bool two = w.k0 == 0;
+      for (int m = 0; m < w.nm; ++m) {
+        ok = wait_warp(smem_u32(&acc_full[n % X_NACC]), n / X_NACC & 1u, abort_flag);
+        if (two) ok = ok && wait_warp(smem_u32(&acc_full[(n + 1) % X_NACC]), (n + 1) / X_NACC & 1u, abort_flag);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (col + h * 32 >= a.N) break;
+          float f[32];
+          tmem_ld<32>(lanes + n % X_NACC * X_BN + h * 32, f);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) f[c] *= sv;
+          if (two) {
+            float z[32];
+            tmem_ld<32>(lanes + (n + 1) % X_NACC * X_BN + h * 32, z);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) f[c] = fmaf(sg, z[c], f[c]);
+          }
+          // (the elected lane is the same every time; at most the other box's store still reads)
+          if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          __syncwarp();
+          put_row<bf16_t>(boxes + box * X_BOX, lane, f);
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (elect_one()) {
+            tma_store_3d(&mp.o, smem_u32(boxes + box * X_BOX), col + h * 32, w.tile * BM + quarter * 32, w.k0 + m);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          __syncwarp();
+          box ^= 1;
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;");
+        __syncwarp();
+        if (lane == 0) {
+          arrive(smem_u32(&acc_empty[n % X_NACC]));
+          if (two) arrive(smem_u32(&acc_empty[(n + 1) % X_NACC]));
+        }
+        n += two ? 2 : 1;
+      }
+    }
+    if (elect_one()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) fc_flag(a.status, FC_DEV_TIMEOUT);
+  if (warp == 0) {
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
 }  // namespace
+
+int run_direct_dx(const Maps& mp, const Args& a, int sms, cudaStream_t s) {
+  static Ready state;
+  if (int rc = ready(gated_bf16_dx_kernel, SMEM_MAX, state, 0)) return rc;
+  const int lists = (int)std::min<int64_t>(a.items, sms / a.n_ct);
+  gated_bf16_dx_kernel<<<lists * a.n_ct, X_THREADS, X_FIXED + 2 * a.nk * X_SLAB, s>>>(mp, a);
+  return fc_check_launch();
+}
 
 template <int MODE>
 int run_direct(const Maps& mp, Args a, int sms, cudaStream_t s) {

@@ -636,8 +636,9 @@ constexpr int MAX_LISTS = 160;  // work lists of a launch: one per 64 output cha
 struct PrepArgs {
   GatedArgs g;
   float* fwd;      // or null
-  bf16_t* direct;  // or null: in place of fwd, the weights as they are, in rows padded with zeros
   float* dx;       // or null
+  bf16_t* direct;  // or null: in place of fwd, the weights as they are, in rows padded with zeros
+  bf16_t* direct_dx;
   int* counters;
 };
 
@@ -648,15 +649,16 @@ __global__ void __launch_bounds__(256) prep_kernel(const PrepArgs p) {
   const int ranks = p.g.L + 1, q = blockIdx.y, l = q < ranks ? q : q - ranks, C = p.g.C, H = p.g.H;
   const T* w = q < ranks ? (const T*)p.g.wv[l] : (const T*)p.g.wg + (int64_t)l * H * C;
   const float sc = ((const float*)p.g.scales)[q < ranks ? l : ranks];
-  const int cp = (C + 3) & ~3, hp = (H + 3) & ~3;
-  const int c8 = (C + 7) & ~7;
-  const int64_t nf = p.direct ? (int64_t)H * c8 : p.fwd ? (int64_t)H * cp : 0, nd = p.dx ? (int64_t)C * hp : 0;
+  const int pad_f = p.direct ? 7 : 3, pad_d = p.direct_dx ? 7 : 3;
+  const int cp = (C + pad_f) & ~pad_f, hp = (H + pad_d) & ~pad_d;
+  const int64_t nf = p.direct || p.fwd ? (int64_t)H * cp : 0, nd = p.direct_dx || p.dx ? (int64_t)C * hp : 0;
   for (int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x; i < nf + nd; i += (int64_t)gridDim.x * 256) {
     const bool f = i < nf;
     const int64_t e = f ? i : i - nf, size = f ? nf : nd;
-    const int kp = f ? (p.direct ? c8 : cp) : hp, r = (int)(e / kp), k = (int)(e - (int64_t)r * kp);
-    if (f && p.direct) {
-      p.direct[q * size + e] = k < C ? Io<bf16_t>::put(Io<T>::get(w[(int64_t)r * C + k])) : Io<bf16_t>::put(0.f);
+    const int kp = f ? cp : hp, r = (int)(e / kp), k = (int)(e - (int64_t)r * kp);
+    if (bf16_t* plain = f ? p.direct : p.direct_dx) {
+      plain[q * size + e] = Io<bf16_t>::put(
+          k >= (f ? C : H) ? 0.f : (float)Io<T>::get(f ? w[(int64_t)r * C + k] : w[(int64_t)k * C + r]));
       continue;
     }
     float x = 0.f;
@@ -750,20 +752,33 @@ static bool one_list_each(int N, int sms) { return (N + BN - 1) / BN <= std::min
 // Whether the products of a reduction over K into N columns keep their weights in shared memory.
 static bool resident(int K, int N, int sms) { return K <= MAX_NK * BK && one_list_each(N, sms); }
 
-// Whether the forward (and the backward's first half) multiplies bfloat16 as it is.
+// Whether the products of a reduction over K into N columns multiply bfloat16 as it is.
 template <typename T>
 static bool direct(int K, int N, int sms) {
   return sizeof(T) == 2 && K <= DIRECT_K && one_list_each(N, sms);
 }
+// The backward does in all its products, or in none: its halves hand each other dv and dz.
+template <typename T>
+static bool direct_backward(int C, int H, int sms) {
+  return direct<T>(C, H, sms) && direct<T>(H, C, sms);
+}
 
 template <int MODE, typename T>
-static int run_products(const Maps& mp, const Args& a, int K, int sms, cudaStream_t s) {
-  if constexpr (sizeof(T) == 2 && MODE != DX) {
-    return direct<T>(K, a.N, sms) ? run_direct<MODE>(mp, a, sms, s) : run_stream<MODE, T>(mp, a, sms, s);
-  } else {
-    return resident(K, a.N, sms) ? run_resident<MODE, T>(mp, a, sms, s) : run_stream<MODE, T>(mp, a, sms, s);
+static int run_products(const Maps& mp, const Args& a, int K, bool dir, int sms, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (dir) {
+      if constexpr (MODE == DX) return run_direct_dx(mp, a, sms, s);
+      else return run_direct<MODE>(mp, a, sms, s);
+    }
   }
+  if constexpr (sizeof(T) == 4 || MODE == DX)
+    if (resident(K, a.N, sms)) return run_resident<MODE, T>(mp, a, sms, s);
+  return run_stream<MODE, T>(mp, a, sms, s);
 }
+
+// Rows of dv and dz parts are whole 128-byte lines: with 200 channels in rows of 200 (208, 256) the
+// backward's first half took 78 (72, 67) us for 100,003 rows.
+constexpr int PARTS_PAD = 64;
 
 // Layout of the workspace (bytes), the same for the size query and the call.
 struct Ws {
@@ -772,7 +787,7 @@ struct Ws {
 
 static Ws layout(int L, int C, int H, int64_t n, int esize, bool backward, int sms) {
   const int64_t ranks = L + 1, comps = ranks * ranks, per = 16 / esize;
-  const int64_t cp = (C + 3) / 4 * 4, hp = (H + 3) / 4 * 4;
+  const int64_t cp = (C + 3) / 4 * 4, hp = (H + PARTS_PAD - 1) / PARTS_PAD * PARTS_PAD;
   const int64_t ce = (C + per - 1) / per * per, he = (H + per - 1) / per * per;
   Ws w{};
   int64_t at = 0;
@@ -822,17 +837,17 @@ static int repitch(const T* src, int64_t src_ld, T* dst, int64_t dst_ld, int wid
 }
 
 template <typename T>
-static Args product_args(const GatedArgs& g, int N, int K, int mode, int sms) {
+static Args product_args(const GatedArgs& g, int N, int K, int mode, bool dir, int sms) {
   Args a{};
   a.L = g.L;
   a.ranks = g.L + 1;
   a.comps = a.ranks * a.ranks;
   a.N = N;
-  const bool dir = mode != DX && direct<T>(K, N, sms);
   a.nk = dir ? (K + DIRECT_BK - 1) / DIRECT_BK : (K + BK - 1) / BK;
   a.tiles = (int)((g.n + BM - 1) / BM);
   const bool res = dir || (resident(K, N, sms) && (sizeof(T) == 4 || mode == DX));
-  a.n_ct = res ? (N + BN - 1) / BN : (N + STREAM_BN - 1) / STREAM_BN;
+  const int width = !res ? STREAM_BN : dir && mode == DX ? DIRECT_DX_BN : BN;
+  a.n_ct = (N + width - 1) / width;
   // with fewer (tile, rank) groups than SMs the components are items of their own (the gate is
   // computed again for each); PRE needs a rank's components together
   a.per_comp = (mode == DX && !res) || (mode != PRE && (int64_t)a.tiles * a.ranks * a.n_ct < sms);
@@ -854,20 +869,19 @@ static Args product_args(const GatedArgs& g, int N, int K, int mode, int sms) {
 }
 
 template <typename T>
-static int run_prep(const GatedArgs& g, void* fwd, float* dx, int* counters, int sms, cudaStream_t s) {
-  const int64_t cp = (g.C + 3) & ~3, c8 = (g.C + 7) & ~7, hp = (g.H + 3) & ~3;
-  const bool dir = direct<T>(g.C, g.H, sms);
-  const int64_t each = g.H * (dir ? c8 : cp) + (dx ? g.C * hp : 0);
-  const PrepArgs p{g, dir ? nullptr : (float*)fwd, dir ? (bf16_t*)fwd : nullptr, dx, counters};
+static int run_prep(const GatedArgs& g, void* fwd, void* dx, bool dir, int* counters, cudaStream_t s) {
+  const int64_t each = (int64_t)g.H * (g.C + 7) + (dx ? (int64_t)g.C * (g.H + 7) : 0);
+  const PrepArgs p{g, dir ? nullptr : (float*)fwd, dir ? nullptr : (float*)dx, dir ? (bf16_t*)fwd : nullptr,
+                   dir ? (bf16_t*)dx : nullptr, counters};
   prep_kernel<T><<<dim3((unsigned)std::min<int64_t>((each + 255) / 256, 256), 2 * (g.L + 1)), 256, 0, s>>>(p);
   return fc_check_launch();
 }
 
 // The maps of x and of the weights that the forward products read.
 template <typename T>
-static bool encode_forward(Maps& mp, const GatedArgs& g, const Rows<T>& x, const void* weights, int sms) {
+static bool encode_forward(Maps& mp, const GatedArgs& g, const Rows<T>& x, const void* weights, bool dir, int sms) {
   const int ranks = g.L + 1, comps = ranks * ranks;
-  if (direct<T>(g.C, g.H, sms))
+  if (dir)
     return encode_rows<T>(&mp.a, x.p, g.C, g.n, comps, x.ld, DIRECT_BK, BM) &&
            encode_rows<T>(&mp.ap, x.p, g.C, g.n, comps, x.ld, DIRECT_K, BM) &&
            encode_weights<bf16_t>(&mp.b, (const bf16_t*)weights, (g.C + 7) & ~7, g.H, 2 * ranks, BN);
@@ -895,14 +909,15 @@ int gated_tc_fwd(const GatedArgs& a, cudaStream_t s) {
   if (x.copied)
     if (int rc = repitch<T>((const T*)a.x, a.C, const_cast<T*>(x.p), x.ld, a.C, a.n * comps, s)) return rc;
   int* counters = (int*)(ws + w.counters);
-  if (int rc = run_prep<T>(a, ws + w.fwd, nullptr, counters, sms, s)) return rc;
-  Args args = product_args<T>(a, a.H, a.C, FWD, sms);
+  const bool dir = direct<T>(a.C, a.H, sms);
+  if (int rc = run_prep<T>(a, ws + w.fwd, nullptr, dir, counters, s)) return rc;
+  Args args = product_args<T>(a, a.H, a.C, FWD, dir, sms);
   args.counter = counters;
   Maps mp;
-  if (!encode_forward<T>(mp, a, x, ws + w.fwd, sms) || !encode_rows<T>(&mp.o, y.p, a.H, a.n, comps, y.ld, 32, 32))
+  if (!encode_forward<T>(mp, a, x, ws + w.fwd, dir, sms) || !encode_rows<T>(&mp.o, y.p, a.H, a.n, comps, y.ld, 32, 32))
     return FC_ERR_UNSUPPORTED;
   mp.a2 = mp.g = mp.gp = mp.o2 = mp.o;  // not used
-  if (int rc = run_products<FWD, T>(mp, args, a.C, sms, s)) return rc;
+  if (int rc = run_products<FWD, T>(mp, args, a.C, dir, sms, s)) return rc;
   if (y.copied) return repitch<T>(y.p, y.ld, (T*)a.y, a.H, a.H, a.n * comps, s);
   return 0;
 }
@@ -913,12 +928,18 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
   const int sms = sm_count();
   if (!sms || !encode_fn()) return FC_ERR_LAUNCH;
   const int ranks = a.L + 1, comps = ranks * ranks;
-  const int64_t hp = (a.H + 3) / 4 * 4;
+  const bool dir = direct_backward<T>(a.C, a.H, sms);
+  const int64_t hp = dir ? (a.H + PARTS_PAD - 1) / PARTS_PAD * PARTS_PAD : (a.H + 3) / 4 * 4;  // row length of dv and dz
   const Ws w = layout(a.L, a.C, a.H, a.n, sizeof(T), true, sms);
   uint8_t* ws = (uint8_t*)a.ws;
   const Rows<T> x = rows_of<T>(a.x, a.C, ws + w.x), gy = rows_of<T>(a.gy, a.H, ws + w.y);
   int* counters = (int*)(ws + w.counters);
-  float *dx = (float*)(ws + w.dx), *dv = (float*)(ws + w.dv), *dz = (float*)(ws + w.dz);
+  void *dx = ws + w.dx, *dv = ws + w.dv, *dz = ws + w.dz;
+  // dv and dz in boxes: floats, or two bfloat16 parts a component
+  auto encode_between = [&](CUtensorMap* map, const void* p, int64_t planes, int box_c, int box_r) {
+    return dir ? encode_rows<bf16_t>(map, p, a.H, a.n, 2 * planes, hp, box_c, box_r)
+               : encode_rows<float>(map, p, a.H, a.n, planes, hp, box_c, box_r);
+  };
   bool any = a.gwg || a.gbias;
   for (int l = 0; l < ranks; ++l) any = any || a.gwv[l];
   if (a.n > 0) {
@@ -926,31 +947,32 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
       if (int rc = repitch<T>((const T*)a.x, a.C, const_cast<T*>(x.p), x.ld, a.C, a.n * comps, s)) return rc;
     if (gy.copied)
       if (int rc = repitch<T>((const T*)a.gy, a.H, const_cast<T*>(gy.p), gy.ld, a.H, a.n * comps, s)) return rc;
-    if (int rc = run_prep<T>(a, ws + w.fwd, a.gx ? dx : nullptr, counters, sms, s)) return rc;
+    if (int rc = run_prep<T>(a, ws + w.fwd, a.gx ? dx : nullptr, dir, counters, s)) return rc;
     Maps mp;
-    if (!encode_forward<T>(mp, a, x, ws + w.fwd, sms) ||
-        !encode_rows<float>(&mp.o, dv, a.H, a.n, comps, hp, 32, 32) ||
+    if (!encode_forward<T>(mp, a, x, ws + w.fwd, dir, sms) || !encode_between(&mp.o, dv, comps, 32, 32) ||
         !encode_rows<T>(&mp.g, gy.p, a.H, a.n, comps, gy.ld, 32, 32) ||
         !encode_rows<T>(&mp.gp, gy.p, a.H, a.n, comps, gy.ld, BN, BM) ||
-        !encode_rows<float>(&mp.o2, dz, a.H, a.n, ranks, hp, 32, 32))
+        !encode_between(&mp.o2, dz, ranks, 32, 32))
       return FC_ERR_UNSUPPORTED;
     mp.a2 = mp.o2;  // not used
-    Args args = product_args<T>(a, a.H, a.C, PRE, sms);
+    Args args = product_args<T>(a, a.H, a.C, PRE, dir, sms);
     args.counter = counters;
-    if (int rc = run_products<PRE, T>(mp, args, a.C, sms, s)) return rc;
+    if (int rc = run_products<PRE, T>(mp, args, a.C, dir, sms, s)) return rc;
     if (a.gx) {
       const Rows<T> gx = rows_of<T>(a.gx, a.C, ws + w.gx);
       Maps md;
-      if (!encode_rows<float>(&md.a, dv, a.H, a.n, comps, hp, BK, BM) ||
-          !encode_rows<float>(&md.ap, dv, a.H, a.n, comps, hp, MAX_NK * BK, BM) ||
-          !encode_rows<float>(&md.a2, dz, a.H, a.n, ranks, hp, BK, BM) ||
-          !encode_weights<float>(&md.b, dx, (int)hp, a.C, 4 * ranks, resident(a.H, a.C, sms) ? BN : STREAM_BN) ||
+      const int box = dir ? DIRECT_BK : BK;
+      if (!encode_between(&md.a, dv, comps, box, BM) || !encode_between(&md.a2, dz, ranks, box, BM) ||
+          !(dir ? encode_weights<bf16_t>(&md.b, (const bf16_t*)dx, (a.H + 7) & ~7, a.C, 2 * ranks, DIRECT_DX_BN)
+                : encode_weights<float>(&md.b, (const float*)dx, (int)hp, a.C, 4 * ranks,
+                                        resident(a.H, a.C, sms) ? BN : STREAM_BN)) ||
+          !encode_between(&md.ap, dv, comps, MAX_NK * BK, BM) ||
           !encode_rows<T>(&md.o, gx.p, a.C, a.n, comps, gx.ld, 32, 32))
         return FC_ERR_UNSUPPORTED;
       md.g = md.gp = md.o2 = md.o;  // not used
-      Args dargs = product_args<T>(a, a.C, a.H, DX, sms);
+      Args dargs = product_args<T>(a, a.C, a.H, DX, dir, sms);
       dargs.counter = counters + MAX_LISTS;
-      if (int rc = run_products<DX, T>(md, dargs, a.H, sms, s)) return rc;
+      if (int rc = run_products<DX, T>(md, dargs, a.H, dir, sms, s)) return rc;
       if (gx.copied)
         if (int rc = repitch<T>(gx.p, gx.ld, (T*)a.gx, a.C, a.C, a.n * comps, s)) return rc;
     }
@@ -963,7 +985,7 @@ int gated_tc_bwd(const GatedArgs& a, cudaStream_t s) {
   }
   o.bias = a.gbias;
   o.scales = (const float*)a.scales;
-  return run_wgrad<T>(ranks, a.C, a.H, a.n, dv, dz, hp, x.p, x.ld, (float*)(ws + w.part), (float*)(ws + w.bias), o,
+  return run_wgrad<T>(ranks, a.C, a.H, a.n, dv, dz, hp, dir, x.p, x.ld, (float*)(ws + w.part), (float*)(ws + w.bias), o,
                       a.status, sms, s);
 }
 

@@ -12,7 +12,7 @@ using namespace tma;
 
 constexpr int BK = 32, THREADS = 512;
 // Reductions of bfloat16 rows and weights up to this length take the kernel without splitting.
-constexpr int DIRECT_K = 256, DIRECT_BK = 64;
+constexpr int DIRECT_K = 256, DIRECT_BK = 64, DIRECT_DX_BN = 128;
 constexpr int EPI_BUF = 4096;  // a warp's 32 x 32 float staging box
 constexpr int BAR_BYTES = 640;
 constexpr int SCHED = 4;  // work items handed out ahead
@@ -259,7 +259,8 @@ __device__ __forceinline__ float fast_dact(int act, float z) {
 #define FC_SETMAXNREG_INC(n) asm volatile("setmaxnreg.inc.sync.aligned.u32 " #n ";")
 
 // Per device: shared-memory size set, and the registers that setmaxnreg shares out checked
-// (the block must be launched with `regs` per thread: its roles' shares are counted on that).
+// (the block must be launched with `regs` per thread: its roles' shares are counted on that; 0
+// where nothing is shared out).
 struct Ready {
   bool done[64] = {};
 };
@@ -272,7 +273,7 @@ static int ready(K kernel, int smem, Ready& r, int regs = 128) {
     return FC_ERR_LAUNCH;
   cudaFuncAttributes at;
   if (cudaFuncGetAttributes(&at, kernel) != cudaSuccess) return FC_ERR_LAUNCH;
-  if (at.numRegs != regs) return FC_ERR_UNSUPPORTED;
+  if (regs && at.numRegs != regs) return FC_ERR_UNSUPPORTED;
   r.done[dev] = true;
   return 0;
 }
@@ -282,6 +283,7 @@ constexpr int STREAM_BN = 128;  // output columns of a tile: streaming kernel
 constexpr int STREAM_KG = 2, STREAM_NACC = 3;
 template <int MODE>
 int run_direct(const Maps& mp, Args a, int sms, cudaStream_t s);
+int run_direct_dx(const Maps& mp, const Args& a, int sms, cudaStream_t s);
 template <int MODE, typename T>
 int run_stream(const Maps& mp, const Args& a, int sms, cudaStream_t s);
 
@@ -291,9 +293,11 @@ struct WOut {
   const float* scales;
 };
 int64_t wgrad_part_count(int ranks, int C, int H, int sms);  // 128 x 128 partial matrices of the workspace
+// dv, dz: float rows, or (parts) two bfloat16 parts per component, rows of dv_ld elements.
 template <typename T>
-int run_wgrad(int ranks, int C, int H, int64_t n, const float* dv, const float* dz, int64_t dv_ld, const T* x,
-              int64_t x_ld, float* part, float* bias_part, const WOut& o, int* status, int sms, cudaStream_t s);
+int run_wgrad(int ranks, int C, int H, int64_t n, const void* dv, const void* dz, int64_t dv_ld, bool parts,
+              const T* x, int64_t x_ld, float* part, float* bias_part, const WOut& o, int* status, int sms,
+              cudaStream_t s);
 
 // (channel, row, component) map of a tensor of rows [comps][ld]; box_c channels x box_r rows,
 // boxes of 128- or 64-byte rows with that swizzle.

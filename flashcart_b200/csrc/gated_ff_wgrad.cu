@@ -24,7 +24,7 @@ constexpr int KG = 2;  // slabs per accumulation unit (see gated_ff_tc.cu)
 struct WArgs {
   int ranks, H, Cn;
   int n_ht, n_ct;
-  int64_t blocks;      // 32-row blocks
+  int64_t blocks;      // row blocks: 32 rows (64: bfloat16 parts)
   int64_t width[8];    // slabs per job of a matrix
   int skip;            // bit per matrix that is not wanted: its slabs keep their place on the
                        // line, so what is wanted does not depend on what else is
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(W_THREADS, 1) wgrad_kernel(const __grid_consta
       // ---------------------------------------------------------------- TMA producer
       int64_t g = 0;
       uint32_t s = 0, lap = 0;
-      bool ok = true;
+      bool ok = true, free = true;  // (peeked: the next stage is free)
       for (int64_t p = begin; p < end && ok;) {
         const Job j = job_at(a, p);
         const bool gates = j.mat >= a.ranks;
@@ -164,10 +164,12 @@ __global__ void __launch_bounds__(W_THREADS, 1) wgrad_kernel(const __grid_consta
           ++nbf;
         }
         for (; p < stop; ++p, ++g) {
-          if (lap > 0 && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
+          if (!free && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
             ok = false;
             break;
           }
+          const uint32_t s_next = (s + 1) % RAW, lap_next = s_next ? lap : lap + 1;
+          free = lap_next == 0 || peek_parity(smem_u32(&empty[s_next]), (lap_next - 1) & 1u);
           if (p + PF < stop) {  // the ring's stages alone do not cover DRAM
             tma_prefetch_3d(md, j.ht * BM, nbf * 32, zd + mf);
             tma_prefetch_3d(&mp.x, j.ct * BN, nbf * 32, zx + mf);
@@ -185,10 +187,8 @@ __global__ void __launch_bounds__(W_THREADS, 1) wgrad_kernel(const __grid_consta
             m = 0;
             ++nb;
           }
-          if (++s == RAW) {
-            s = 0;
-            ++lap;
-          }
+          s = s_next;
+          lap = lap_next;
         }
       }
       for (int t = 0; t < RAW; ++t) {
@@ -388,6 +388,240 @@ __global__ void __launch_bounds__(W_THREADS, 1) wgrad_kernel(const __grid_consta
   }
 }
 
+// The same from two bfloat16 parts of dv and dz and bfloat16 rows x: the tensor cores take both
+// operands M- and N-major, as they lie in memory, so slabs of 64 rows go from DRAM to shared
+// memory and nothing is transposed. dz's column sums (the bias) are a product with a tile of ones.
+// Bound by DRAM (200 MB for 100,003 rows of 96 x 200 channels, 31 us at the copy rate).
+// The 12 warps: 0 TMA producer, 1 MMA issue, 4-11 epilogue (unit sums).
+constexpr int P_ROWS = 64, P_BOX = P_ROWS * 128;  // 64 channels of 64 rows
+constexpr int P_STAGE = 6 * P_BOX, P_STAGES = 4;  // hi, lo and x, two boxes each
+constexpr int P_KG = 4;                           // slabs per accumulation unit: 32 accumulations
+constexpr int P_ONES = 2048, P_THREADS = 12 * 32;
+constexpr int P_SMEM = P_STAGES * P_STAGE + P_ONES + BAR_BYTES + 1024;
+static_assert(P_SMEM <= 227 * 1024, "shared memory per CTA");
+
+// M- or N-major operand of 128-byte rows (64 channels): 8 KB to the next 64 channels, 1 KB to the
+// next 8 rows of the reduction.
+__device__ __forceinline__ uint64_t make_desc_mn(uint32_t saddr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr >> 4) & 0x3FFF);
+  d |= (uint64_t)(P_BOX >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+template <int N, bool B_MN>
+__device__ __forceinline__ void mma_parts(uint32_t d, uint64_t da, uint64_t db, uint32_t acc) {
+  constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (B_MN ? 1u << 16 : 0u) |
+                             ((uint32_t)(N >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(acc));
+}
+
+__global__ void __launch_bounds__(P_THREADS, 1)
+    wgrad_parts_kernel(const __grid_constant__ WMaps mp, const WArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ones = smem + P_STAGES * P_STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ones + P_ONES);
+  uint64_t* empty = full + P_STAGES;
+  uint64_t* acc_full = empty + P_STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  constexpr int B_COLS = 2 * BN;  // behind the accumulators: the bias's
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (threadIdx.x == 32) {
+    auto init = [](uint64_t* b, int n) {
+      asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(n));
+    };
+    for (int s = 0; s < P_STAGES; ++s) {
+      init(&full[s], 1);
+      init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      init(&acc_full[b], 1);
+      init(&acc_empty[b], 8);
+    }
+    init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  for (int i = threadIdx.x; i < P_ONES / 4; i += P_THREADS) reinterpret_cast<uint32_t*>(ones)[i] = 0x3F803F80u;
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;");
+  const uint32_t tmem = *tmem_slot;
+  const int64_t begin = cta_begin(a, blockIdx.x), end = cta_begin(a, blockIdx.x + 1);
+
+  if (warp == 0) {
+    if (elect_one()) {
+      int64_t g = 0;
+      uint32_t s = 0, lap = 0;
+      bool ok = true, free = true;  // (peeked: the next stage is free)
+      for (int64_t p = begin; p < end && ok;) {
+        const Job j = job_at(a, p);
+        const bool gates = j.mat >= a.ranks;
+        const int l = gates ? j.mat - a.ranks : j.mat, w = gates ? 1 : 2 * l + 1;
+        const int64_t stop = min(end, j.last);
+        if (a.skip >> j.mat & 1) {
+          p = stop;
+          continue;
+        }
+        const CUtensorMap* md = gates ? &mp.dz : &mp.dv;
+        const int zd = gates ? l : l * l, zx = gates ? 0 : l * l;
+        int nb = (int)((p - j.first) / w), m = (int)((p - j.first) - (int64_t)nb * w);
+        for (; p < stop; ++p, ++g) {
+          if (!free && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
+            ok = false;
+            break;
+          }
+          const uint32_t s_next = (s + 1) % P_STAGES, lap_next = s_next ? lap : lap + 1;
+          free = lap_next == 0 || peek_parity(smem_u32(&empty[s_next]), (lap_next - 1) & 1u);
+          const uint32_t st = smem_u32(smem + s * P_STAGE), fb = smem_u32(&full[s]);
+          arrive_tx(fb, P_STAGE);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int h0 = j.ht * BM + half * 64, c0 = j.ct * BN + half * 64;
+            tma_load_3d(st + half * P_BOX, md, h0, nb * P_ROWS, 2 * (zd + m), fb);
+            tma_load_3d(st + (2 + half) * P_BOX, md, h0, nb * P_ROWS, 2 * (zd + m) + 1, fb);
+            tma_load_3d(st + (4 + half) * P_BOX, &mp.x, c0, nb * P_ROWS, zx + m, fb);
+          }
+          if (++m == w) {
+            m = 0;
+            ++nb;
+          }
+          s = s_next;
+          lap = lap_next;
+        }
+      }
+      for (int t = 0; t < P_STAGES; ++t) {
+        const int64_t uses = g > t ? (g - 1 - t) / P_STAGES + 1 : 0;
+        if (uses > 0) drain_bar(smem_u32(&full[t]), (uint32_t)((uses - 1) & 1));
+      }
+    }
+  } else if (warp == 1) {
+    const uint64_t desc = make_desc_mn(smem_u32(smem)), desc_ones = make_desc(smem_u32(ones));
+    uint32_t s = 0, lap = 0, ab = 0, acc_phase = 0;
+    bool ok = true, ready_a = false;
+    for (int64_t p = begin; p < end && ok;) {
+      const Job j = job_at(a, p);
+      const int slabs = (int)(min(end, j.last) - p);
+      p += slabs;
+      if (a.skip >> j.mat & 1) continue;
+      const bool bias = a.bias_part && j.mat >= a.ranks && j.ct == 0;
+#pragma unroll 1
+      for (int t = 0; t < slabs; ++t) {
+        const bool opens = t % P_KG == 0, closes = t % P_KG == P_KG - 1 || t + 1 == slabs;
+        if (opens) ok = wait_warp(smem_u32(&acc_empty[ab]), acc_phase ^ 1u, abort_flag);
+        if (!ready_a) ok = ok && wait_warp(smem_u32(&full[s]), lap & 1u, abort_flag);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;");
+        const uint32_t s_next = (s + 1) % P_STAGES, lap_next = s_next ? lap : lap + 1;
+        const bool peek = peek_parity(smem_u32(&full[s_next]), lap_next & 1u);
+        if (elect_one()) {
+          const uint32_t d = tmem + ab * (uint32_t)BN, db = tmem + (uint32_t)B_COLS + ab * 16u;
+          const uint64_t st = desc + (uint64_t)(s * (P_STAGE >> 4)), x = st + (uint64_t)(4 * P_BOX >> 4);
+#pragma unroll
+          for (int part = 1; part >= 0; --part)  // the low parts first: a sum is truncated less while it is small
+#pragma unroll
+            for (int kk = 0; kk < P_ROWS / 16; ++kk) {
+              const uint64_t da = st + (uint64_t)((part * 2 * P_BOX + kk * 2048) >> 4);
+              const uint32_t more = opens && part == 1 && kk == 0 ? 0u : 1u;
+              mma_parts<BN, true>(d, da, x + (uint64_t)(kk * 2048 >> 4), more);
+              if (bias) mma_parts<16, false>(db, da, desc_ones, more);
+            }
+          commit(smem_u32(&empty[s]));
+          if (closes) commit(smem_u32(&acc_full[ab]));
+        }
+        ready_a = __all_sync(0xffffffffu, peek);
+        s = s_next;
+        lap = lap_next;
+        if (closes) {
+          acc_phase ^= ab;
+          ab ^= 1u;
+        }
+      }
+    }
+    if (elect_one()) {
+      commit(smem_u32(drain));
+      drain_bar(smem_u32(drain), 0);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ epilogue: unit sums
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    uint32_t ab = 0, acc_phase = 0;
+    bool ok = true;
+    for (int64_t p = begin; p < end && ok;) {
+      const Job j = job_at(a, p);
+      const int slabs = (int)(min(end, j.last) - p);
+      p += slabs;
+      if (a.skip >> j.mat & 1) continue;
+      const bool bias = a.bias_part && j.mat >= a.ranks && j.ct == 0 && half == 0;
+      float acc[64], bsum = 0.f;
+#pragma unroll
+      for (int c = 0; c < 64; ++c) acc[c] = 0.f;
+#pragma unroll 1
+      for (int t = 0; t < slabs; t += P_KG) {
+        if (!wait_warp(smem_u32(&acc_full[ab]), acc_phase, abort_flag)) {
+          ok = false;
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;");
+#pragma unroll
+        for (int cb = 0; cb < 4; ++cb) {
+          float f[16];
+          tmem_ld<16>(lanes + ab * (uint32_t)BN + (uint32_t)(half * 64 + cb * 16), f);
+#pragma unroll
+          for (int c = 0; c < 16; ++c) acc[cb * 16 + c] += f[c];
+        }
+        if (bias) {
+          float f[16];
+          tmem_ld<16>(lanes + (uint32_t)B_COLS + ab * 16u, f);
+          bsum += f[0];
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;");
+        __syncwarp();
+        if (lane == 0) arrive(smem_u32(&acc_empty[ab]));
+        acc_phase ^= ab;
+        ab ^= 1u;
+      }
+      if (!ok) break;
+      const int64_t at = blockIdx.x + j.index;
+      float4* out = reinterpret_cast<float4*>(a.part + (at * BM + quarter * 32 + lane) * BN + half * 64);
+#pragma unroll
+      for (int c = 0; c < 16; ++c)
+        out[c] = make_float4(acc[4 * c], acc[4 * c + 1], acc[4 * c + 2], acc[4 * c + 3]);
+      if (bias) {  // (a part's slot holds two sums)
+        a.bias_part[at * 2 * BM + quarter * 32 + lane] = bsum;
+        a.bias_part[(at * 2 + 1) * BM + quarter * 32 + lane] = 0.f;
+      }
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;");
+  __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) fc_flag(a.status, FC_DEV_TIMEOUT);
+  if (warp == 0) {
+    asm volatile("tcgen05.fence::after_thread_sync;");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+  }
+}
+
 // Partial matrices added in the order of the CTAs. A block takes four rows of a job's tile: its
 // warps 4 r + p add every fourth partial of row r from the p-th on, and the four sums are added
 // in order. The bias goes with the ct = 0 gate jobs.
@@ -455,15 +689,17 @@ int64_t wgrad_part_count(int ranks, int C, int H, int sms) {
 }
 
 template <typename T>
-int run_wgrad(int ranks, int C, int H, int64_t n, const float* dv, const float* dz, int64_t dv_ld, const T* x,
-              int64_t x_ld, float* part, float* bias_part, const WOut& o, int* status, int sms, cudaStream_t s) {
+int run_wgrad(int ranks, int C, int H, int64_t n, const void* dv, const void* dz, int64_t dv_ld, bool parts,
+              const T* x, int64_t x_ld, float* part, float* bias_part, const WOut& o, int* status, int sms,
+              cudaStream_t s) {
   WArgs wa{};
   wa.ranks = ranks;
   wa.H = H;
   wa.Cn = C;
   wa.n_ht = (H + BM - 1) / BM;
   wa.n_ct = (C + BN - 1) / BN;
-  wa.blocks = (n + 31) / 32;
+  const int rows = parts ? P_ROWS : 32;
+  wa.blocks = (n + rows - 1) / rows;
   for (int l = 0; l < ranks; ++l) {
     wa.width[l] = wa.blocks * (2 * l + 1);
     wa.width[ranks + l] = wa.blocks;
@@ -480,23 +716,33 @@ int run_wgrad(int ranks, int C, int H, int64_t n, const float* dv, const float* 
     wa.ctas = (int)std::min<int64_t>(sms, (wa.total + 3) / 4);
     const int comps = ranks * ranks;
     WMaps wm;
-    if (!encode_rows<float>(&wm.dv, dv, H, n, comps, dv_ld, BM, 32) ||
-        !encode_rows<float>(&wm.dz, dz, H, n, ranks, dv_ld, BM, 32) ||
-        !encode_rows<T>(&wm.x, x, C, n, comps, x_ld, BN, 32))
-      return FC_ERR_UNSUPPORTED;
-    constexpr int smem = WCfg<T>::SMEM;
-    static Ready state;
-    if (int rc = ready(wgrad_kernel<T>, smem, state, W_REGS)) return rc;
-    wgrad_kernel<T><<<wa.ctas, W_THREADS, smem, s>>>(wm, wa);
+    if (parts) {
+      if (!encode_rows<bf16_t>(&wm.dv, dv, H, n, 2 * comps, dv_ld, 64, P_ROWS) ||
+          !encode_rows<bf16_t>(&wm.dz, dz, H, n, 2 * ranks, dv_ld, 64, P_ROWS) ||
+          !encode_rows<T>(&wm.x, x, C, n, comps, x_ld, 64, P_ROWS))
+        return FC_ERR_UNSUPPORTED;
+      static Ready state;
+      if (int rc = ready(wgrad_parts_kernel, P_SMEM, state, 0)) return rc;
+      wgrad_parts_kernel<<<wa.ctas, P_THREADS, P_SMEM, s>>>(wm, wa);
+    } else {
+      if (!encode_rows<float>(&wm.dv, dv, H, n, comps, dv_ld, BM, 32) ||
+          !encode_rows<float>(&wm.dz, dz, H, n, ranks, dv_ld, BM, 32) ||
+          !encode_rows<T>(&wm.x, x, C, n, comps, x_ld, BN, 32))
+        return FC_ERR_UNSUPPORTED;
+      constexpr int smem = WCfg<T>::SMEM;
+      static Ready state;
+      if (int rc = ready(wgrad_kernel<T>, smem, state, W_REGS)) return rc;
+      wgrad_kernel<T><<<wa.ctas, W_THREADS, smem, s>>>(wm, wa);
+    }
     if (int rc = fc_check_launch()) return rc;
   }
   wgrad_sum_kernel<T><<<(unsigned)(2 * ranks * wa.n_ht * wa.n_ct * (BM / SUM_ROWS)), SUM_ROWS * SUM_PARTS * 32, 0,
                         s>>>(wa, o);
   return fc_check_launch();
 }
-template int run_wgrad<float>(int, int, int, int64_t, const float*, const float*, int64_t, const float*, int64_t, float*,
-                              float*, const WOut&, int*, int, cudaStream_t);
-template int run_wgrad<bf16_t>(int, int, int, int64_t, const float*, const float*, int64_t, const bf16_t*, int64_t,
+template int run_wgrad<float>(int, int, int, int64_t, const void*, const void*, int64_t, bool, const float*, int64_t,
+                              float*, float*, const WOut&, int*, int, cudaStream_t);
+template int run_wgrad<bf16_t>(int, int, int, int64_t, const void*, const void*, int64_t, bool, const bf16_t*, int64_t,
                                float*, float*, const WOut&, int*, int, cudaStream_t);
 
 }  // namespace gtc
