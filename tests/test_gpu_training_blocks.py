@@ -87,6 +87,24 @@ def test_embedding_bad_index(cuda_device):
         ops.check_device_status()
 
 
+@pytest.mark.parametrize("dtype", [F32, F64, BF16])
+@pytest.mark.parametrize("dim", [1, 2, 3, 4, 5, 7, 8, 9, 15, 31, 33, 63])
+def test_embedding_vectors_across_rows(cuda_device, dtype, dim):
+    # rows that are no whole vectors, a wrong index on either side of a row's end
+    ops.check_device_status()
+    t = _randn(torch.Generator().manual_seed(dim), 6, dim, dtype=dtype)
+    for rows in (1, 2, 259):
+        idx = torch.randint(0, 6, (rows,), device="cuda")
+        want = t[idx]
+        assert torch.equal(ops.embedding(t, idx), want)
+        idx[::5] = 6
+        idx[-1:] = -2
+        want = torch.where(((idx >= 0) & (idx < 6))[:, None], want, torch.zeros_like(want))
+        assert torch.equal(ops.embedding(t, idx), want)
+        with pytest.raises(RuntimeError, match="outside"):
+            ops.check_device_status()
+
+
 def test_embedding_differences_and_second_derivative(cuda_device):
     t = torch.randn(5, 3, dtype=F64, device="cuda", requires_grad=True)
     idx = torch.tensor([0, 4, 4, 1, 4, 0], device="cuda")
