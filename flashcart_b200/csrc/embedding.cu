@@ -2,7 +2,8 @@
 //
 // Forward: out[i, :] = offset + scale * table[idx[i], :]. Bound by DRAM: the output write
 // (element tables stay in L1 / L2). One 16-byte vector of the output per thread and step,
-// four steps' loads in flight.
+// four steps' loads in flight. Measured: 27,648 rows of 2,944 float32 channels 61 us (5.3 TB/s),
+// 2^26 elements in rows of 64 62 us (4.4 TB/s).
 //
 // Backward: d_table[v, :] = scale * sum over {i : idx[i] = v} of grad[i, :], in an order
 // fixed by the sizes alone (no atomics), so equal inputs give equal bits. The tokens are
@@ -12,7 +13,10 @@
 // registers; a token whose rows lie inside one chunk is written at once, a token that spans
 // chunks leaves one partial sum per chunk in the workspace, and a second kernel adds the
 // partial sums. Bound by the one read of grad; the sort moves 8 to 16 bytes per row and
-// pass. Sums are float (double for 64-bit tables), rounded once.
+// pass. Sums are float (double for 64-bit tables), rounded once. Measured: 1,492,998 rows of 16
+// float32 channels into 4 types 55 us (sort 18, sums 29, joining 9; 16 us for one read of grad at
+// the copy rate); 65,537 rows of 512 bfloat16 channels into 50,000 types 76 us (sort 28, bounds and
+// zero rows 14, sums 22, joining 12).
 //
 // An index outside [0, n_types) raises FC_DEV_BAD_INDEX; its output row is written as zeros
 // and its gradient row is ignored (it sorts behind every token as key n_types).

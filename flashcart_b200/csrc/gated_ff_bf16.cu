@@ -1,5 +1,5 @@
-// Gated feed-forward block for bfloat16 rows on tcgen05 tensor cores (sm_100a): the forward and
-// the backward's first half, both operands bfloat16.
+// Gated feed-forward block for bfloat16 rows on tcgen05 tensor cores (sm_100a): the forward, the
+// backward's first half and the input gradient, both operands bfloat16.
 //
 // Mathematics and row layout: gated_ff.cu; modes, work items and lists: gated_ff_tc.cu. Rows and
 // weights are bfloat16, so their products are exact in the float accumulator and one product a
@@ -11,9 +11,10 @@
 //
 // What bounds it: the epilogue. 100,003 rows of 96 -> 200 channels are 59 MB (9 us), but a
 // gate costs about 25 instructions, two of them on the special-function units.
-// Measured there: forward 32 us; the backward's first half 57 us (219 MB, 34 us at the copy rate).
+// Measured there: forward 32 us; the backward's first half 66 us (219 MB, 34 us at the copy rate).
 // Rows widened to tf32 in tensor memory, times two tf32 parts of the scaled weights, with one
-// group of eight epilogue warps, took 61 and 100 us.
+// group of eight epilogue warps, took 61 and 100 us. (With dv and dz as floats the first half took
+// 57 us, and what reads them 46 us more.)
 //
 // Roles of the 20 warps (one persistent CTA per SM):
 //   warp 0       TMA producer of A slabs
@@ -523,7 +524,9 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
 // second one: their scale is another). An item is one rank of 128 rows and 128 input channels, so
 // dv and dz, twice the size of everything else, are read once up to 128 channels.
 //
-// What bounds it: DRAM (179 MB for 100,003 rows of 96 <- 200 channels, 28 us at the copy rate).
+// What bounds it: DRAM (179 MB for 100,003 rows of 96 <- 200 channels, 28 us at the copy rate), but
+// a CTA's ring of 64 KB and 782 tiles on 148 CTAs keep it at 52 us; from float dv and dz (split by
+// threads, gated_ff_stream.cu) it took 73 us.
 //
 // The 12 warps: 0 TMA producer of A slabs, 1 MMA issue, 2 TMA producer of the weights, 4-11
 // epilogue (two per lane quarter, 64 columns each).

@@ -15,12 +15,17 @@
 //   DX   dx_k = dv_k Wv_l (+ sum_l dz_l Wg_l for k = 0): items are (128 rows, component)
 //
 // What bounds it: DRAM (x in, y out: 453 MB for 27,648 x 16 rows of 128 channels, 70 us at the
-// copy rate), with the tensor cores close behind (63 us). A ring whose stages held A and the
-// weights' slabs together was three deep in shared memory and waited for its copies (149 us:
-// gated_ff_stream.cu, still used above 128 channels). Here the item's two weight matrices stay
-// in shared memory (64 output channels x 128 x hi, lo: 64 KB each), work lists are ordered by
-// rank so that they are loaded a few times per launch, and the ring holds A slabs alone. The
-// price is that x is read from L2 once per 64 output channels.
+// copy rate), with the tensor cores close behind (66 us: three products at half the measured
+// bfloat16 rate). Measured there: FWD 110 us (4.1 TB/s), PRE 157 us (736 MB, 4.7 TB/s), DX 114 us
+// (510 MB, 4.5 TB/s); in a loop of seconds the power limit takes another sixth. A slab's MMAs take
+// 385 cycles and its copy 220 of the 870 that it costs: what is left is the latency of the
+// barriers between the roles.
+// A ring whose stages held A and the weights' slabs together was three deep in shared memory and
+// waited for its copies (FWD 149 us, DX 143 us: gated_ff_stream.cu, which still serves above 128
+// channels). Here the item's two weight matrices stay in shared memory (64 output channels x 128 x
+// hi, lo: 64 KB each), work lists are ordered by rank so that they are loaded a few times per
+// launch, and the ring holds A slabs alone. The price is that x is read from L2 once per 64 output
+// channels.
 //
 // A tensor-core accumulation truncates the running sum (measured relative error of one
 // accumulator: 4.5e-7 after 12 instructions, 8.2e-7 after 24, 1.6e-6 after 48), so a slab's
