@@ -1,10 +1,18 @@
-// Gated feed-forward products with more than 128 channels to reduce over: weights streamed
-// (gated_ff_tc.cu keeps them in shared memory below that; measured on 27,648 x 16 rows of 128
-// channels: this kernel 149 us forward, 143 us for the input gradient).
+// Gated feed-forward products with more than 128 channels to reduce over (bfloat16 rows: 256):
+// weights streamed (gated_ff_tc.cu keeps them in shared memory below that; measured on 27,648 x 16
+// rows of 128 channels: this kernel 149 us forward and 143 us for the input gradient, that one 110
+// and 114).
+//
+// What bounds it: the tensor cores (three products: 58 us for 100,003 rows of 200 -> 200 channels);
+// measured there 135 us forward, 217 us first half of the backward, 123 us input gradient. A stage
+// carries 32 KB of weights beside 16 KB of rows, so copies, splitters and MMAs together keep shared
+// memory busy for 900 cycles a slab where the MMAs alone take 770, and four splitter warps do not
+// hide behind them. PRE computes a gate again for each of its rank's components: 64 gates beside 64
+// sums are what its registers hold.
 //
 // One persistent CTA per SM, 16 warps:
 //   warp 0       TMA producer, and the CTA's draw from the work list (an atomic counter)
-//   warp 1       MMA issue (one thread)
+//   warp 1       MMA issue
 //   warps 4-7    splitters: the A slab (128 rows x 32 channels) to tf32 parts in tensor memory
 //   warps 8-15   epilogue: two warps per lane quarter, 64 columns each
 // Every stage of the operand ring holds an A slab and the matching slab of the weights' two
@@ -20,7 +28,7 @@ namespace gtc {
 
 constexpr int BN = STREAM_BN, NACC = STREAM_NACC;
 constexpr int TILE_B = BN * BK * 4;
-constexpr int EPI_WARPS = 8, EPI_BYTES = EPI_WARPS * 2 * EPI_BUF;
+constexpr int EPI_WARPS = 8;
 constexpr int A_COLS = 128;  // tensor-memory columns of the A parts' ring; the accumulators behind them
 
 template <int MODE, typename T>
@@ -29,7 +37,9 @@ struct Cfg {
   static constexpr int TILE_A = BM * BK * (A32 ? 4 : 2);
   static constexpr int STAGE = TILE_A + 2 * TILE_B;
   static constexpr int A_STAGE = A32 ? 2 * BK : BK;  // tensor-memory columns
-  static constexpr int STAGES = A32 ? 3 : 4;
+  // staging boxes per epilogue warp: PRE holds g's two; the others do with one for a fourth stage
+  static constexpr int BUFS = MODE == PRE ? 2 : 1, EPI_BYTES = EPI_WARPS * BUFS * EPI_BUF;
+  static constexpr int STAGES = A32 && MODE == PRE ? 3 : 4;
   static constexpr int A_RING = A_COLS / A_STAGE;
   static constexpr int SMEM = STAGES * STAGE + EPI_BYTES + BAR_BYTES + 1024;
   static_assert(A_COLS + NACC * BN <= 512, "tensor memory");
@@ -81,7 +91,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* epi = smem + S * C::STAGE;
-  uint64_t* full = reinterpret_cast<uint64_t*>(epi + EPI_BYTES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(epi + C::EPI_BYTES);
   uint64_t* split = full + S;
   uint64_t* empty = split + S;
   uint64_t* a_free = empty + S;  // the MMAs have read a slot of the A ring
@@ -149,7 +159,8 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
       constexpr uint32_t bytes = C::TILE_A + 2 * TILE_B;
       int next = (int)blockIdx.x;
       int64_t g = 0;
-      bool ok = true;
+      uint32_t s = 0, lap = 0;
+      bool ok = true, free = true;  // (peeked: the next stage is free)
       for (int q = 0; ok; ++q) {
         const int s4 = q % SCHED;
         if (q >= SCHED &&
@@ -177,17 +188,20 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
               mat = a.ranks + w.l;
             }
             for (int kt = 0; kt < a.nk; ++kt, ++g) {
-              const int s = (int)(g % S);
-              if (g >= S && !wait_phase(smem_u32(&empty[s]), (uint32_t)(((g / S) - 1) & 1), abort_flag)) {
+              if (!free && !wait_phase(smem_u32(&empty[s]), (lap - 1) & 1u, abort_flag)) {
                 ok = false;
                 break;
               }
+              const uint32_t s_next = (s + 1) % S, lap_next = s_next ? lap : lap + 1;
+              free = lap_next == 0 || peek_parity(smem_u32(&empty[s_next]), (lap_next - 1) & 1u);
               uint8_t* st = smem + s * C::STAGE;
               const uint32_t fb = smem_u32(&full[s]);
               arrive_tx(fb, bytes);
               tma_load_3d(smem_u32(st), ma, kt * BK, w.tile * BM, z, fb);
               tma_load_3d(smem_u32(st + C::TILE_A), &mp.b, kt * BK, w.ct * BN, mat, fb);
               tma_load_3d(smem_u32(st + C::TILE_A + TILE_B), &mp.b, kt * BK, w.ct * BN, mat + 2 * a.ranks, fb);
+              s = s_next;
+              lap = lap_next;
             }
           }
       }
@@ -196,85 +210,84 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
         const int64_t uses = g > s ? (g - 1 - s) / S + 1 : 0;
         if (uses > 0) drain_bar(smem_u32(&full[s]), (uint32_t)((uses - 1) & 1));
       }
-    } else if (warp == 1 && elect_one()) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------------- MMA issue
-      int64_t g = 0, u = 0;
-      bool ok = true;
+      uint32_t s = 0, phase = 0, slot = 0, b = 0, acc_phase = 0;
+      bool ok = true, split_ready = false, acc_ready = false;  // answers about the next slab and accumulator
       for (int q = 0; ok; ++q) {
-        const int s4 = q % SCHED;
-        if (!wait_phase(smem_u32(&sched_full[s4]), (uint32_t)((q / SCHED) & 1), abort_flag)) break;
-        const int it = *reinterpret_cast<volatile int*>(&sched[s4]);
-        arrive(smem_u32(&sched_empty[s4]));
+        const int it = next_item(q);
         if (it < 0) break;
         const Item w = item_of<MODE>(a, it);
-        const int passes = substeps(w) * segments(w);
-        for (int p = 0; p < passes && ok; ++p)
-          for (int j = 0; j < a.nu && ok; ++j, ++u) {
-            const int b = (int)(u % NACC);
-            const int64_t v = u / NACC;
-            if (v >= 1 && !wait_phase(smem_u32(&acc_empty[b]), (uint32_t)((v - 1) & 1), abort_flag)) {
-              ok = false;
-              break;
-            }
+        const int units = substeps(w) * segments(w) * a.nu;
+        int kt = 0;
+        for (int j = 0; j < units; ++j) {
+          if (!acc_ready) ok = wait_warp(smem_u32(&acc_empty[b]), acc_phase ^ 1u, abort_flag);
+          const uint32_t d = tmem + (uint32_t)A_COLS + b * (uint32_t)BN;
+          const uint32_t b_next = b + 1 == (uint32_t)NACC ? 0u : b + 1, acc_next = acc_phase ^ (b_next ? 0u : 1u);
+          const int n = min(a.kg, a.nk - kt);
+#pragma unroll 1
+          for (int i = 0; i < n; ++i) {
+            if (!split_ready) ok = ok && wait_warp(smem_u32(&split[s]), phase, abort_flag);
+            if (!ok) break;
             asm volatile("tcgen05.fence::after_thread_sync;");
-            const uint32_t d = tmem + (uint32_t)(A_COLS + b * BN);
-            const int k_end = min(a.nk, (j + 1) * a.kg);
-            for (int kt = j * a.kg; kt < k_end; ++kt, ++g) {
-              const int s = (int)(g % S);
-              if (!wait_phase(smem_u32(&split[s]), (uint32_t)((g / S) & 1), abort_flag)) {
-                ok = false;
-                break;
-              }
-              asm volatile("tcgen05.fence::after_thread_sync;");
-              uint8_t* st = smem + s * C::STAGE;
-              const uint64_t dbh = make_desc(smem_u32(st + C::TILE_A));
-              const uint64_t dbl = make_desc(smem_u32(st + C::TILE_A + TILE_B));
-              const int slot = (int)(g % C::A_RING);
-              const uint32_t tah = tmem + (uint32_t)(slot * C::A_STAGE), tal = tah + (uint32_t)BK;
+            const uint32_t s_next = s + 1 == (uint32_t)S ? 0u : s + 1, phase_next = phase ^ (s_next ? 0u : 1u);
+            const bool peek = peek_parity(smem_u32(&split[s_next]), phase_next);
+            const bool peek_acc = peek_parity(smem_u32(&acc_empty[b_next]), acc_next ^ 1u);
+            const uint64_t dbh = make_desc(smem_u32(smem + s * C::STAGE + C::TILE_A)), dbl = dbh + (TILE_B >> 4);
+            const uint32_t tah = tmem + slot * (uint32_t)C::A_STAGE, tal = tah + (uint32_t)BK;
+            if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < BK / 8; ++kk) {
-                const uint64_t off = (uint64_t)((kk * 32) >> 4);
-                mma_ta<BN>(d, tah + kk * 8, dbl + off, (kt > j * a.kg || kk > 0) ? 1u : 0u);
-                if (C::A32) mma_ta<BN>(d, tal + kk * 8, dbh + off, 1u);
+                mma_ta<BN>(d, tah + kk * 8, dbl + 2 * kk, (i > 0 || kk > 0) ? 1u : 0u);
+                if (C::A32) mma_ta<BN>(d, tal + kk * 8, dbh + 2 * kk, 1u);
               }
 #pragma unroll
-              for (int kk = 0; kk < BK / 8; ++kk) mma_ta<BN>(d, tah + kk * 8, dbh + (uint64_t)((kk * 32) >> 4), 1u);
+              for (int kk = 0; kk < BK / 8; ++kk) mma_ta<BN>(d, tah + kk * 8, dbh + 2 * kk, 1u);
               // the stage and the A slot are free once these MMAs have completed
               commit(smem_u32(&empty[s]));
               commit(smem_u32(&a_free[slot]));
+              if (i + 1 == n) commit(smem_u32(&acc_full[b]));
             }
-            if (ok) commit(smem_u32(&acc_full[b]));
+            split_ready = __all_sync(0xffffffffu, peek);
+            acc_ready = __all_sync(0xffffffffu, peek_acc);
+            s = s_next;
+            phase = phase_next;
+            slot = slot + 1 == (uint32_t)C::A_RING ? 0u : slot + 1;
           }
+          if (!ok) break;
+          kt = kt + n == a.nk ? 0 : kt + n;
+          b = b_next;
+          acc_phase = acc_next;
+        }
       }
-      commit(smem_u32(drain));  // every MMA completes before tensor memory is freed
-      drain_bar(smem_u32(drain), 0);
+      if (elect_one()) {
+        commit(smem_u32(drain));  // every MMA completes before tensor memory is freed
+        drain_bar(smem_u32(drain), 0);
+      }
+      __syncwarp();
     }
   } else if (warp < 8) {
     FC_SETMAXNREG_DEC(96);
     // ------------------------------------------------------------------ splitters
     const int r = (warp & 3) * 32 + lane;  // row of the slab, lane of tensor memory
-    int64_t g = 0;
-    bool ok = true;
+    uint32_t s = 0, phase = 0, slot = 0, slot_phase = 1;  // (slots are free at first)
+    bool ok = true, full_ready = false, slot_ready = false;
     for (int q = 0; ok; ++q) {
       const int it = next_item(q);
       if (it < 0) break;
       const Item w = item_of<MODE>(a, it);
-      const int64_t end = g + (int64_t)substeps(w) * segments(w) * a.nk;
-      for (; g < end; ++g) {
-        const int s = (int)(g % S);
-        if (!wait_warp(smem_u32(&full[s]), (uint32_t)((g / S) & 1), abort_flag)) {
-          ok = false;
-          break;
-        }
-        const int slot = (int)(g % C::A_RING);
-        if (g >= C::A_RING &&
-            !wait_warp(smem_u32(&a_free[slot]), (uint32_t)((g / C::A_RING - 1) & 1), abort_flag)) {
-          ok = false;
-          break;
-        }
+      for (int left = substeps(w) * segments(w) * a.nk; left > 0; --left) {
+        if (!full_ready) ok = wait_warp(smem_u32(&full[s]), phase, abort_flag);
+        if (!slot_ready) ok = ok && wait_warp(smem_u32(&a_free[slot]), slot_phase, abort_flag);
+        if (!ok) break;
+        const uint32_t s_next = s + 1 == (uint32_t)S ? 0u : s + 1, phase_next = phase ^ (s_next ? 0u : 1u);
+        const uint32_t slot_next = slot + 1 == (uint32_t)C::A_RING ? 0u : slot + 1;
+        const uint32_t slot_phase_next = slot_phase ^ (slot_next ? 0u : 1u);
+        const bool peek_full = peek_parity(smem_u32(&full[s_next]), phase_next);
+        const bool peek_slot = peek_parity(smem_u32(&a_free[slot_next]), slot_phase_next);
         asm volatile("tcgen05.fence::after_thread_sync;");
         const uint8_t* slab = smem + s * C::STAGE;
-        const uint32_t ta = tmem + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(slot * C::A_STAGE);
+        const uint32_t ta = tmem + ((uint32_t)((warp & 3) * 32) << 16) + slot * (uint32_t)C::A_STAGE;
         if constexpr (C::A32) {
           uint32_t x[32];
 #pragma unroll
@@ -299,26 +312,31 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) arrive(smem_u32(&split[s]));
+        full_ready = __all_sync(0xffffffffu, peek_full);
+        slot_ready = __all_sync(0xffffffffu, peek_slot);
+        s = s_next;
+        phase = phase_next;
+        slot = slot_next;
+        slot_phase = slot_phase_next;
       }
     }
   } else {
     FC_SETMAXNREG_INC(184);
     // ------------------------------------------------------------------ epilogue
     const int quarter = warp & 3, half = (warp - 8) >> 2;
-    uint8_t* stage0 = epi + (warp - 8) * 2 * EPI_BUF;
+    uint8_t* stage0 = epi + (warp - 8) * C::BUFS * EPI_BUF;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(A_COLS + half * 64);
     const float sa = MODE == DX ? 0.f : __ldg(a.scales + a.ranks + 1);
-    int64_t u = 0;
-    int nbuf = 0;
+    uint32_t u = 0;
     uint32_t aux_phase = 0;
     bool ok = true;
     // units u .. u+count-1 are complete (their accumulators are read and then given back)
-    auto wait_unit = [&](int64_t v) {
+    auto wait_unit = [&](uint32_t v) {
       const bool done = wait_warp(smem_u32(&acc_full[v % NACC]), (uint32_t)((v / NACC) & 1), abort_flag);
       asm volatile("tcgen05.fence::after_thread_sync;");
       return done;
     };
-    auto free_unit = [&](int64_t v) {
+    auto free_unit = [&](uint32_t v) {
       asm volatile("tcgen05.fence::before_thread_sync;");
       __syncwarp();
       if (lane == 0) arrive(smem_u32(&acc_empty[v % NACC]));
@@ -359,12 +377,10 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
 #pragma unroll
         for (int cb = 0; cb < 2; ++cb)
           if (cb < nch) {
-            if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             __syncwarp();
-            uint8_t* buf = stage0 + nbuf * EPI_BUF;
-            put_row<T>(buf, lane, acc + cb * 32);
-            send(&mp.o, buf, col0 + cb * 32, row0, w.k0);
-            nbuf ^= 1;
+            put_row<T>(stage0, lane, acc + cb * 32);
+            send(&mp.o, stage0, col0 + cb * 32, row0, w.k0);
           }
       } else {
         // the gate: pre-activations of this thread's row and 64 columns
@@ -391,7 +407,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
         }
         if constexpr (MODE == FWD) {
 #pragma unroll
-          for (int c = 0; c < 64; ++c) z[c] = sa * gated_act<float>(a.act, z[c]);
+          for (int c = 0; c < 64; ++c) z[c] = sa * fast_act(a.act, z[c]);
           for (int m = 0; m < w.nm && ok; ++m) {
             float acc[64];
 #pragma unroll
@@ -413,12 +429,10 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb)
               if (cb < nch) {
-                if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+                if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
                 __syncwarp();
-                uint8_t* buf = stage0 + nbuf * EPI_BUF;
-                put_row<T>(buf, lane, acc + cb * 32);
-                send(&mp.o, buf, col0 + cb * 32, row0, w.k0 + m);
-                nbuf ^= 1;
+                put_row<T>(stage0, lane, acc + cb * 32);
+                send(&mp.o, stage0, col0 + cb * 32, row0, w.k0 + m);
               }
           }
         } else {
