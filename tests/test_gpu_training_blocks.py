@@ -307,6 +307,30 @@ def test_gated_large_passes_repeat_their_bits(cuda_device, dtype, n, l_max, c, h
         assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gated_more_than_2_to_31_elements(cuda_device, dtype):
+    # 1,100 times the same 1,000 rows: every copy has the first one's results, and the weights'
+    # gradients are 1,100 times its own
+    n, reps, l_max, c = 1000, 1100, 3, 128
+    x, wv, wg, b, sc, g = R.gated_inputs(n, l_max, c, c, True, dtype, "cuda", seed=7)
+    ins = [wg, b, *wv]
+    for t in ins:
+        t.requires_grad_(True)
+
+    def both(x, g):
+        x = x.requires_grad_(True)
+        y = ops.gated_feed_forward(x, wv, wg, b, sc, l_max, "silu")
+        return y.detach(), *torch.autograd.grad(y, [x, *ins], g)
+
+    want_y, want_x, *_ = both(x.clone(), g)
+    _, exact = R.gated_grads(x, wv, wg, b, sc, l_max, "silu", g)
+    y, gx, *got = both(x.repeat(reps, 1), g.repeat(reps, 1))
+    assert y.numel() > 2 ** 31
+    assert bool((y.view(reps, n, -1) == want_y).all()) and bool((gx.view(reps, n, -1) == want_x).all())
+    for a, w in zip(got, exact[1:]):
+        assert _rel(a, reps * w) <= _gated_tol(dtype, c, 7 * n * reps)
+
+
 def test_gated_subsets_of_gradients(cuda_device):
     x, wv, wg, b, sc, g = R.gated_inputs(300, 2, 64, 64, True, F32, "cuda")
     every = [x, wg, b, *wv]
