@@ -343,6 +343,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) gated_tc_kernel(const __grid_co
             if (through) commit(smem_u32(&w_free[slot]));
           }
           __syncwarp();
+          // an odd number of slabs swaps the warps' slabs from pass to pass: the other one's weights
+          // have to be there as well before this warp's next pass
+          if (check_w && (nk & 1))
+            for (int kt = first ^ 1; kt < nk; kt += 2)
+              ok = ok && wait_warp(smem_u32(&w_full[slot * MAX_NK + kt]), (w_phase >> slot) & 1u, abort_flag);
           par ^= nk & 1;
           if (!ok) break;
           check &= ~(1u << slot);

@@ -292,10 +292,14 @@ def test_gated_water_box_size(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype,n,l_max,c,h", [(F32, 27648, 3, 128, 128), (BF16, 27648, 3, 128, 128),
-                                               (F32, 9001, 2, 200, 136), (BF16, 100003, 0, 96, 200)])
+                                               (F32, 9001, 2, 200, 136), (BF16, 100003, 0, 96, 200),
+                                               (F32, 13869, 3, 48, 88), (F32, 27648, 2, 96, 96),
+                                               (F32, 27648, 3, 24, 32), (F32, 27648, 1, 160, 224),
+                                               (BF16, 20001, 2, 40, 72), (BF16, 9001, 1, 300, 136)])
 def test_gated_large_passes_repeat_their_bits(cuda_device, dtype, n, l_max, c, h):
     # one ring stage refilled while a few of its values are still being read shows in one product of
-    # 10^5: about one pass of three at these sizes, so a hundred passes show it
+    # 10^5: about one pass of three at these sizes, so a hundred passes show it. Odd numbers of slabs
+    # (88, 96, 24 channels): weights used before they are there
     x, wv, wg, _, scales, g = R.gated_inputs(n, l_max, c, h, False, dtype, "cuda", seed=3)
     for t in (x, wg, *wv):
         t.requires_grad_(True)
