@@ -11,7 +11,7 @@
 //
 // What bounds it: the epilogue. 100,003 rows of 96 -> 200 channels are 59 MB (9 us), but a
 // gate costs about 25 instructions, two of them on the special-function units.
-// Measured there: forward 32 us; the backward's first half 66 us (219 MB, 34 us at the copy rate).
+// Measured there: forward 31 us; the backward's first half 64 us (219 MB, 34 us at the copy rate).
 // Rows widened to tf32 in tensor memory, times two tf32 parts of the scaled weights, with one
 // group of eight epilogue warps, took 61 and 100 us. (With dv and dz as floats the first half took
 // 57 us, and what reads them 46 us more.)
@@ -52,6 +52,25 @@ struct DCfg {
   static constexpr int FIXED = EPI_WARPS * BUFS * BOX + BAR_BYTES + 1024;
   static int stages(int nk) { return std::min(MAX_STAGES, (SMEM_MAX - FIXED - 2 * nk * W_SLAB) / TILE_A); }
   static int smem(int nk, int st) { return FIXED + 2 * nk * W_SLAB + st * TILE_A; }
+};
+
+// Every step-th item of a list, without a division per item (what one thread does for an item bounds
+// the short ones).
+struct Walk {
+  int tile, q, step, tiles, end;
+  __device__ __forceinline__ Walk(const Args& a, int first, int step_)
+      : q(first / a.tiles), step(step_), tiles(a.tiles), end(a.per_comp ? a.comps : a.ranks) {
+    tile = first - q * a.tiles;
+  }
+  __device__ __forceinline__ bool more() const { return q < end; }
+  __device__ __forceinline__ void next() {
+    tile += step;
+    while (tile >= tiles) {
+      tile -= tiles;
+      ++q;
+    }
+  }
+  __device__ __forceinline__ WorkItem item(const Args& a) const { return work_item(a, tile, q); }
 };
 
 // D (+)= A x B of one 64-channel slab, both K-major in shared memory; N rows of B.
@@ -150,7 +169,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
 
   // The CTA's items: every `lists`-th of its column tile's list. (Drawn from a shared counter and
   // handed to the warps through barriers, each item cost every warp a barrier's answer.)
-  const int first = (int)blockIdx.x / a.n_ct, lists = (int)gridDim.x / a.n_ct, items = (int)a.items;
+  const int first = (int)blockIdx.x / a.n_ct, lists = (int)gridDim.x / a.n_ct;
 
   if (warp < EPI_WARP0) {
     FC_SETMAXNREG_DEC(40);
@@ -160,16 +179,19 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
       uint32_t lap = 0;  // of the ring
       int64_t g = 0;
       bool ok = true, free = true;  // (peeked: the next stage is free)
-      for (int it = first; it < items && ok; it += lists) {
-        const WorkItem w = work_item(a, it);
+      Walk at(a, first, lists);
+      WorkItem w = at.item(a);
+      for (bool more = at.more(); more && ok;) {
+        at.next();
+        more = at.more();
+        const WorkItem wn = at.item(a);  // (used where there is more)
         const int lead = w.k0 == 0 ? 0 : 1;  // passes before the first component's
         for (int p = 0; p < lead + w.nm && ok; ++p) {
           const int z = p < lead ? 0 : w.k0 + p - lead;
           if (p + 1 < lead + w.nm) {
             tma_prefetch_3d(&mp.ap, 0, w.tile * BM, w.k0 + p + 1 - lead);
             if (MODE == PRE) tma_prefetch_3d(&mp.gp, ct * BN, w.tile * BM, w.k0 + p + 1 - lead);
-          } else if (it + lists < items) {
-            const WorkItem wn = work_item(a, it + lists);
+          } else if (more) {
             tma_prefetch_3d(&mp.ap, 0, wn.tile * BM, 0);
             if (MODE == PRE) tma_prefetch_3d(&mp.gp, ct * BN, wn.tile * BM, wn.k0);
           }
@@ -188,6 +210,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
             lap = lap_next;
           }
         }
+        w = wn;
       }
       // the last copy into every stage must have landed before the CTA exits
       for (int t = 0; t < S; ++t) {
@@ -198,8 +221,8 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
       // ---------------------------------------------------------------- weight producer
       int rank = -1, loads[2] = {0, 0};
       bool ok = true;
-      for (int it = first; it < items && ok; it += lists) {
-        const WorkItem w = work_item(a, it);
+      for (Walk at(a, first, lists); at.more() && ok; at.next()) {
+        const WorkItem w = at.item(a);
         if (w.l == rank) continue;
         rank = w.l;
 #pragma unroll
@@ -229,8 +252,13 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
       uint32_t s = 0, lap = 0, pc[2] = {0u, 0u};  // passes of each group so far
       bool ok = true, ready_a = false;  // (peeked: the next slab is there)
       int group = 1;
-      for (int it = first; it < items && ok; it += lists) {
-        const WorkItem w = work_item(a, it);
+      bool acc_ready = false;  // (peeked: the next pass's accumulator is free)
+      Walk at(a, first, lists);
+      WorkItem w = at.item(a);
+      for (bool more = at.more(); more && ok;) {
+        at.next();
+        more = at.more();
+        const WorkItem wn = at.item(a);
         group ^= 1;
         bool check = false;
         if (w.l != rank) {
@@ -251,7 +279,12 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
           // epilogue frees the first one before the second
           const bool two = both && p == 0;
           const uint32_t n2 = n + (two ? 1u : 0u), b = group * C::NG + n % C::NG, b2 = group * C::NG + n2 % C::NG;
-          ok = wait_warp(smem_u32(&acc_empty[b2]), (n2 / C::NG & 1u) ^ 1u, abort_flag);
+          if (!acc_ready) ok = wait_warp(smem_u32(&acc_empty[b2]), (n2 / C::NG & 1u) ^ 1u, abort_flag);
+          acc_ready = false;
+          // the accumulator that the next pass waits for: this group's next one, or the other's
+          const bool same = p + 1 < passes;
+          const uint32_t nx = same ? n + 1 : (group ? pc[0] : pc[1]) + (wn.k0 == 0 ? 1u : 0u);
+          const uint32_t bx = (same ? group : group ^ 1) * C::NG + nx % C::NG;
           const uint32_t slot = p == 0 ? 0u : 1u;
           for (int kt = 0; kt < nk; ++kt) {
             if (check && p < 2) {
@@ -264,6 +297,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
             asm volatile("tcgen05.fence::after_thread_sync;");
             const uint32_t s_next = s + 1 == (uint32_t)S ? 0u : s + 1, lap_next = s_next ? lap : lap + 1;
             const bool peek = peek_parity(smem_u32(&full[s_next]), lap_next & 1u);
+            const bool peek_acc = peek_parity(smem_u32(&acc_empty[bx]), (nx / C::NG & 1u) ^ 1u);
             if (elect_one()) {
               const uint64_t da = adesc + (uint64_t)(s * (TILE_A >> 4));
               const uint64_t db = wdesc + (uint64_t)((2 * kt + slot) * (W_SLAB >> 4));
@@ -276,6 +310,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
               commit(smem_u32(&empty[s]));  // the stage is free once these MMAs have completed
             }
             ready_a = __all_sync(0xffffffffu, peek);
+            acc_ready = __all_sync(0xffffffffu, peek_acc);
             s = s_next;
             lap = lap_next;
           }
@@ -288,6 +323,7 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
         }
         if (group) pc[1] = n;
         else pc[0] = n;
+        w = wn;
       }
       if (elect_one()) {
         commit(smem_u32(drain));  // every MMA completes before tensor memory is freed
@@ -353,8 +389,8 @@ __global__ void __launch_bounds__(D_THREADS, 1) gated_bf16_kernel(const __grid_c
       __syncwarp();
     };
     uint32_t box = 0, box_phase = 0;  // PRE: the box in turn; bit b: parity of landed[b]'s next completion
-    for (int it = first + group * lists; it < items && ok; it += 2 * lists) {
-      const WorkItem w = work_item(a, it);
+    for (Walk at(a, first + group * lists, 2 * lists); at.more() && ok; at.next()) {
+      const WorkItem w = at.item(a);
       const int row0 = w.tile * BM + quarter * 32;
       const float sv = __ldg(a.scales + w.l);
       // ask for component m's box of g

@@ -50,10 +50,9 @@ struct WorkItem {
 };
 
 // Lists run through the ranks (high ones first: most work), all tiles of one before the next.
-__device__ __forceinline__ WorkItem work_item(const Args& a, int it) {
+__device__ __forceinline__ WorkItem work_item(const Args& a, int tile, int q) {
   WorkItem w;
-  const int q = it / a.tiles;
-  w.tile = it - q * a.tiles;
+  w.tile = tile;
   if (a.per_comp) {
     w.k0 = a.comps - 1 - q;
     w.l = gated_rank_of(w.k0);
@@ -64,6 +63,10 @@ __device__ __forceinline__ WorkItem work_item(const Args& a, int it) {
     w.nm = 2 * w.l + 1;
   }
   return w;
+}
+__device__ __forceinline__ WorkItem work_item(const Args& a, int it) {
+  const int q = it / a.tiles;
+  return work_item(a, it - q * a.tiles, q);
 }
 
 // N consecutive columns of this thread's lane (warp-collective), waited for in the same statement:
