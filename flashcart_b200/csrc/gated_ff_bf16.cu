@@ -9,9 +9,10 @@
 // one's products run. For scalars (component 0) the gate and value products share one pass over
 // the slab.
 //
-// What bounds it: the epilogue. 100,003 rows of 96 -> 200 channels are 59 MB (9 us), but a
-// gate costs about 25 instructions, two of them on the special-function units.
-// Measured there: forward 31 us; the backward's first half 64 us (219 MB, 34 us at the copy rate).
+// What bounds it: the barriers between copy, issue and epilogue. 100,003 rows of 96 -> 200 channels
+// are 59 MB (9 us) and their gates 12 us of the special-function units, but a scalar item costs 1.3
+// us whatever columns its epilogue has. Measured there: forward 31 us; the backward's first half 64
+// us (219 MB, 34 us at the copy rate).
 // Rows widened to tf32 in tensor memory, times two tf32 parts of the scaled weights, with one
 // group of eight epilogue warps, took 61 and 100 us. (With dv and dz as floats the first half took
 // 57 us, and what reads them 46 us more.)
