@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(256) embed_fwd_vec(const T* __restrict__ table
   }
 }
 
-// Rows of any length from a vector's on: a thread writes aligned vectors of the flat output, whose
+// Rows of any length from a vector's on, of a table that has rows (a wrong index reads row 0, and what
+// it reads is not written): a thread writes aligned vectors of the flat output, whose
 // elements belong to one row or two, so every element is read from one of two places without a
 // branch (a warp's lanes cross rows at different elements). Two vectors per thread and step. 67 M
 // elements in rows of 63: 81 us in float32 and 69 in bfloat16 (with a row test per element, as
@@ -234,7 +235,7 @@ int embed_fwd(const void* table_, int64_t V, int64_t D, const int64_t* idx, int6
     else
       embed_fwd_vec<T, uint64_t><<<grid, 256, 0, s>>>(table, V, (int)(D / NV), idx, units, (A)scale, (A)offset, out,
                                                       status);
-  } else if (D >= NV && !(ao & 15) && R * D < ((int64_t)1 << 31) && V * D < ((int64_t)1 << 31)) {
+  } else if (V > 0 && D >= NV && !(ao & 15) && R * D < ((int64_t)1 << 31) && V * D < ((int64_t)1 << 31)) {
     const int64_t b = (R * D + 512 * NV - 1) / (512 * NV);
     const unsigned grid = (unsigned)(b < 148 * 16 ? b : 148 * 16);
     embed_fwd_odd<T><<<grid, 256, 0, s>>>(table, (uint32_t)V, (uint32_t)D, idx, (uint32_t)R, (uint32_t)(R * D),
