@@ -1879,6 +1879,19 @@ def _gated_composed(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Ten
     return (v.view(n, ranks * ranks, h) * a.index_select(1, of)).reshape(n, ranks * ranks * h).to(dtype)
 
 
+def _gated_composed_grads(g: Tensor, x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor,
+                          gate_bias: Optional[Tensor], scales: Tensor, l_max: int, activation: str,
+                          need: Sequence[bool]) -> List[Optional[Tensor]]:
+    """Gradients of (x, gate_weight, gate_bias, *value_weights) as a differentiable composition,
+    None where ``need`` is false. They are taken with respect to views: a saved tensor may be an
+    ancestor of another one (a weight used twice), may stand in two places, and has hooks that
+    belong to the caller's backward, not to this one."""
+    ins = [None if t is None else t.view_as(t) for t in (x, gate_weight, gate_bias, *value_weights)]
+    y = _gated_composed(ins[0], ins[3:], ins[1], ins[2], scales, l_max, activation)
+    got = iter(torch.autograd.grad(y, [t for t, n in zip(ins, need) if n], g, create_graph=True))
+    return [next(got) if n else None for n in need]
+
+
 class _GatedFeedForward(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_weight, gate_bias, scales, l_max, activation, *value_weights):
@@ -1891,12 +1904,8 @@ class _GatedFeedForward(torch.autograd.Function):
         x, wg, b, scales, *wv = ctx.saved_tensors
         l_max, activation = ctx.args
         need = [ctx.needs_input_grad[i] for i in (0, 1, 2, *range(6, 6 + len(wv)))]
-        if torch.is_grad_enabled():
-            # a second derivative is wanted: the gradient as a differentiable composition
-            ins = [x, wg, b, *wv]
-            y = _gated_composed(x, wv, wg, b, scales, l_max, activation)
-            got = iter(torch.autograd.grad(y, [t for t, n in zip(ins, need) if n], g, create_graph=True))
-            outs = [next(got) if n else None for n in need]
+        if torch.is_grad_enabled():  # a second derivative is wanted
+            outs = _gated_composed_grads(g, x, wv, wg, b, scales, l_max, activation, need)
         else:
             outs = _gated_ff_bwd(g, x, wv, wg, b, scales, l_max, activation, need)
         return (*outs[:3], None, None, None, *outs[3:])

@@ -28,3 +28,54 @@ def test_embedding_in_an_empty_table(cuda_device, dtype, dim):
             ops.check_device_status()
     assert ops.embedding(table, idx[:0]).shape == (0, dim)
     ops.check_device_status()
+
+
+def _leaves(*ts):
+    return [None if t is None else t.detach().clone().requires_grad_(True) for t in ts]
+
+
+@pytest.mark.parametrize("graph", [False, True])
+@pytest.mark.parametrize("use", ["twice", "value and gate", "two ranks"])
+def test_gated_weights_in_two_places(cuda_device, graph, use):
+    """A weight used by two calls of which one feeds the other, and one tensor as two of a call's
+    weights: every gradient is the definition's, whether or not the backward builds a graph."""
+    l_max = 1 if use == "two ranks" else 0
+    x, wv, wg, b, sc, g = R.gated_inputs(7, l_max, 6, 6, True, F64, "cuda", seed=1)
+
+    def run(f):
+        xs, w0, w1, gate, bias = _leaves(x, wv[0], wv[-1], wg, b)
+        ws = [w0, w0] if use == "two ranks" else [w0]
+        gate = w0 if use == "value and gate" else gate
+        y = f(xs, ws, gate, bias, sc, l_max, "silu")
+        if use == "twice":
+            y = f(y, ws, gate, bias, sc, l_max, "silu")
+        ins = [xs, w0, bias] + ([] if use == "value and gate" else [gate])
+        return [t.detach() for t in torch.autograd.grad(y, ins, g, create_graph=graph)]
+
+    for got, want in zip(run(ops.gated_feed_forward), run(R.gated)):
+        # sums of some dozen terms, twice over
+        assert ((got - want).norm() / want.norm()).item() <= 2.0 ** -53 * 512
+
+
+@pytest.mark.parametrize("graph", [False, True])
+def test_gated_gradient_hooks_run_once(cuda_device, graph):
+    """A hook that scales a gradient scales it once, and none runs for what is not asked for."""
+    x, wv, wg, b, sc, g = R.gated_inputs(5, 1, 4, 4, True, F64, "cuda", seed=2)
+
+    def run(f, hooks):
+        xs, w0, w1, gate, bias = _leaves(x, *wv, wg, b)
+        seen = []
+        if hooks:
+            for name, t, k in (("x", xs, 10.0), ("w", w0, 3.0), ("gate", gate, 7.0)):
+                t.register_hook(lambda v, name=name, k=k: seen.append(name) or k * v)
+        y = f(xs, [w0, w1], gate, bias, sc, 1, "sigmoid")
+        return torch.autograd.grad(y, [xs, w0, gate, bias], g, create_graph=graph), seen
+
+    (gx, gw, gg, gb), seen = run(ops.gated_feed_forward, True)
+    assert sorted(seen) == ["gate", "w", "x"]
+    plain, _ = run(ops.gated_feed_forward, False)
+    for got, want, k in zip((gx, gw, gg, gb), plain, (10.0, 3.0, 7.0, 1.0)):
+        assert torch.equal(got, k * want)
+    xs, w0, w1, gate, bias = _leaves(x, *wv, wg, b)
+    w0.register_hook(lambda v: pytest.fail("the weight's gradient was not asked for"))
+    torch.autograd.grad(ops.gated_feed_forward(xs, [w0, w1], gate, bias, sc, 1, "sigmoid"), xs, g, create_graph=graph)
