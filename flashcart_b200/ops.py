@@ -23,6 +23,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from flashcart_b200 import _native as N
 
@@ -1579,7 +1580,8 @@ class timed_region:
 # Element embedding, gated feed-forward and irreps dropout. They take float32, float64 and
 # bfloat16 rows, return every gradient, and may be differentiated twice (force training). The
 # entry points run as autograd functions on the impl functions below, without the dispatcher's
-# cost per call; the same operators are registered as flashcart::* for traced programs.
+# cost per call; the same operators are registered as flashcart::* for traced programs, and the
+# entry points go through them where something records or replaces operator calls.
 
 
 def _block_code(dtype: torch.dtype, what: str) -> int:
@@ -1591,7 +1593,17 @@ def _block_code(dtype: torch.dtype, what: str) -> int:
 
 
 def _grad_needed(*tensors: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call is an autograd function's: gradients are wanted, or inputs may have the
+    tangents of forward-mode differentiation."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+            or forward_ad._current_level >= 0)
+
+
+def _recorded() -> bool:
+    """Whether operator calls are compiled, traced, or seen by a dispatch mode (make_fx, fake
+    tensors, counters): a call past the dispatcher would be missing there."""
+    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
+            or torch._C._get_tracing_state() is not None)
 
 
 # The host's share of a call decides small sizes, so these calls pass plain integers and look
@@ -1674,6 +1686,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, index, scale, offset):
         ctx.save_for_backward(index)
+        ctx.save_for_forward(index)
         ctx.args = (table.shape[0], scale)
         return _embedding_fwd(table, index, scale, offset)
 
@@ -1685,6 +1698,10 @@ class _Embedding(torch.autograd.Function):
             return _EmbeddingGrad.apply(g, index, n, scale), None, None, None
         return _embedding_bwd(g, index, n, scale), None, None, None
 
+    @staticmethod
+    def jvp(ctx, table_t, *_):
+        return embedding(table_t, ctx.saved_tensors[0], ctx.args[1])
+
 
 class _EmbeddingGrad(torch.autograd.Function):
     """The table gradient as a function of the output gradient (its gradient is a lookup)."""
@@ -1692,13 +1709,21 @@ class _EmbeddingGrad(torch.autograd.Function):
     @staticmethod
     def forward(ctx, g, index, n_types, scale):
         ctx.save_for_backward(index)
-        ctx.scale = scale
+        ctx.save_for_forward(index)
+        ctx.args = (n_types, scale)
         return _embedding_bwd(g, index, n_types, scale)
 
     @staticmethod
     def backward(ctx, v):
         (index,) = ctx.saved_tensors
-        return embedding(v, index, ctx.scale), None, None, None
+        return embedding(v, index, ctx.args[1]), None, None, None
+
+    @staticmethod
+    def jvp(ctx, g_t, *_):
+        n_types, scale = ctx.args
+        if _grad_needed(g_t):
+            return _EmbeddingGrad.apply(g_t, ctx.saved_tensors[0], n_types, scale)
+        return _embedding_bwd(g_t, ctx.saved_tensors[0], n_types, scale)
 
 
 def embedding(table: Tensor, index: Tensor, scale: float = 1.0, offset: float = 0.0) -> Tensor:
@@ -1710,7 +1735,7 @@ def embedding(table: Tensor, index: Tensor, scale: float = 1.0, offset: float = 
     inputs give equal bits), in float32 (float64 for float64 tables) and rounded once. An
     index outside the table sets ``FC_DEV_BAD_INDEX`` (:func:`check_device_status`); its row
     is zeros and its gradient is dropped."""
-    if torch.compiler.is_compiling():
+    if _recorded():
         return torch.ops.flashcart.embedding_fwd(table, index, float(scale), float(offset))
     if _grad_needed(table):
         return _Embedding.apply(table, index, float(scale), float(offset))
@@ -1745,6 +1770,7 @@ class _IrrepsDropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, rng, p, l_max):
         ctx.save_for_backward(rng)
+        ctx.save_for_forward(rng)
         ctx.args = (p, l_max)
         return _irreps_dropout(x, rng, p, l_max)
 
@@ -1752,6 +1778,10 @@ class _IrrepsDropout(torch.autograd.Function):
     def backward(ctx, g):
         (rng,) = ctx.saved_tensors
         return irreps_dropout(g, rng, *ctx.args), None, None, None
+
+    @staticmethod
+    def jvp(ctx, x_t, *_):
+        return irreps_dropout(x_t, ctx.saved_tensors[0], *ctx.args)
 
 
 def irreps_dropout(x: Tensor, rng: Tensor, p: float, l_max: int = 0) -> Tensor:
@@ -1763,7 +1793,7 @@ def irreps_dropout(x: Tensor, rng: Tensor, p: float, l_max: int = 0) -> Tensor:
     from them in the gradient and never stored, so they must not change in between (advance a
     copy, as :class:`flashcart_b200.nn.blocks.IrrepsDropout` does). ``p = 1`` drops everything;
     a dropped element is 0 whatever it held."""
-    if torch.compiler.is_compiling():
+    if _recorded():
         return torch.ops.flashcart.irreps_dropout(x, rng, float(p), int(l_max))
     if _grad_needed(x):
         return _IrrepsDropout.apply(x, rng, float(p), int(l_max))
@@ -1910,6 +1940,10 @@ class _GatedFeedForward(torch.autograd.Function):
             outs = _gated_ff_bwd(g, x, wv, wg, b, scales, l_max, activation, need)
         return (*outs[:3], None, None, None, *outs[3:])
 
+    @staticmethod
+    def jvp(ctx, *tangents):
+        raise NotImplementedError("gated_feed_forward has no forward-mode derivative")
+
 
 def gated_feed_forward(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor, gate_bias: Optional[Tensor],
                        scales: Tensor, l_max: int, activation: str) -> Tensor:
@@ -1924,7 +1958,7 @@ def gated_feed_forward(x: Tensor, value_weights: Sequence[Tensor], gate_weight: 
     float64 rows, and constant. float32 products are 3xTF32 on the tensor cores. The backward
     recomputes the products from ``x``; weight gradients do not depend on timing. A backward
     that builds a graph (force training) runs as a composition of twice-differentiable maps."""
-    if torch.compiler.is_compiling():
+    if _recorded():
         return torch.ops.flashcart.gated_ff_fwd(x, list(value_weights), gate_weight, gate_bias, scales, int(l_max),
                                                 activation)
     if _grad_needed(x, gate_weight, gate_bias, *value_weights):

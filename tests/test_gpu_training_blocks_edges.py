@@ -79,3 +79,49 @@ def test_gated_gradient_hooks_run_once(cuda_device, graph):
     xs, w0, w1, gate, bias = _leaves(x, *wv, wg, b)
     w0.register_hook(lambda v: pytest.fail("the weight's gradient was not asked for"))
     torch.autograd.grad(ops.gated_feed_forward(xs, [w0, w1], gate, bias, sc, 1, "sigmoid"), xs, g, create_graph=graph)
+
+
+def test_forward_mode(cuda_device):
+    """Tangents of the linear operators (also where nothing needs a gradient); the gated block,
+    which has none, says so."""
+    fw = torch.autograd.forward_ad
+    gen = torch.Generator().manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=gen, dtype=F64).cuda()
+    idx = torch.tensor([0, 4, 4, 1], device="cuda")
+    rng = torch.tensor([4, 4], device="cuda")
+    table, t_table, x, t_x = r(5, 3), r(5, 3), r(3, 9 * 5), r(3, 9 * 5)
+    for grad in (False, True):
+        with fw.dual_level():
+            dual = lambda t, v: fw.make_dual(t.clone().requires_grad_(grad), v)
+            y = fw.unpack_dual(ops.embedding(dual(table, t_table), idx, 0.7, 1.0))
+            assert torch.equal(y.primal.detach(), ops.embedding(table, idx, 0.7, 1.0))
+            assert torch.equal(y.tangent, ops.embedding(t_table, idx, 0.7))
+            y = fw.unpack_dual(ops.irreps_dropout(dual(x, t_x), rng, 0.4, 2))
+            assert torch.equal(y.tangent, ops.irreps_dropout(t_x, rng, 0.4, 2))
+            gx, wv, wg, b, sc, _ = R.gated_inputs(3, 1, 4, 4, True, F64, "cuda")
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.gated_feed_forward(dual(gx, gx), wv, wg, b, sc, 1, "silu")
+            ops.gated_feed_forward(gx, wv, wg, b, sc, 1, "silu")  # nothing to carry: as ever
+    t = table.clone().requires_grad_(True)
+    assert torch.autograd.gradcheck(lambda w: ops.embedding(w, idx, 0.7, 1.0), (t,), check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(lambda w: ops.embedding(w, idx, 0.7, 1.0) ** 2, (t,), check_fwd_over_rev=True)
+    t = x.clone().requires_grad_(True)
+    assert torch.autograd.gradcheck(lambda v: ops.irreps_dropout(v, rng, 0.4, 2), (t,), check_forward_ad=True)
+
+
+def test_calls_are_recorded(cuda_device):
+    """Traced programs hold the operators, not what a call past the dispatcher leaves behind."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x, wv, wg, b, sc, _ = R.gated_inputs(6, 0, 8, 8, True, F32, "cuda")
+    rng = torch.tensor([1, 2], device="cuda")
+    idx = torch.arange(6, device="cuda") % 3
+
+    def f(x, w, table):
+        y = ops.gated_feed_forward(x + ops.embedding(table, idx), [w], wg, b, sc, 0, "silu")
+        return ops.irreps_dropout(y, rng, 0.5)
+
+    table = torch.randn(3, 8, device="cuda")
+    other = (x * 2, wv[0] - 1, table + 1)
+    for traced in (make_fx(f)(x, wv[0], table), torch.jit.trace(f, (x, wv[0], table), check_trace=False)):
+        assert torch.equal(traced(*other), f(*other))
