@@ -2047,7 +2047,7 @@ def _(x, value_weights, gate_weight, gate_bias, scales, l_max, activation):
 def gated_ff_bwd(grad_y: Tensor, x: Tensor, value_weights: List[Tensor], gate_weight: Tensor,
                  gate_bias: Optional[Tensor], scales: Tensor, l_max: int,
                  activation: str) -> Tuple[Tensor, Tensor, Tensor, List[Tensor]]:
-    """First-order gradients (x, gate_weight, gate_bias or an empty tensor, value_weights)."""
+    """Gradients (x, gate_weight, gate_bias or an empty tensor, value_weights)."""
     gx, gwg, gb, *gwv = _gated_ff_bwd(grad_y, x, value_weights, gate_weight, gate_bias, scales, l_max, activation,
                                       [True] * (3 + len(value_weights)))
     return gx, gwg, x.new_empty((0,)) if gb is None else gb, gwv
@@ -2072,4 +2072,28 @@ def _gated_backward(ctx, g):
     return gx, gwv, gwg, None if b is None else gb, None, None, None
 
 
+def _gated_bwd_setup(ctx, inputs, output):
+    g, x, wv, wg, b, scales, l_max, activation = inputs
+    ctx.save_for_backward(g, x, wg, b, scales, *wv)
+    ctx.args = (l_max, activation)
+
+
+def _gated_bwd_backward(ctx, vx, vwg, vb, vwv):
+    g, x, wg, b, scales, *wv = ctx.saved_tensors
+    outer = torch.is_grad_enabled()
+    with torch.enable_grad():
+        # views (see _gated_composed_grads); what needs no gradient outside needs one in here
+        g, x, wg, b, *wv = (None if t is None else t.view_as(t) if t.requires_grad and outer
+                            else t.detach().requires_grad_(True) for t in (g, x, wg, b, *wv))
+        need = [True, True, b is not None] + [True] * len(wv)
+        outs = _gated_composed_grads(g, x, wv, wg, b, scales, *ctx.args, need)
+        asked = [(o, v) for o, v in zip(outs, (vx, vwg, vb, *vwv)) if o is not None and v is not None]
+        ins = [t for t in (g, x, wg, b, *wv) if t is not None]
+        got = iter(torch.autograd.grad([o for o, _ in asked], ins, [v for _, v in asked], create_graph=outer,
+                                       allow_unused=True))
+    g, x, wg, b, *wv = (None if t is None else next(got) for t in (g, x, wg, b, *wv))
+    return g, x, wv, wg, b, None, None, None
+
+
 gated_ff_fwd.register_autograd(_gated_backward, setup_context=_gated_setup)
+gated_ff_bwd.register_autograd(_gated_bwd_backward, setup_context=_gated_bwd_setup)

@@ -125,3 +125,20 @@ def test_calls_are_recorded(cuda_device):
     other = (x * 2, wv[0] - 1, table + 1)
     for traced in (make_fx(f)(x, wv[0], table), torch.jit.trace(f, (x, wv[0], table), check_trace=False)):
         assert torch.equal(traced(*other), f(*other))
+
+
+@pytest.mark.parametrize("l_max,act,bias", [(0, "silu", False), (1, "sigmoid", True)])
+def test_registered_gated_operator_twice(cuda_device, l_max, act, bias):
+    """The registered operator's second derivative: differences, and the entry point's."""
+    x, wv, wg, b, sc, g = R.gated_inputs(3, l_max, 3, 2, bias, F64, "cuda")
+    ins = [t.requires_grad_(True) for t in (x, wg, *([b] if bias else []), *wv)]
+    n = 3 if bias else 2
+    f = lambda op: lambda x, wg, *rest: op(x, list(rest[n - 2:]), wg, rest[0] if bias else None, sc, l_max, act)
+    registered = f(torch.ops.flashcart.gated_ff_fwd)
+    assert torch.autograd.gradgradcheck(registered, ins)
+    second = []
+    for call in (registered, f(ops.gated_feed_forward)):
+        (gx,) = torch.autograd.grad(call(*ins), x, g, create_graph=True)
+        second.append(torch.autograd.grad(gx.square().sum(), ins))
+    for a, c in zip(*second):
+        assert ((a - c).norm() / c.norm()).item() <= 1e-13  # some hundred roundings of 2^-53
