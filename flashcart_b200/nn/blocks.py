@@ -44,23 +44,37 @@ class ScaledEmbedding(nn.Module):
 
 class IrrepsDropout(_NoSpecialParameters, nn.Module):
     """Dropout of whole irreps: one decision per (row, rank, channel), shared by the rank's
-    components, so the layer commutes with rotations. Every training call takes the next
-    offset of the seed's stream (device buffer ``rng`` = (seed, offset)); identity in
-    evaluation."""
+    components, so the layer commutes with rotations; identity in evaluation.
 
-    def __init__(self, p: float, l_max: int = 0, seed: int = 0):
+    Without a seed every training call draws the mask's 128 bits from torch's generator of the
+    device, as ``nn.Dropout`` does: ``torch.manual_seed`` decides (ranks seeded apart drop
+    apart), a restored generator state resumes the masks, and activation checkpointing, which
+    restores it too, recomputes the same ones. With a seed the layer has a stream of its own,
+    the device buffer ``rng`` = (key, calls so far), which is not part of the state dict; such
+    a layer cannot tell which call a recomputation stands for and refuses to be recomputed."""
+
+    def __init__(self, p: float, l_max: int = 0, seed: Optional[int] = None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"p must lie in [0, 1]. Provided: {p}.")
         self.p, self.l_max = float(p), int(l_max)
-        self.register_buffer("rng", torch.tensor([int(seed), 0], dtype=torch.int64), persistent=False)
-        self.register_buffer("advance", torch.tensor([0, 1], dtype=torch.int64), persistent=False)
+        own = lambda *v: None if seed is None else torch.tensor(v, dtype=torch.int64)
+        self.register_buffer("rng", own(0 if seed is None else int(seed), 0), persistent=False)
+        self.register_buffer("advance", own(0, 1), persistent=False)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if not self.training or self.p == 0.0:
             return x
-        state = self.rng.clone()  # the gradient regenerates the mask from these two numbers
-        self.rng.add_(self.advance)
+        # the gradient regenerates the mask from these two numbers
+        if self.rng is None:
+            state = torch.empty(2, dtype=torch.int64, device=x.device).random_()
+        else:
+            if not torch.compiler.is_compiling() and torch._C._current_graph_task_id() != -1:
+                raise RuntimeError("IrrepsDropout with a seed of its own was called inside a backward (activation "
+                                   "checkpointing?), where it would draw another mask than the forward did; leave "
+                                   "the seed out to use torch's generator")
+            state = self.rng.clone()
+            self.rng.add_(self.advance)
         return ops.irreps_dropout(x, state, self.p, self.l_max)
 
     def extra_repr(self) -> str:
@@ -74,7 +88,7 @@ class GatedFeedForward(EquivariantGatedLayer):
 
     def __init__(self, l_max: int, in_features: int, hidden_features: Optional[int] = None,
                  gate_activation: str = "silu", gate_bias: bool = True, use_triton: bool = False,
-                 dropout: float = 0.0, seed: int = 0):
+                 dropout: float = 0.0, seed: Optional[int] = None):
         super().__init__(l_max, in_features, hidden_features, gate_activation, gate_bias, use_triton)
         self.dropout = IrrepsDropout(dropout, l_max, seed)
         self.register_buffer("scales", torch.cat([self.value_linear.scale.reshape(-1),
@@ -82,7 +96,8 @@ class GatedFeedForward(EquivariantGatedLayer):
                                                   self.gate_activation.scale.reshape(1)]), persistent=False)
 
     @classmethod
-    def from_layer(cls, layer: EquivariantGatedLayer, dropout: float = 0.0, seed: int = 0) -> "GatedFeedForward":
+    def from_layer(cls, layer: EquivariantGatedLayer, dropout: float = 0.0,
+                   seed: Optional[int] = None) -> "GatedFeedForward":
         """The same parameters (shared, not copied)."""
         with torch.random.fork_rng(devices=[]):  # the initial weights drawn here are thrown away
             new = cls(layer.l_max, layer.in_features, layer.hidden_features, layer.gate_activation_name,
@@ -117,12 +132,13 @@ class _FusedPathWeights(ProductPathWeights):
         return ops.embedding(self.delta.weight, atom_types, 1.0, 1.0)
 
 
-def use_training_blocks(model: nn.Module, dropout: float = 0.0, seed: int = 0) -> nn.Module:
+def use_training_blocks(model: nn.Module, dropout: float = 0.0, seed: Optional[int] = None) -> nn.Module:
     """Put the training blocks into a :class:`~flashcart_b200.model.flashcart.FlashCartPotential`
     (in place; returned for convenience): the element embeddings, the element-dependent path
     weights and the gated layers. Parameters, their names and the model's results stay the
     same, up to rounding; ``dropout`` > 0 drops hidden irreps of the gated layers in training
-    mode (each layer has its own stream of ``seed``)."""
+    mode, from torch's generator or, with a ``seed``, from a stream of each layer (see
+    :class:`IrrepsDropout`; give every rank of a data-parallel run a seed of its own)."""
     if isinstance(model.embedding, nn.Embedding):
         model.embedding = ScaledEmbedding.from_embedding(model.embedding)
     for inter in model.interactions:
@@ -135,5 +151,6 @@ def use_training_blocks(model: nn.Module, dropout: float = 0.0, seed: int = 0) -
                 weights.__class__ = _FusedPathWeights  # same attributes, another lookup
     if model.nonlinearity:
         for k, layer in enumerate(model.nonlinearities):
-            model.nonlinearities[k] = GatedFeedForward.from_layer(layer, dropout, seed + k)
+            model.nonlinearities[k] = GatedFeedForward.from_layer(layer, dropout,
+                                                                   None if seed is None else seed + k)
     return model

@@ -6,6 +6,7 @@ import torch
 
 import block_refs as R
 from flashcart_b200 import ops
+from flashcart_b200.nn.blocks import IrrepsDropout
 
 pytestmark = pytest.mark.gpu
 
@@ -142,3 +143,52 @@ def test_registered_gated_operator_twice(cuda_device, l_max, act, bias):
         second.append(torch.autograd.grad(gx.square().sum(), ins))
     for a, c in zip(*second):
         assert ((a - c).norm() / c.norm()).item() <= 1e-13  # some hundred roundings of 2^-53
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_dropout_under_checkpointing(cuda_device, reentrant):
+    """A recomputed forward has the mask that the loss had; a layer with a stream of its own,
+    which cannot know it, refuses."""
+    from torch.utils.checkpoint import checkpoint
+
+    layer = IrrepsDropout(0.5, l_max=1).train()
+    x = torch.randn(200, 4 * 8, device="cuda", requires_grad=True)
+    for _ in range(2):  # the second call's recomputation is not the first's mask
+        y = checkpoint(lambda t: layer(t) * 1.0, x, use_reentrant=reentrant)
+        want = y.detach() / x.detach()
+        x.grad = None
+        y.sum().backward()
+        assert torch.allclose(x.grad, want, rtol=1e-6, atol=0)
+        assert set(want.round().unique().tolist()) == {0.0, 2.0}
+    own = IrrepsDropout(0.5, l_max=1, seed=3).cuda().train()
+    y = checkpoint(lambda t: own(t) * 1.0, x, use_reentrant=reentrant)
+    with pytest.raises(RuntimeError, match="leave the seed out"):
+        y.sum().backward()
+
+
+def test_dropout_follows_torch_generator(cuda_device):
+    layer = IrrepsDropout(0.5).train()
+    x = torch.ones(100, 16, device="cuda")
+    torch.manual_seed(1)
+    a, state, b = layer(x), torch.cuda.get_rng_state(), layer(x)
+    assert not torch.equal(a, b)
+    torch.cuda.set_rng_state(state)
+    assert torch.equal(layer(x), b)
+    torch.manual_seed(1)
+    assert torch.equal(layer(x), a)
+    torch.manual_seed(2)
+    assert not torch.equal(layer(x), a)
+    assert not list(layer.state_dict()) and IrrepsDropout(0.5).cuda().eval()(x) is x
+    # a captured step draws on with every replay
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        layer(x)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        y = layer(x)
+    graph.replay()
+    first = y.clone()
+    graph.replay()
+    assert not torch.equal(first, y)
