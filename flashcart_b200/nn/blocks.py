@@ -132,6 +132,15 @@ class _FusedPathWeights(ProductPathWeights):
         return ops.embedding(self.delta.weight, atom_types, 1.0, 1.0)
 
 
+def _layer_seed(seed: Optional[int], layer: int) -> Optional[int]:
+    """A key of its own for every layer of every seed: the seeds' first keys lie far apart (seed
+    times an odd number near 2^64 / 1.618, modulo 2^64), as signed 64-bit integers."""
+    if seed is None:
+        return None
+    key = (int(seed) * 0x9E3779B97F4A7C15 + layer) % 2 ** 64
+    return key - 2 ** 64 if key >= 2 ** 63 else key
+
+
 def use_training_blocks(model: nn.Module, dropout: float = 0.0, seed: Optional[int] = None) -> nn.Module:
     """Put the training blocks into a :class:`~flashcart_b200.model.flashcart.FlashCartPotential`
     (in place; returned for convenience): the element embeddings, the element-dependent path
@@ -151,6 +160,5 @@ def use_training_blocks(model: nn.Module, dropout: float = 0.0, seed: Optional[i
                 weights.__class__ = _FusedPathWeights  # same attributes, another lookup
     if model.nonlinearity:
         for k, layer in enumerate(model.nonlinearities):
-            model.nonlinearities[k] = GatedFeedForward.from_layer(layer, dropout,
-                                                                   None if seed is None else seed + k)
+            model.nonlinearities[k] = GatedFeedForward.from_layer(layer, dropout, _layer_seed(seed, k))
     return model

@@ -1,0 +1,27 @@
+"""Training blocks as modules, without a GPU: what they keep of the layers they stand for, and
+what they refuse."""
+
+import copy
+
+import pytest
+import torch
+import torch.nn as nn
+
+from flashcart_b200.model.flashcart import FlashCartPotential
+from flashcart_b200.nn.blocks import IrrepsDropout, use_training_blocks
+
+ARCH = dict(elements=["H", "C"], r_max=4.0, n_hidden_feats=8, l_max_hidden_feats=1, l_max_edge_attrs=1, n_radial=4,
+            n_interactions=3, correlation=2, layer_norm=True, nonlinearity=True, avg_neighbors=12.0,
+            element_agnostic_interaction=False, element_agnostic_product=False, n_element_interaction_features=4)
+
+
+def test_dropout_streams_of_layers_and_seeds():
+    """No layer of one seed shares its stream with another layer, of this seed or of another."""
+    stock = FlashCartPotential(**ARCH)
+    keys = []
+    for seed in (0, 1, 2, 3, -1, 10 ** 6, 2 ** 63 - 1):
+        model = use_training_blocks(copy.deepcopy(stock), dropout=0.1, seed=seed)
+        layers = [m for m in model.modules() if isinstance(m, IrrepsDropout)]
+        assert len(layers) > 1
+        keys += [int(m.rng[0]) for m in layers]
+    assert len(set(keys)) == len(keys)
