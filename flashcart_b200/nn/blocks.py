@@ -31,8 +31,18 @@ class ScaledEmbedding(nn.Module):
         self.weight = nn.Parameter(torch.randn(n_types, features)) if weight is None else weight
 
     @classmethod
+    def stands_for(cls, emb: nn.Module) -> bool:
+        """Whether ``emb`` is a plain table: a padding index, a norm limit, frequency scaling and
+        sparse gradients are not this module's."""
+        return (type(emb) is nn.Embedding and emb.padding_idx is None and emb.max_norm is None
+                and not emb.scale_grad_by_freq and not emb.sparse)
+
+    @classmethod
     def from_embedding(cls, emb: nn.Embedding, scale: float = 1.0, offset: float = 0.0) -> "ScaledEmbedding":
         """The same table (shared, not copied)."""
+        if not cls.stands_for(emb):
+            raise ValueError(f"ScaledEmbedding stands for plain embeddings only (no padding_idx, max_norm, "
+                             f"scale_grad_by_freq or sparse gradients). Provided: {emb}.")
         return cls(emb.num_embeddings, emb.embedding_dim, scale, offset, weight=emb.weight)
 
     def forward(self, index: torch.Tensor) -> torch.Tensor:
@@ -145,18 +155,19 @@ def use_training_blocks(model: nn.Module, dropout: float = 0.0, seed: Optional[i
     """Put the training blocks into a :class:`~flashcart_b200.model.flashcart.FlashCartPotential`
     (in place; returned for convenience): the element embeddings, the element-dependent path
     weights and the gated layers. Parameters, their names and the model's results stay the
-    same, up to rounding; ``dropout`` > 0 drops hidden irreps of the gated layers in training
+    same, up to rounding (embeddings with options that :class:`ScaledEmbedding` does not have stay
+    as they are); ``dropout`` > 0 drops hidden irreps of the gated layers in training
     mode, from torch's generator or, with a ``seed``, from a stream of each layer (see
     :class:`IrrepsDropout`; give every rank of a data-parallel run a seed of its own)."""
-    if isinstance(model.embedding, nn.Embedding):
+    if ScaledEmbedding.stands_for(model.embedding):
         model.embedding = ScaledEmbedding.from_embedding(model.embedding)
     for inter in model.interactions:
-        if isinstance(inter.emb_i, nn.Embedding):
-            inter.emb_i = ScaledEmbedding.from_embedding(inter.emb_i)
-            inter.emb_j = ScaledEmbedding.from_embedding(inter.emb_j)
+        for name in ("emb_i", "emb_j"):
+            if ScaledEmbedding.stands_for(getattr(inter, name)):
+                setattr(inter, name, ScaledEmbedding.from_embedding(getattr(inter, name)))
     for product in model.products:
         for weights in product.path_weights:
-            if weights.element_dependent:
+            if weights.element_dependent and ScaledEmbedding.stands_for(weights.delta):
                 weights.__class__ = _FusedPathWeights  # same attributes, another lookup
     if model.nonlinearity:
         for k, layer in enumerate(model.nonlinearities):

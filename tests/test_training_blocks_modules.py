@@ -8,7 +8,7 @@ import torch
 import torch.nn as nn
 
 from flashcart_b200.model.flashcart import FlashCartPotential
-from flashcart_b200.nn.blocks import IrrepsDropout, use_training_blocks
+from flashcart_b200.nn.blocks import IrrepsDropout, ScaledEmbedding, use_training_blocks
 
 ARCH = dict(elements=["H", "C"], r_max=4.0, n_hidden_feats=8, l_max_hidden_feats=1, l_max_edge_attrs=1, n_radial=4,
             n_interactions=3, correlation=2, layer_norm=True, nonlinearity=True, avg_neighbors=12.0,
@@ -25,3 +25,18 @@ def test_dropout_streams_of_layers_and_seeds():
         assert len(layers) > 1
         keys += [int(m.rng[0]) for m in layers]
     assert len(set(keys)) == len(keys)
+
+
+@pytest.mark.parametrize("options", [dict(padding_idx=0), dict(max_norm=1.0), dict(scale_grad_by_freq=True),
+                                     dict(sparse=True)])
+def test_embeddings_with_options_are_not_replaced(options):
+    emb = nn.Embedding(2, 8, **options)
+    with pytest.raises(ValueError, match="plain embeddings"):
+        ScaledEmbedding.from_embedding(emb)
+    model = FlashCartPotential(**ARCH)
+    model.embedding, model.interactions[0].emb_j = emb, nn.Embedding(2, 4, **options)
+    blocks = use_training_blocks(model)
+    assert blocks.embedding is emb and type(blocks.interactions[0].emb_j) is nn.Embedding
+    assert type(blocks.interactions[0].emb_i) is ScaledEmbedding
+    plain = nn.Embedding(2, 8)
+    assert ScaledEmbedding.from_embedding(plain).weight is plain.weight
