@@ -20,6 +20,7 @@
 //
 // An index outside [0, n_types) raises FC_DEV_BAD_INDEX; its output row is written as zeros
 // and its gradient row is ignored (it sorts behind every token as key n_types).
+#include <atomic>
 #include <cstring>
 
 #include "fc_vec.cuh"
@@ -416,6 +417,9 @@ __global__ void __launch_bounds__(SORT_THREADS)
     }
 }
 
+// Bytes of sort_small's dynamic shared memory: two buffers of keys and of rows, the warps' counters.
+static constexpr int small_bytes(int R) { return (4 * ((R + 31) & ~31) + (SMALL_THREADS / 32) * 256) * 4; }
+
 // The whole sort of up to SMALL_ROWS tokens in one block: the same three steps a pass, with
 // keys and rows ping-ponged in shared memory (one launch where latency is all that counts).
 __global__ void __launch_bounds__(SMALL_THREADS) sort_small(const int64_t* __restrict__ idx, int R, int64_t V,
@@ -750,6 +754,20 @@ struct EmbedWs {
   int64_t keys[2], order[2], hist, totals, start, partial, sums, bytes;
 };
 
+// The largest sort's shared memory is allowed once per device: the limit is the kernel's, not the
+// call's, and other host threads launch it with other sizes.
+static bool sort_small_ready() {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (done[dev].load(std::memory_order_acquire)) return true;
+  if (cudaFuncSetAttribute(sort_small, cudaFuncAttributeMaxDynamicSharedMemorySize, small_bytes(SMALL_ROWS)) !=
+      cudaSuccess)
+    return false;
+  done[dev].store(true, std::memory_order_release);
+  return true;
+}
+
 // Blocks that share a token's chunks: several where the types alone would leave SMs idle, but
 // at least 64 chunks each.
 static int combine_slices(int64_t V, const SumPlan& sp) {
@@ -815,11 +833,8 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
   A* partial = (A*)(p + w.partial);
   int at = 0;  // which of the pair holds the sorted tokens
   if (R > 0 && R <= SMALL_ROWS) {
-    const int cap = ((int)R + 31) & ~31;
-    const int bytes = (4 * cap + (SMALL_THREADS / 32) * 256) * 4;
-    if (cudaFuncSetAttribute(sort_small, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-      return FC_ERR_LAUNCH;
-    sort_small<<<1, SMALL_THREADS, bytes, s>>>(idx, (int)R, V, so.passes, so.bits, keys[0], order[0], start, status);
+    if (!sort_small_ready()) return FC_ERR_LAUNCH;
+    sort_small<<<1, SMALL_THREADS, small_bytes((int)R), s>>>(idx, (int)R, V, so.passes, so.bits, keys[0], order[0], start, status);
   } else if (R > 0) {
     const unsigned tiles = (unsigned)((R + SORT_TILE - 1) / SORT_TILE);
     for (int pass = 0; pass < so.passes; ++pass) {

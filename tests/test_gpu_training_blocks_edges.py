@@ -1,6 +1,8 @@
 """Training-block operators on the GPU where a rule of their launches ends: empty tables, the
 largest rows and widths, several host threads, sizes whose races or rounding small ones hide."""
 
+import threading
+
 import pytest
 import torch
 
@@ -192,3 +194,27 @@ def test_dropout_follows_torch_generator(cuda_device):
     first = y.clone()
     graph.replay()
     assert not torch.equal(first, y)
+
+
+def test_embedding_gradients_from_several_threads(cuda_device):
+    """Host threads whose calls need different shared memory of the one-block sort."""
+    errors = []
+
+    def work(rows):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                idx = torch.arange(rows, device="cuda") % 5
+                grad = torch.ones(rows, 4, device="cuda")
+                want = torch.bincount(idx, minlength=5).float()[:, None].expand(5, 4)
+                for _ in range(300):
+                    got = torch.ops.flashcart.embedding_bwd(grad, idx, 5, 1.0)
+                assert torch.equal(got, want)
+        except Exception as e:  # told to the main thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(rows,)) for rows in (8192, 7, 8000, 64, 6000, 900)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
