@@ -20,6 +20,7 @@
 //
 // An index outside [0, n_types) raises FC_DEV_BAD_INDEX; its output row is written as zeros
 // and its gradient row is ignored (it sorts behind every token as key n_types).
+#include <algorithm>
 #include <atomic>
 #include <cstring>
 
@@ -691,46 +692,50 @@ __global__ void __launch_bounds__(THREADS)
   }
   __syncthreads();
   const int n = count, lane = threadIdx.x & (lanes - 1), g = threadIdx.x / lanes, groups = THREADS / lanes;
-  const int64_t col = ((int64_t)blockIdx.y * lanes + lane) * PC;
-  for (int e = 0; e < n; ++e) {
-    const int64_t v = list[e][0];
-    const int cf = list[e][1], cl = list[e][2];
-    if (cl < 0) {
-      if (blockIdx.y == 0 && blockIdx.z == 0)
-        zero_row<T>(d_table + v * D, D, vec, threadIdx.x, THREADS);
-      continue;
-    }
-    const int len = cl - cf + 1, c0 = cf + (int)((int64_t)len * blockIdx.z / slices),
-              c1 = cf + (int)((int64_t)len * (blockIdx.z + 1) / slices);
-    A acc[PC];
-#pragma unroll
-    for (int k = 0; k < PC; ++k) acc[k] = A(0);
-    if (col < Dp) {
-#pragma unroll 8
-      for (int c = c0 + g; c < c1; c += groups) {
-        Pack<A, PC> q;
-        q.load(partial + ((int64_t)c * 2 + (c == cf ? 1 : 0)) * Dp + col);
-#pragma unroll
-        for (int k = 0; k < PC; ++k) acc[k] += q.at(k);
+  const int64_t col_tiles = (Dp + (int64_t)lanes * PC - 1) / ((int64_t)lanes * PC);
+  // (64-bit rows may have more tiles than a grid is high)
+  for (int64_t tile = blockIdx.y; tile < col_tiles; tile += gridDim.y) {
+    const int64_t col = (tile * lanes + lane) * PC;
+    for (int e = 0; e < n; ++e) {
+      const int64_t v = list[e][0];
+      const int cf = list[e][1], cl = list[e][2];
+      if (cl < 0) {
+        if (tile == 0 && blockIdx.z == 0)
+          zero_row<T>(d_table + v * D, D, vec, threadIdx.x, THREADS);
+        continue;
       }
-    }
+      const int len = cl - cf + 1, c0 = cf + (int)((int64_t)len * blockIdx.z / slices),
+                c1 = cf + (int)((int64_t)len * (blockIdx.z + 1) / slices);
+      A acc[PC];
 #pragma unroll
-    for (int k = 0; k < PC; ++k) red[threadIdx.x][k] = acc[k];
-    for (int half = groups / 2; half > 0; half >>= 1) {
-      __syncthreads();
-      if (g < half)
+      for (int k = 0; k < PC; ++k) acc[k] = A(0);
+      if (col < Dp) {
+#pragma unroll 8
+        for (int c = c0 + g; c < c1; c += groups) {
+          Pack<A, PC> q;
+          q.load(partial + ((int64_t)c * 2 + (c == cf ? 1 : 0)) * Dp + col);
 #pragma unroll
-        for (int k = 0; k < PC; ++k) red[threadIdx.x][k] += red[threadIdx.x + half * lanes][k];
-    }
-    __syncthreads();
-    if (g == 0)
-#pragma unroll
-      for (int k = 0; k < PC; ++k)
-        if (col + k < D) {
-          if (slices > 1) sums[(v * slices + blockIdx.z) * Dp + col + k] = red[threadIdx.x][k];
-          else d_table[v * D + col + k] = Io<T>::put(scale * red[threadIdx.x][k]);
+          for (int k = 0; k < PC; ++k) acc[k] += q.at(k);
         }
-    __syncthreads();
+      }
+#pragma unroll
+      for (int k = 0; k < PC; ++k) red[threadIdx.x][k] = acc[k];
+      for (int half = groups / 2; half > 0; half >>= 1) {
+        __syncthreads();
+        if (g < half)
+#pragma unroll
+          for (int k = 0; k < PC; ++k) red[threadIdx.x][k] += red[threadIdx.x + half * lanes][k];
+      }
+      __syncthreads();
+      if (g == 0)
+#pragma unroll
+        for (int k = 0; k < PC; ++k)
+          if (col + k < D) {
+            if (slices > 1) sums[(v * slices + blockIdx.z) * Dp + col + k] = red[threadIdx.x][k];
+            else d_table[v * D + col + k] = Io<T>::put(scale * red[threadIdx.x][k]);
+          }
+      __syncthreads();
+    }
   }
 }
 
@@ -882,7 +887,8 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
       if (per_block > threads) per_block = threads;
       A* sums = (A*)(p + w.sums);
       const dim3 cgrid((unsigned)((cands + per_block - 1) / per_block),
-                       (unsigned)((sp.Dp + (int64_t)lanes * PC - 1) / ((int64_t)lanes * PC)), (unsigned)slices);
+                       (unsigned)std::min<int64_t>((sp.Dp + (int64_t)lanes * PC - 1) / ((int64_t)lanes * PC), 65535),
+                       (unsigned)slices);
       const auto combine = by_token ? embed_combine<T, 512> : embed_combine<T, 256>;
       combine<<<cgrid, threads, 0, s>>>(partial, keys[at], start, (int)R, V, D, sp.Dp, sp.Lc, sp.chunks, by_token,
                                         (int)per_block, lanes, slices, vec, (A)scale, sums, d_table);

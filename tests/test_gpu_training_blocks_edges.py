@@ -218,3 +218,15 @@ def test_embedding_gradients_from_several_threads(cuda_device):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+@pytest.mark.parametrize("dtype", [F32, F64])
+def test_embedding_of_the_widest_rows(cuda_device, dtype):
+    """2^22 features, over several chunks of sorted rows: the joining kernel's column tiles exceed
+    what a launch takes in 64 bits."""
+    rows, dim = 40, 2 ** 22
+    idx = torch.arange(rows, device="cuda") % 2
+    grad = torch.ones(rows, dim, dtype=dtype, device="cuda")
+    grad[:, -1] = 2.0
+    got = torch.ops.flashcart.embedding_bwd(grad, idx, 2, 1.0)
+    assert bool((got[:, :-1] == rows // 2).all()) and bool((got[:, -1] == rows).all())
