@@ -133,41 +133,43 @@ __global__ void __launch_bounds__(256) gated_gemm(const F f, const KF depth, int
   __shared__ A as[GK][GT + 1], bs[GK][GT + 1];
   const int z = blockIdx.z, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
   const int64_t r0 = (int64_t)blockIdx.x * GT;
-  const int c0 = blockIdx.y * GT;
   const int64_t K = depth(z);
-  A acc[4][4];
+  // (the gates of 2^20 channels in four ranks have more column tiles than a grid is high)
+  for (int c0 = blockIdx.y * GT; c0 < N; c0 += gridDim.y * GT) {
+    A acc[4][4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = A(0);
-  for (int64_t k0 = 0; k0 < K; k0 += GK) {
+      for (int j = 0; j < 4; ++j) acc[i][j] = A(0);
+    for (int64_t k0 = 0; k0 < K; k0 += GK) {
 #pragma unroll
-    for (int t = 0; t < GT * GK / 256; ++t) {
-      const int e = threadIdx.x + t * 256, k = e & (GK - 1), o = e >> 4;
-      as[k][o] = (r0 + o < R && k0 + k < K) ? f.lhs(z, r0 + o, k0 + k) : A(0);
-      bs[k][o] = (c0 + o < N && k0 + k < K) ? f.rhs(z, k0 + k, c0 + o) : A(0);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < GK; ++k) {
-      A p[4], q[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[i] = as[k][ty + 16 * i];
-        q[i] = bs[k][tx + 16 * i];
+      for (int t = 0; t < GT * GK / 256; ++t) {
+        const int e = threadIdx.x + t * 256, k = e & (GK - 1), o = e >> 4;
+        as[k][o] = (r0 + o < R && k0 + k < K) ? f.lhs(z, r0 + o, k0 + k) : A(0);
+        bs[k][o] = (c0 + o < N && k0 + k < K) ? f.rhs(z, k0 + k, c0 + o) : A(0);
       }
+      __syncthreads();
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int k = 0; k < GK; ++k) {
+        A p[4], q[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] += p[i] * q[j];
+        for (int i = 0; i < 4; ++i) {
+          p[i] = as[k][ty + 16 * i];
+          q[i] = bs[k][tx + 16 * i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] += p[i] * q[j];
+      }
+      __syncthreads();
     }
-    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (r0 + ty + 16 * i < R && c0 + tx + 16 * j < N) f.put(z, r0 + ty + 16 * i, c0 + tx + 16 * j, acc[i][j]);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (r0 + ty + 16 * i < R && c0 + tx + 16 * j < N) f.put(z, r0 + ty + 16 * i, c0 + tx + 16 * j, acc[i][j]);
 }
 #endif
 
@@ -185,7 +187,7 @@ template <typename A, class F, class KF>
 static int run_gemm(const F& f, const KF& depth, int64_t R, int N, int zs, cudaStream_t s) {
   if (R <= 0 || N <= 0 || zs <= 0) return 0;
 #ifndef FC_HOST_EMU
-  const dim3 grid((unsigned)((R + GT - 1) / GT), (unsigned)((N + GT - 1) / GT), (unsigned)zs);
+  const dim3 grid((unsigned)((R + GT - 1) / GT), (unsigned)std::min((N + GT - 1) / GT, 65535), (unsigned)zs);
   gated_gemm<A><<<grid, 256, 0, s>>>(f, depth, R, N);
   return fc_check_launch();
 #else

@@ -230,3 +230,15 @@ def test_embedding_of_the_widest_rows(cuda_device, dtype):
     grad[:, -1] = 2.0
     got = torch.ops.flashcart.embedding_bwd(grad, idx, 2, 1.0)
     assert bool((got[:, :-1] == rows // 2).all()) and bool((got[:, -1] == rows).all())
+
+
+def test_gated_float64_of_the_widest_gates(cuda_device):
+    """2^20 hidden channels in four ranks: the gates' column tiles exceed what a launch takes."""
+    x, wv, wg, b, sc, g = R.gated_inputs(2, 3, 1, 2 ** 20, False, F64, "cuda")
+    x.requires_grad_(True)
+    y = ops.gated_feed_forward(x, wv, wg, None, sc, 3, "silu")
+    (gx,) = torch.autograd.grad(y, x, g)
+    want_y, (want_x, *_) = R.gated_grads(x, wv, wg, None, sc, 3, "silu", g)
+    # one product a value; sums of 5 x 2^20 terms whose roundings do not add up in one direction
+    assert ((y.detach() - want_y).norm() / want_y.norm()).item() <= 2.0 ** -53 * 32
+    assert ((gx - want_x).norm() / want_x.norm()).item() <= 2.0 ** -53 * 5 * 2 ** 20
