@@ -797,7 +797,8 @@ struct Ws {
 
 static Ws layout(int L, int C, int H, int64_t n, int esize, bool backward, int sms) {
   const int64_t ranks = L + 1, comps = ranks * ranks, per = 16 / esize;
-  const int64_t cp = (C + 3) / 4 * 4, hp = (H + PARTS_PAD - 1) / PARTS_PAD * PARTS_PAD;
+  const int64_t pad = esize == 2 ? PARTS_PAD : 4;  // (float rows have no parts)
+  const int64_t cp = (C + 3) / 4 * 4, hp = (H + pad - 1) / pad * pad;
   const int64_t ce = (C + per - 1) / per * per, he = (H + per - 1) / per * per;
   Ws w{};
   int64_t at = 0;
@@ -816,15 +817,17 @@ static Ws layout(int L, int C, int H, int64_t n, int esize, bool backward, int s
     w.part = take(parts * BM * BM * 4);
     w.bias = take(parts * 2 * BM * 4);
   }
-  // copies with 16-byte rows, used where the caller's rows are not (or are misaligned)
-  w.x = take(n * comps * ce * esize);
-  w.y = take(n * comps * he * esize);  // y, or the output gradient
-  if (backward) w.gx = take(n * comps * ce * esize);
+  // copies in rows of whole 16 bytes, where the caller's are not
+  const bool copy_c = ce != C, copy_h = he != H;
+  if (copy_c) w.x = take(n * comps * ce * esize);
+  if (copy_h) w.y = take(n * comps * he * esize);  // y, or the output gradient
+  if (copy_c && backward) w.gx = take(n * comps * ce * esize);
   w.bytes = at;
   return w;
 }
 
-// A tensor as TMA can address it: itself, or a copy with padded rows.
+// A tensor as TMA can address it: itself (16-byte aligned, the caller's check), or a copy with
+// padded rows.
 template <typename T>
 struct Rows {
   const T* p;
@@ -835,7 +838,7 @@ struct Rows {
 template <typename T>
 static Rows<T> rows_of(const void* p, int width, void* room) {
   constexpr int per = 16 / sizeof(T);
-  if (width % per == 0 && !(reinterpret_cast<uintptr_t>(p) & 15)) return {(const T*)p, width, false};
+  if (width % per == 0) return {(const T*)p, width, false};
   return {(const T*)room, (width + per - 1) / per * per, true};
 }
 

@@ -1835,6 +1835,12 @@ def _gated_args(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor,
     return N.GatedFfDesc(int(l_max), int(c), int(h), _GATE_ACTS[activation], code)
 
 
+def _gated_rows(t: Tensor, width: int) -> Tensor:
+    """Contiguous rows; aligned, where rows of whole 16 bytes are read in place."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 and width * t.element_size() & 15 == 0 else t
+
+
 def _gated_workspace(lib, d: N.GatedFfDesc, n: int, backward: bool, device) -> Tensor:
     nb = lib.fc_gated_ff_workspace_bytes(ctypes.byref(d), n, int(backward))
     if nb < 0:
@@ -1845,7 +1851,7 @@ def _gated_workspace(lib, d: N.GatedFfDesc, n: int, backward: bool, device) -> T
 def _gated_ff_fwd(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor, gate_bias: Optional[Tensor],
                   scales: Tensor, l_max: int, activation: str) -> Tensor:
     d = _gated_args(x, value_weights, gate_weight, gate_bias, scales, l_max, activation)
-    x, wg, sc = x.contiguous(), gate_weight.contiguous(), scales.contiguous()
+    x, wg, sc = _gated_rows(x, d.in_features), gate_weight.contiguous(), scales.contiguous()
     wv = [w.contiguous() for w in value_weights]
     b = None if gate_bias is None else gate_bias.contiguous()
     y = x.new_empty((x.shape[0], (l_max + 1) ** 2 * d.hidden_features))
@@ -1866,7 +1872,8 @@ def _gated_ff_bwd(grad_y: Tensor, x: Tensor, value_weights: Sequence[Tensor], ga
         raise ValueError(f"gated_feed_forward: grad_y must be {(x.shape[0], (l_max + 1) ** 2 * d.hidden_features)} of "
                          f"{x.dtype}, got {tuple(grad_y.shape)} of {grad_y.dtype}")
     _same_device("gated_feed_forward", x, grad_y)
-    g, x, wg, sc = grad_y.contiguous(), x.contiguous(), gate_weight.contiguous(), scales.contiguous()
+    g, x = _gated_rows(grad_y, d.hidden_features), _gated_rows(x, d.in_features)
+    wg, sc = gate_weight.contiguous(), scales.contiguous()
     wv = [w.contiguous() for w in value_weights]
     b = None if gate_bias is None else gate_bias.contiguous()
     ins = [x, wg, b, *wv]

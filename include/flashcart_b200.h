@@ -364,7 +364,10 @@ int fc_irreps_dropout(int32_t l_max, int32_t features, int32_t dtype, const void
  * FC_F32 (3xTF32 tensor-core products), FC_F64 or FC_BF16 (float accumulation and gates, one
  * rounding of y). The backward recomputes the products from x and writes the gradients that
  * are not NULL (grad_value_weights: NULL, or l_max+1 pointers, each of which may be NULL);
- * none depends on timing. workspace: fc_gated_ff_workspace_bytes bytes, 16-byte aligned. */
+ * none depends on timing. workspace: fc_gated_ff_workspace_bytes bytes, 16-byte aligned. x, y,
+ * grad_y and grad_x are read and written in place, and 16-byte aligned, where their channels
+ * are whole 16 bytes (FC_F32: fours, FC_BF16: eights); the workspace holds padded copies of
+ * those whose channels are not. */
 #define FC_GATE_SILU 0
 #define FC_GATE_SIGMOID 1
 typedef struct fc_gated_ff_desc {

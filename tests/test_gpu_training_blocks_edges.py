@@ -1,12 +1,14 @@
 """Training-block operators on the GPU where a rule of their launches ends: empty tables, the
 largest rows and widths, several host threads, sizes whose races or rounding small ones hide."""
 
+import ctypes
 import threading
 
 import pytest
 import torch
 
 import block_refs as R
+from flashcart_b200 import _native as N
 from flashcart_b200 import ops
 from flashcart_b200.nn.blocks import IrrepsDropout
 
@@ -242,3 +244,33 @@ def test_gated_float64_of_the_widest_gates(cuda_device):
     # one product a value; sums of 5 x 2^20 terms whose roundings do not add up in one direction
     assert ((y.detach() - want_y).norm() / want_y.norm()).item() <= 2.0 ** -53 * 32
     assert ((gx - want_x).norm() / want_x.norm()).item() <= 2.0 ** -53 * 5 * 2 ** 20
+
+
+@pytest.mark.parametrize("dtype,code", [(F32, N.FC_F32), (BF16, N.FC_BF16)])
+def test_gated_workspace_holds_what_a_call_needs(cuda_device, dtype, code):
+    """Nothing of the size of x for a forward, and dv and dz for a backward; what padded copies
+    there are, rows that need them have."""
+    n, l_max, c = 27648, 3, 128
+    size = torch.empty(0, dtype=dtype).element_size()
+    query = lambda c, h, back: N.lib().fc_gated_ff_workspace_bytes(
+        ctypes.byref(N.GatedFfDesc(l_max, c, h, N.FC_GATE_SILU, code)), n, back)
+    assert query(c, c, 0) <= 8 * 2 ** 20
+    # (both in float, or two bfloat16 parts) and the partial weight gradients
+    assert query(c, c, 1) <= n * (16 + 4) * c * 4 + 64 * 2 ** 20
+    odd = n * 16 * 33 * size
+    assert query(33, c, 0) >= odd and query(c, 33, 0) >= odd
+    assert query(33, c, 1) >= n * 20 * c * 4 + 2 * odd and query(c, 33, 1) >= n * 20 * 33 * 4 + odd
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c,h", [(32, 32), (33, 32), (32, 33), (7, 9)])
+def test_gated_misaligned_rows(cuda_device, dtype, c, h):
+    """Rows whose memory begins off a 16-byte boundary, with and without whole vectors."""
+    x, wv, wg, b, sc, g = R.gated_inputs(150, 1, c, h, True, dtype, "cuda")
+    off = lambda t: torch.empty(t.numel() + 1, dtype=dtype, device="cuda")[1:].view_as(t).copy_(t)
+    got = []
+    for rows, grad in ((x, g), (off(x), off(g))):
+        ins = [t.detach().requires_grad_(True) for t in (rows, wg, b, *wv)]
+        y = ops.gated_feed_forward(ins[0], ins[3:], ins[1], ins[2], sc, 1, "silu")
+        got.append([y.detach(), *torch.autograd.grad(y, ins, grad)])
+    assert all(torch.equal(p, q) for p, q in zip(*got))
