@@ -221,8 +221,8 @@ __device__ __forceinline__ void put_row(uint8_t* buf, int r, const float* f) {
 
 // sigma(z) by the hardware's base-2 exponential and reciprocal. The exponent -z log2(e) is
 // formed as a float and its remainder, 2^(t + r) = 2^t (1 + r ln 2), so its rounding does not
-// grow with |z|; the power stays finite (the reciprocal of 2^127 is flushed to 0). NaN stays NaN
-// (through r). Every instruction counts: a rank's gates are computed between two passes of the
+// grow with |z|; the power stays finite (the reciprocal of 2^127 is flushed to 0). Where t itself
+// overflows (|z| > 2.36e38) there is no remainder to add. NaN stays NaN (through r). Every instruction counts: a rank's gates are computed between two passes of the
 // tensor cores, with both accumulators taken.
 __device__ __forceinline__ float fast_sigmoid(float z) {
   const float hi = 1.44269502f, lo = 1.92596303e-8f;  // log2(e)
@@ -230,7 +230,7 @@ __device__ __forceinline__ float fast_sigmoid(float z) {
   const float r = fmaf(-z, lo, fmaf(-z, hi, -t));
   float e, s;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(t, 127.f)));
-  e = fabsf(z) == __int_as_float(0x7f800000) ? e : fmaf(e, r * 0.693147181f, e);  // (r is NaN there)
+  e = fabsf(t) == __int_as_float(0x7f800000) ? e : fmaf(e, r * 0.693147181f, e);  // (r is no number there)
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.f + e));
   return s;
 }

@@ -274,3 +274,22 @@ def test_gated_misaligned_rows(cuda_device, dtype, c, h):
         y = ops.gated_feed_forward(ins[0], ins[3:], ins[1], ins[2], sc, 1, "silu")
         got.append([y.detach(), *torch.autograd.grad(y, ins, grad)])
     assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("c", [8, 136, 264])
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+def test_gated_gates_at_the_ends_of_the_type(cuda_device, dtype, c, act):
+    """Pre-activations up to the type's largest value: gates of 0 and 1, finite gradients."""
+    x = torch.ones(4, c, dtype=dtype, device="cuda", requires_grad=True)
+    w = (torch.eye(c, device="cuda") / 4).to(dtype).requires_grad_(True)
+    b = torch.tensor([-3.3e38, -2.5e38, -2.3e38, -1e38, 1e38, 2.3e38, 2.5e38, 3.3e38], device="cuda").to(dtype)
+    bias = b.repeat(c // 8)
+    sc = torch.ones(3, device="cuda")
+    y = ops.gated_feed_forward(x, [w], w, bias, sc, 0, act)
+    z = (bias.double() + 0.25).float().double()
+    want = torch.where(z > 0, torch.ones_like(z) if act == "sigmoid" else z, torch.zeros_like(z)) / 4
+    # the product, the sum with the bias and the gate are one rounding each, then the storage's
+    assert ((y.double() - want).abs() <= (4 * 2.0 ** -24 + (2.0 ** -8 if dtype == BF16 else 0)) * want).all()
+    gx, gw = torch.autograd.grad(y, [x, w], torch.full_like(y, 2.0 ** -20))
+    assert torch.isfinite(gx).all() and torch.isfinite(gw).all()
