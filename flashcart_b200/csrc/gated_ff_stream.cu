@@ -10,6 +10,10 @@
 // hide behind them. PRE computes a gate again for each of its rank's components: 64 gates beside 64
 // sums are what its registers hold.
 //
+// A tensor-core accumulation truncates, so no accumulator runs over more than 64 products (96: PRE
+// above 192 channels): the error does not grow with the channels (float32 gradients of 320 to 16,384
+// channels: 7e-7 to 1e-6; 4e-5 at 16,384 when PRE's three accumulators shared all of them).
+//
 // One persistent CTA per SM, 16 warps:
 //   warp 0       TMA producer, and the CTA's draw from the work list (an atomic counter)
 //   warp 1       MMA issue
@@ -84,7 +88,9 @@ __device__ __forceinline__ Item item_of(const Args& a, int it) {
   return w;
 }
 
-template <int MODE, typename T>
+// LONG (PRE): a component has more units than there are accumulators. A kernel of its own: that loop's
+// registers cost the short reductions 3%.
+template <int MODE, typename T, bool LONG>
 __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_constant__ Maps mp, const Args a) {
   using C = Cfg<MODE, T>;
   constexpr int S = C::STAGES;
@@ -449,19 +455,57 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
                 arrive_tx(ab, 32 * 32 * sizeof(T));
                 tma_load_3d(smem_u32(stage0 + cb * EPI_BUF), &mp.g, col0 + cb * 32, row0, w.k0 + m, ab);
               }
-            for (int j = 0; j < a.nu; ++j)
+            for (int cb = 0; cb < nch; ++cb) {
+              const uint32_t ab = smem_u32(&aux[(warp - 8) * 2 + cb]);
+              const uint32_t par = (aux_phase >> cb) & 1u;
+              aux_phase ^= 1u << cb;
+              if (!wait_warp(ab, par, abort_flag)) {
+                drain_bar(ab, par);  // the copy may still land: let it, before the buffer goes
+                __syncwarp();
+                ok = false;
+              }
+            }
+            // g v is a sum over v's units: they are multiplied and given back a few at a time, as many as
+            // there are accumulators, so that none of them runs longer than a unit (the first few are
+            // what the later ones leave over: those are a full set)
+            auto units16 = [&](int count, int c0, float* v) {  // 16 columns of the units from u on, added
+              tmem_ld<16>(lane_base + (uint32_t)((u % NACC) * BN + c0), v);
+              for (int j = 1; j < count; ++j) {
+                float v2[16];
+                tmem_ld<16>(lane_base + (uint32_t)(((u + j) % NACC) * BN + c0), v2);
+#pragma unroll
+                for (int c = 0; c < 16; ++c) v[c] += v2[c];
+              }
+            };
+            int units = a.nu;
+#pragma unroll 1
+            while (LONG && units > NACC) {
+              const int count = units % NACC ? units % NACC : NACC;
+              for (int j = 0; j < count; ++j)
+                if (!wait_unit(u + j)) ok = false;
+#pragma unroll
+              for (int q = 0; q < 4; ++q)  // 16 of the warp's 64 columns
+                if (q / 2 < nch) {
+                  float v[16];
+                  units16(count, q * 16, v);
+                  const uint8_t* buf = stage0 + q / 2 * EPI_BUF;
+                  constexpr int PER = 16 / sizeof(T);
+#pragma unroll
+                  for (int c = 0; c < 16 / PER; ++c) {
+                    Pack<T, PER> gp;
+                    gp.raw = *reinterpret_cast<const uint4*>(buf + chunk_at<T>(lane, (q % 2) * (16 / PER) + c));
+#pragma unroll
+                    for (int k = 0; k < PER; ++k) sum[q * 16 + c * PER + k] += Io<T>::get(gp.at(k)) * v[c * PER + k];
+                  }
+                }
+              for (int j = 0; j < count; ++j, ++u) free_unit(u);
+              units -= count;
+            }
+            for (int j = 0; j < units; ++j)
               if (!wait_unit(u + j)) ok = false;
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb)
               if (cb < nch) {
-                const uint32_t ab = smem_u32(&aux[(warp - 8) * 2 + cb]);
-                const uint32_t par = (aux_phase >> cb) & 1u;
-                aux_phase ^= 1u << cb;
-                if (!wait_warp(ab, par, abort_flag)) {
-                  drain_bar(ab, par);  // the copy may still land: let it, before the buffer goes
-                  __syncwarp();
-                  ok = false;
-                }
                 uint8_t* buf = stage0 + cb * EPI_BUF;
                 uint4 raw[sizeof(T) == 2 ? 4 : 1];
                 if constexpr (sizeof(T) == 2) {  // rows of g and of dv differ in width: all of g first
@@ -472,13 +516,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                   float v[16];
-                  tmem_ld<16>(lane_base + (uint32_t)((u % NACC) * BN + cb * 32 + h * 16), v);
-                  for (int j = 1; j < a.nu; ++j) {
-                    float v2[16];
-                    tmem_ld<16>(lane_base + (uint32_t)(((u + j) % NACC) * BN + cb * 32 + h * 16), v2);
-#pragma unroll
-                    for (int c = 0; c < 16; ++c) v[c] += v2[c];
-                  }
+                  units16(units, cb * 32 + h * 16, v);
 #pragma unroll
                   for (int c4 = 0; c4 < 4; ++c4) {
                     float4* at = reinterpret_cast<float4*>(buf + chunk_at<float>(lane, h * 4 + c4));
@@ -505,7 +543,7 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
                 }
                 send(&mp.o, buf, col0 + cb * 32, row0, w.k0 + m);
               }
-            for (int j = 0; j < a.nu; ++j, ++u) free_unit(u);
+            for (int j = 0; j < units; ++j, ++u) free_unit(u);
           }
           if (!ok) break;
           if (elect_one()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
@@ -538,10 +576,17 @@ __global__ void __launch_bounds__(THREADS, 1) gated_stream_kernel(const __grid_c
 template <int MODE, typename T>
 int run_stream(const Maps& mp, const Args& args, int sms, cudaStream_t s) {
   constexpr int smem = Cfg<MODE, T>::SMEM;
-  static Ready state;
-  if (int rc = ready(gated_stream_kernel<MODE, T>, smem, state)) return rc;
   const int grid = (int)std::min<int64_t>(args.items, sms);
-  gated_stream_kernel<MODE, T><<<grid, THREADS, smem, s>>>(mp, args);
+  if constexpr (MODE == PRE)
+    if (args.nu > NACC) {
+      static Ready state;
+      if (int rc = ready(gated_stream_kernel<MODE, T, true>, smem, state)) return rc;
+      gated_stream_kernel<MODE, T, true><<<grid, THREADS, smem, s>>>(mp, args);
+      return fc_check_launch();
+    }
+  static Ready state;
+  if (int rc = ready(gated_stream_kernel<MODE, T, false>, smem, state)) return rc;
+  gated_stream_kernel<MODE, T, false><<<grid, THREADS, smem, s>>>(mp, args);
   return fc_check_launch();
 }
 template int run_stream<FWD, float>(const Maps&, const Args&, int, cudaStream_t);

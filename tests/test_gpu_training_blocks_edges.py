@@ -293,3 +293,19 @@ def test_gated_gates_at_the_ends_of_the_type(cuda_device, dtype, c, act):
     assert ((y.double() - want).abs() <= (4 * 2.0 ** -24 + (2.0 ** -8 if dtype == BF16 else 0)) * want).all()
     gx, gw = torch.autograd.grad(y, [x, w], torch.full_like(y, 2.0 ** -20))
     assert torch.isfinite(gx).all() and torch.isfinite(gw).all()
+
+
+@pytest.mark.parametrize("l_max", [0, 1])
+@pytest.mark.parametrize("c", [320, 1024, 4096, 16384])
+def test_gated_error_of_long_reductions(cuda_device, c, l_max):
+    """float32 results from long rows. Two chained products (z and v, then the gradient's), each
+    with three terms of 2^-22 (the parts' rounding, the left-out low x low) and 48 truncating
+    accumulations in a unit of the reduction; the units' additions are rounded, so they grow the
+    error by the square root of their number at most: 2^-24 times 16 for 256 units."""
+    x, wv, wg, b, sc, g = R.gated_inputs(64, l_max, c, 40, True, F32, "cuda", seed=c)
+    ins = [t.requires_grad_(True) for t in (x, wg, b, *wv)]
+    y = ops.gated_feed_forward(x, wv, wg, b, sc, l_max, "silu")
+    want_y, want = R.gated_grads(x, wv, wg, b, sc, l_max, "silu", g)
+    bound = 2 * (3 * 2.0 ** -22 + 48 * 2.0 ** -24 + 16 * 2.0 ** -24)
+    for got, ref in zip((y.detach(), *torch.autograd.grad(y, ins, g)), (want_y, *want)):
+        assert ((got.double() - ref).norm() / ref.norm()).item() <= bound
