@@ -48,7 +48,7 @@ EXPORTED_SYMBOLS = (
     "fc_linear_dbwd", "fc_halo_pack", "fc_halo_unpack", "fc_edge_geometry_fwd", "fc_edge_geometry_bwd",
     "fc_edge_geometry_vec_fwd", "fc_edge_geometry_vec_bwd",
     "fc_embedding_fwd", "fc_embedding_bwd_workspace_bytes", "fc_embedding_bwd", "fc_irreps_dropout",
-    "fc_gated_ff_workspace_bytes", "fc_gated_ff_fwd", "fc_gated_ff_bwd",
+    "fc_block_launches", "fc_gated_ff_workspace_bytes", "fc_gated_ff_fwd", "fc_gated_ff_bwd",
 )
 
 
@@ -180,6 +180,8 @@ def bind(path: str) -> ctypes.CDLL:
     lib.fc_embedding_bwd_workspace_bytes.argtypes = [_I64, _I64, _I64, _I32]
     lib.fc_embedding_bwd.restype = ctypes.c_int
     lib.fc_embedding_bwd.argtypes = [_P, _P, _I64, _I64, _I64, _I32, _F64, _P, _P, _P, _P]
+    lib.fc_block_launches.restype = ctypes.c_int64
+    lib.fc_block_launches.argtypes = []
     lib.fc_irreps_dropout.restype = ctypes.c_int
     lib.fc_irreps_dropout.argtypes = [_I32, _I32, _I32, _P, _P, _F64, _I64, _P, _P]
     lib.fc_gated_ff_workspace_bytes.restype = ctypes.c_int64

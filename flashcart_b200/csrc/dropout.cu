@@ -172,7 +172,7 @@ static int dropout_launch(const T* x, const int64_t* rng, T* y, const DropArgs& 
     dropout_kernel<T, L, VEC, UN, uint32_t><<<grid, 256, 0, s>>>(x, rng, y, a);
   else
     dropout_kernel<T, L, VEC, UN, uint64_t><<<grid, 256, 0, s>>>(x, rng, y, a);
-  return fc_check_launch();
+  return fc_launched(1);
 }
 
 template <typename T>

@@ -251,7 +251,7 @@ int embed_fwd(const void* table_, int64_t V, int64_t D, const int64_t* idx, int6
     else
       embed_fwd_flat<T, 1><<<grid, 256, 0, s>>>(table, V, D, idx, R * D, (A)scale, (A)offset, out, status);
   }
-  return fc_check_launch();
+  return fc_launched(1);
 }
 
 // ------------------------------------------------------------------------------ token sort
@@ -837,9 +837,11 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
   int *hist = (int*)(p + w.hist), *totals = (int*)(p + w.totals), *start = (int*)(p + w.start);
   A* partial = (A*)(p + w.partial);
   int at = 0;  // which of the pair holds the sorted tokens
+  int launches = 0;
   if (R > 0 && R <= SMALL_ROWS) {
     if (!sort_small_ready()) return FC_ERR_LAUNCH;
     sort_small<<<1, SMALL_THREADS, small_bytes((int)R), s>>>(idx, (int)R, V, so.passes, so.bits, keys[0], order[0], start, status);
+    launches = 1;
   } else if (R > 0) {
     const unsigned tiles = (unsigned)((R + SORT_TILE - 1) / SORT_TILE);
     for (int pass = 0; pass < so.passes; ++pass) {
@@ -851,6 +853,7 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
                                                          status);
       // few tiles: every scatter block adds their counts itself (a launch less)
       const int scanned = tiles > 64;
+      launches += 2 + scanned;
       if (scanned) sort_scan<<<so.digits, 256, 0, s>>>(hist, (int)tiles, totals);
       if (pass == 0)
         sort_scatter<true><<<tiles, SORT_THREADS, 0, s>>>(idx, nullptr, nullptr, R, V, shift, so.bits, so.digits, hist,
@@ -861,13 +864,17 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
       at = to;
     }
   }
-  if (fc_check_launch()) return FC_ERR_LAUNCH;
+  if (fc_launched(launches)) return FC_ERR_LAUNCH;
+  launches = 0;
   // with one pass the sort has placed the tokens, and embed_combine writes the empty rows
   const int by_token = V <= sp.chunks;
-  if (R == 0 || so.passes > 1 || !by_token || sp.chunks == 1)
+  if (R == 0 || so.passes > 1 || !by_token || sp.chunks == 1) {
     embed_bounds<T><<<(unsigned)((V + 1 + 255) / 256), 256, 0, s>>>(keys[at], (int)R, V, D, vec, start, d_table);
+    ++launches;
+  }
   if (R > 0) {
     const unsigned grid = (unsigned)((sp.chunks * sp.col_tiles * sp.lanes + 255) / 256);
+    ++launches;
     if (vec)
       embed_sum<T, Io<T>::VEC, true><<<grid, 256, 0, s>>>(grad, keys[at], order[at], start, (int)R, V, D, sp.Lc,
                                                           sp.chunks, sp.lanes, sp.col_tiles, (A)scale, partial, sp.Dp,
@@ -880,6 +887,7 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
       int lanes = 1;
       while (lanes < 32 && (int64_t)lanes * PC < sp.Dp) lanes *= 2;
       const int slices = combine_slices(V, sp);
+      launches += slices > 1 ? 2 : 1;
       const int64_t cands = by_token ? V : sp.chunks;
       int64_t per_block = (cands + 148 * 4 - 1) / (148 * 4);
       // few types: long spans, large blocks; else most spans are a few chunks
@@ -897,7 +905,7 @@ int embed_bwd(const void* grad_, const int64_t* idx, int64_t R, int64_t V, int64
             sums, start, V, D, sp.Dp, sp.Lc, slices, (A)scale, d_table);
     }
   }
-  return fc_check_launch();
+  return fc_launched(launches);
 }
 
 #endif

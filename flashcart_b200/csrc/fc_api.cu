@@ -894,6 +894,8 @@ int fc_halo_unpack(const void* buf, int64_t n_idx, int64_t row_elems, int32_t dt
 
 // ------------------------------------------------------------------ training blocks
 
+int64_t fc_block_launches(void) { return fc_launch_count(); }
+
 static int block_dtype_check(int32_t dtype, const char* what) {
   if (dtype == FC_F32 || dtype == FC_F64 || dtype == FC_BF16) return FC_OK;
   return fail(FC_ERR_INVALID, "%s: dtype must be f32, f64 or bf16", what);

@@ -11,6 +11,19 @@
 
 namespace fc {
 
+// Kernels that this host thread has launched for the training blocks.
+inline int64_t& fc_launch_count() {
+  static thread_local int64_t n = 0;
+  return n;
+}
+#ifndef FC_HOST_EMU
+// Launcher epilogue behind n launches.
+inline int fc_launched(int n) {
+  fc_launch_count() += n;
+  return fc_check_launch();
+}
+#endif
+
 struct bf16_t {
   uint16_t bits;
 };

@@ -189,7 +189,7 @@ static int run_gemm(const F& f, const KF& depth, int64_t R, int N, int zs, cudaS
 #ifndef FC_HOST_EMU
   const dim3 grid((unsigned)((R + GT - 1) / GT), (unsigned)std::min((N + GT - 1) / GT, 65535), (unsigned)zs);
   gated_gemm<A><<<grid, 256, 0, s>>>(f, depth, R, N);
-  return fc_check_launch();
+  return fc_launched(1);
 #else
   (void)s;
   for (int z = 0; z < zs; ++z) {
@@ -268,7 +268,7 @@ static int run_slices(const typename Io<T>::Acc* part, int slices, int64_t count
                       T* out, cudaStream_t s) {
 #ifndef FC_HOST_EMU
   gated_slices_kernel<T><<<(unsigned)((count + 255) / 256), 256, 0, s>>>(part, slices, count, scale, out);
-  return fc_check_launch();
+  return fc_launched(1);
 #else
   (void)s;
   for (int64_t e = 0; e < count; ++e)
@@ -331,7 +331,7 @@ int gated_simple_bwd(const GatedArgs& a, cudaStream_t s) {
   if (total > 0) {
     const int64_t b = (total + 255) / 256;
     gated_pointwise_kernel<T><<<(unsigned)std::min<int64_t>(b, 1 << 20), 256, 0, s>>>(a, v, z, total);
-    if (int rc = fc_check_launch()) return rc;
+    if (int rc = fc_launched(1)) return rc;
   }
 #else
   for (int64_t e = 0; e < total; ++e) gated_pointwise<T>(a, v, z, e);
@@ -364,7 +364,7 @@ int gated_simple_bwd(const GatedArgs& a, cudaStream_t s) {
     if (w.slices_g > 0) {
       gated_bias_kernel<A><<<dim3((unsigned)((width + 255) / 256), (unsigned)w.slices_g), 256, 0, s>>>(z, a.n, width,
                                                                                                         w.slice_g, part);
-      if (int rc = fc_check_launch()) return rc;
+      if (int rc = fc_launched(1)) return rc;
     }
 #else
     for (int t = 0; t < w.slices_g; ++t)

@@ -841,7 +841,7 @@ int run_direct_dx(const Maps& mp, const Args& a, int sms, cudaStream_t s) {
   if (int rc = ready(gated_bf16_dx_kernel, SMEM_MAX, state, 0)) return rc;
   const int lists = (int)std::min<int64_t>(a.items, sms / a.n_ct);
   gated_bf16_dx_kernel<<<lists * a.n_ct, X_THREADS, X_FIXED + 2 * a.nk * X_SLAB, s>>>(mp, a);
-  return fc_check_launch();
+  return fc_launched(1);
 }
 
 template <int MODE>
@@ -852,7 +852,7 @@ int run_direct(const Maps& mp, Args a, int sms, cudaStream_t s) {
   if (int rc = ready(gated_bf16_kernel<MODE>, SMEM_MAX, state, D_REGS)) return rc;
   const int lists = (int)std::min<int64_t>(a.items, sms / a.n_ct);
   gated_bf16_kernel<MODE><<<lists * a.n_ct, D_THREADS, C::smem(a.nk, a.stages), s>>>(mp, a);
-  return fc_check_launch();
+  return fc_launched(1);
 }
 template int run_direct<FWD>(const Maps&, Args, int, cudaStream_t);
 template int run_direct<PRE>(const Maps&, Args, int, cudaStream_t);

@@ -582,12 +582,12 @@ int run_stream(const Maps& mp, const Args& args, int sms, cudaStream_t s) {
       static Ready state;
       if (int rc = ready(gated_stream_kernel<MODE, T, true>, smem, state)) return rc;
       gated_stream_kernel<MODE, T, true><<<grid, THREADS, smem, s>>>(mp, args);
-      return fc_check_launch();
+      return fc_launched(1);
     }
   static Ready state;
   if (int rc = ready(gated_stream_kernel<MODE, T, false>, smem, state)) return rc;
   gated_stream_kernel<MODE, T, false><<<grid, THREADS, smem, s>>>(mp, args);
-  return fc_check_launch();
+  return fc_launched(1);
 }
 template int run_stream<FWD, float>(const Maps&, const Args&, int, cudaStream_t);
 template int run_stream<PRE, float>(const Maps&, const Args&, int, cudaStream_t);

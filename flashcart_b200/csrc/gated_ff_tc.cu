@@ -753,7 +753,7 @@ static int run_resident(const Maps& mp, Args a, int sms, cudaStream_t s) {
   if (int rc = ready(gated_tc_kernel<MODE, T>, SMEM_MAX, state, TC_REGS)) return rc;
   const int lists = (int)std::min<int64_t>(a.items, sms / a.n_ct);
   gated_tc_kernel<MODE, T><<<lists * a.n_ct, TC_THREADS, C::smem(a.nk, a.stages), s>>>(mp, a);
-  return fc_check_launch();
+  return fc_launched(1);
 }
 
 // A column tile has its work list, and every list some CTAs.
@@ -846,7 +846,7 @@ template <typename T>
 static int repitch(const T* src, int64_t src_ld, T* dst, int64_t dst_ld, int width, int64_t rows, cudaStream_t s) {
   const int64_t b = (rows * width + 255) / 256;
   repitch_kernel<T><<<(unsigned)std::min<int64_t>(b, 148 * 32), 256, 0, s>>>(src, src_ld, dst, dst_ld, width, rows);
-  return fc_check_launch();
+  return fc_launched(1);
 }
 
 template <typename T>
@@ -888,7 +888,7 @@ static int run_prep(const GatedArgs& g, void* fwd, void* dx, bool dir, int* coun
   const PrepArgs p{g, dir ? nullptr : (float*)fwd, dir ? nullptr : (float*)dx, dir ? (bf16_t*)fwd : nullptr,
                    dir ? (bf16_t*)dx : nullptr, counters};
   prep_kernel<T><<<dim3((unsigned)std::min<int64_t>((each + 255) / 256, 256), 2 * (g.L + 1)), 256, 0, s>>>(p);
-  return fc_check_launch();
+  return fc_launched(1);
 }
 
 // The maps of x and of the weights that the forward products read.

@@ -739,11 +739,11 @@ int run_wgrad(int ranks, int C, int H, int64_t n, const void* dv, const void* dz
       if (int rc = ready(wgrad_kernel<T>, smem, state, W_REGS)) return rc;
       wgrad_kernel<T><<<wa.ctas, W_THREADS, smem, s>>>(wm, wa);
     }
-    if (int rc = fc_check_launch()) return rc;
+    if (int rc = fc_launched(1)) return rc;
   }
   wgrad_sum_kernel<T><<<(unsigned)(2 * ranks * wa.n_ht * wa.n_ct * (BM / SUM_ROWS)), SUM_ROWS * SUM_PARTS * 32, 0,
                         s>>>(wa, o);
-  return fc_check_launch();
+  return fc_launched(1);
 }
 template int run_wgrad<float>(int, int, int, int64_t, const void*, const void*, int64_t, bool, const float*, int64_t,
                               float*, float*, const WOut&, int*, int, cudaStream_t);

@@ -1620,12 +1620,15 @@ def _launch_on(device: torch.device) -> Tuple[int, int]:
     return st, torch._C._cuda_getCurrentRawStream(idx)
 
 
-def _run(what: str, kernels: int, tensors, device: torch.device, fn, *args) -> None:
+def _run(what: str, tensors, device: torch.device, fn, *args) -> None:
     if _TIMER is None:
         rc = fn(*args)
     else:
-        with _timed(what[3:], kernels, _nbytes(*tensors)):
+        launched = N.lib().fc_block_launches
+        before = launched()
+        with _timed(what[3:], 0, _nbytes(*tensors)):
             rc = fn(*args)
+        _TIMER.launches += launched() - before
     if rc or _DEBUG_CHECK:
         _after(N.lib(), rc, what, device)
 
@@ -1657,7 +1660,7 @@ def _embedding_fwd(table: Tensor, index: Tensor, scale: float, offset: float) ->
     out = t.new_empty(tuple(idx.shape) + (t.shape[1],))
     dev = t.device
     status, stream = _launch_on(dev)
-    _run("fc_embedding_fwd", 1, (t, idx, out), dev, N.lib().fc_embedding_fwd, _addr(t), t.shape[0], t.shape[1], code,
+    _run("fc_embedding_fwd", (t, idx, out), dev, N.lib().fc_embedding_fwd, _addr(t), t.shape[0], t.shape[1], code,
          _addr(idx), idx.numel(), scale, offset, _addr(out), status, stream)
     return out
 
@@ -1677,7 +1680,7 @@ def _embedding_bwd(grad_out: Tensor, index: Tensor, n_types: int, scale: float) 
         N.check(lib, int(nb), "fc_embedding_bwd_workspace_bytes")
     ws = torch.empty(int(nb), dtype=torch.uint8, device=g.device)
     status, stream = _launch_on(g.device)
-    _run("fc_embedding_bwd", 4, (g, idx, out), g.device, lib.fc_embedding_bwd, _addr(g), _addr(idx), idx.numel(),
+    _run("fc_embedding_bwd", (g, idx, out), g.device, lib.fc_embedding_bwd, _addr(g), _addr(idx), idx.numel(),
          int(n_types), d, code, scale, _addr(ws), _addr(out), status, stream)
     return out
 
@@ -1761,7 +1764,7 @@ def _irreps_dropout(x: Tensor, rng: Tensor, p: float, l_max: int) -> Tensor:
     x, rng = x.contiguous(), rng.contiguous()
     y = torch.empty_like(x)
     _, stream = _launch_on(x.device)
-    _run("fc_irreps_dropout", 1, (x, y), x.device, N.lib().fc_irreps_dropout, l_max, features, code, _addr(x),
+    _run("fc_irreps_dropout", (x, y), x.device, N.lib().fc_irreps_dropout, l_max, features, code, _addr(x),
          _addr(rng), p, x.shape[0], _addr(y), stream)
     return y
 
@@ -1858,7 +1861,7 @@ def _gated_ff_fwd(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tenso
     lib = N.lib()
     ws = _gated_workspace(lib, d, x.shape[0], False, x.device)
     status, stream = _launch_on(x.device)
-    _run("fc_gated_ff_fwd", 2, (x, y, wg, b, *wv), x.device, lib.fc_gated_ff_fwd, ctypes.byref(d), _addr(x),
+    _run("fc_gated_ff_fwd", (x, y, wg, b, *wv), x.device, lib.fc_gated_ff_fwd, ctypes.byref(d), _addr(x),
          _ptr_array(wv), _addr(wg), _addr(b), _addr(sc), x.shape[0], _addr(ws), _addr(y), status, stream)
     return y
 
@@ -1885,7 +1888,7 @@ def _gated_ff_bwd(grad_y: Tensor, x: Tensor, value_weights: Sequence[Tensor], ga
     status, stream = _launch_on(x.device)
     # an empty x still has its place: what is null is not wanted
     gx = None if outs[0] is None or x.shape[0] == 0 else _addr(outs[0])
-    _run("fc_gated_ff_bwd", 5, (g, *ins, *outs), x.device, lib.fc_gated_ff_bwd, ctypes.byref(d), _addr(g), _addr(x),
+    _run("fc_gated_ff_bwd", (g, *ins, *outs), x.device, lib.fc_gated_ff_bwd, ctypes.byref(d), _addr(g), _addr(x),
          _ptr_array(wv), _addr(wg), _addr(b), _addr(sc), x.shape[0], _addr(ws), gx, _ptr_array(outs[3:]),
          _addr(outs[1]), _addr(outs[2]), status, stream)
     return outs

@@ -342,6 +342,10 @@ int fc_embedding_bwd(const void* grad_out, const int64_t* idx, int64_t n_rows, i
                      int32_t dtype, double scale, void* workspace, void* grad_table, int32_t* status,
                      fc_stream_t stream);
 
+/* Kernels that the calling thread has launched so far through the training blocks' entry points
+ * (fc_embedding_*, fc_irreps_dropout, fc_gated_ff_*): how many a call takes depends on its sizes. */
+int64_t fc_block_launches(void);
+
 /* ---------------------------------------------------------------- irreps dropout
  * y = x * keep / (1 - p) on rank-block rows (n_rows, (l_max+1)^2 * features), one decision
  * per (row, rank, channel) shared by the rank's components. keep comes from a counter-based

@@ -309,3 +309,46 @@ def test_gated_error_of_long_reductions(cuda_device, c, l_max):
     bound = 2 * (3 * 2.0 ** -22 + 48 * 2.0 ** -24 + 16 * 2.0 ** -24)
     for got, ref in zip((y.detach(), *torch.autograd.grad(y, ins, g)), (want_y, *want)):
         assert ((got.double() - ref).norm() / ref.norm()).item() <= bound
+
+
+def test_kernel_timer_counts_launches(cuda_device):
+    """What the timer counts for a call is what the GPU ran, whatever the sizes."""
+    from torch.profiler import ProfilerActivity, profile
+
+    own = ("embed_", "sort_", "dropout_kernel", "gated_", "wgrad_", "prep_kernel", "repitch_kernel")
+
+    def count(f):
+        timer = ops.KernelTimer()
+        torch.cuda.synchronize()
+        with profile(activities=[ProfilerActivity.CUDA]) as prof:
+            ops.set_kernel_timer(timer)
+            try:
+                f()
+            finally:
+                ops.set_kernel_timer(None)
+            torch.cuda.synchronize()
+        seen = [e for e in prof.events() if e.device_type == torch.autograd.DeviceType.CUDA
+                and any(name in e.name for name in own)]
+        return timer.launches, len(seen)
+
+    def embed(rows, types, dim):
+        idx = torch.arange(rows, device="cuda") % types
+        grad = torch.ones(rows, dim, device="cuda")
+        return lambda: torch.ops.flashcart.embedding_bwd(grad, idx, types, 1.0)
+
+    def gated(n, l_max, c, h, dtype, only_x=False):
+        x, wv, wg, b, sc, g = R.gated_inputs(n, l_max, c, h, True, dtype, "cuda")
+        ins = [t.requires_grad_(True) for t in ((x,) if only_x else (x, wg, b, *wv))]
+        return lambda: torch.autograd.grad(ops.gated_feed_forward(x, wv, wg, b, sc, l_max, "silu"), ins, g)
+
+    x, rng = torch.ones(50, 64, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    calls = [lambda: ops.irreps_dropout(x, rng, 0.5), lambda: ops.embedding(x, rng), embed(10, 2, 8), embed(9000, 3, 8),
+             embed(200_000, 300, 64), embed(200_000, 70_000, 4), embed(200_000, 3, 4), gated(40, 1, 32, 32, F32),
+             gated(40, 1, 33, 31, F32), gated(40, 0, 200, 40, F32, True), gated(40, 1, 32, 32, BF16),
+             gated(40, 0, 300, 33, BF16), gated(40, 1, 5, 7, F64)]
+    for f in calls:
+        f()
+    counts = [count(f) for f in calls]
+    if not any(seen for _, seen in counts):
+        pytest.skip("the profiler records no kernels here")
+    assert all(a == b and a > 0 for a, b in counts), counts
