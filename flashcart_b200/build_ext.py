@@ -16,6 +16,7 @@ import argparse
 import concurrent.futures as cf
 import glob
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -34,6 +35,9 @@ NVCC_FLAGS = [
     "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
     "-DNDEBUG",
 ]
+# Kernels whose warps share out the block's registers (setmaxnreg): their shares are counted on this
+# many per thread, and a launch with another number is refused. So it is checked when they are built.
+SHARED_REGISTERS = {"gated_tc_kernel": 96, "gated_stream_kernel": 128, "gated_bf16_kernel": 96, "wgrad_kernel": 72}
 EMU_FLAGS = ["-x", "c++", "-std=c++17", "-DFC_HOST_EMU", "-O1", "-fPIC"]
 
 
@@ -72,6 +76,21 @@ def _run(cmd: List[str]) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"command failed ({res.returncode}): {' '.join(cmd)}\n{res.stdout}\n{res.stderr}")
+    check_registers(res.stdout + res.stderr)
+
+
+def check_registers(report: str) -> int:
+    """Compare ptxas' report with SHARED_REGISTERS; the number of kernels compared."""
+    found = 0
+    for entry in re.split(r"Compiling entry function ", report)[1:]:
+        name, used = entry.split("'")[1], re.search(r"Used (\d+) registers", entry)
+        for kernel, want in SHARED_REGISTERS.items():
+            if f"{len(kernel)}{kernel}" in name and used:
+                found += 1
+                if int(used.group(1)) != want:
+                    raise RuntimeError(f"{name} uses {used.group(1)} registers per thread; the shares of its warps "
+                                       f"are counted on {want}")
+    return found
 
 
 def generate() -> None:
@@ -101,7 +120,8 @@ def _compile_all(tag: str, compile_cmd, jobs: int) -> List[str]:
 
 def build_cuda(jobs: int = 8) -> str:
     nvcc = _nvcc()
-    objs = _compile_all("cuda", lambda s, o: [nvcc, *NVCC_FLAGS, "-c", s, "-o", o], jobs)
+    report = lambda s: ["-Xptxas", "-v"] if os.path.basename(s).startswith("gated_ff") else []
+    objs = _compile_all("cuda", lambda s, o: [nvcc, *NVCC_FLAGS, *report(s), "-c", s, "-o", o], jobs)
     os.makedirs(LIB_DIR, exist_ok=True)
     if not os.path.exists(CUDA_LIB) or max(os.path.getmtime(o) for o in objs) > os.path.getmtime(CUDA_LIB):
         tmp = CUDA_LIB + ".tmp"

@@ -10,6 +10,7 @@ import torch.nn as nn
 
 from abi_calls import p
 from flashcart_b200 import _native as N
+from flashcart_b200 import build_ext
 from flashcart_b200.model.flashcart import FlashCartPotential
 from flashcart_b200.nn.blocks import IrrepsDropout, ScaledEmbedding, use_training_blocks
 
@@ -61,3 +62,18 @@ def test_gated_rows_in_place_have_to_be_aligned(emu_lib):
     assert call(4, 4, x=off) == (no, no) and b"x must be 16-byte aligned" in emu_lib.fc_last_error()
     assert call(4, 4, y=off) == (no, ok) and call(4, 4, gy=off) == (ok, no) and call(4, 4, gx=off) == (ok, no)
     assert call(3, 3, x=off, y=off, gy=off, gx=off) == (ok, ok)
+
+
+def test_build_checks_shared_registers():
+    line = ("ptxas info    : Compiling entry function '{}' for 'sm_100a'\n"
+            "ptxas info    : Function properties for {}\n    0 bytes stack frame\n"
+            "ptxas info    : Used {} registers, used 2 barriers\n")
+    tc, other = "_ZN2fc3gtc15gated_tc_kernelILi0EfEEvNS0_4MapsENS0_4ArgsE", "_ZN2fc3gtc11prep_kernelIfEEvNS0_8PrepArgsE"
+    assert build_ext.check_registers(line.format(tc, tc, 96) + line.format(other, other, 40)) == 1
+    assert build_ext.check_registers("") == 0
+    for used in (88, 104):
+        with pytest.raises(RuntimeError, match=f"uses {used} registers"):
+            build_ext.check_registers(line.format(other, other, 96) + line.format(tc, tc, used))
+    # every kernel of the table is one of the sources'
+    text = "".join(open(f).read() for f in build_ext.sources() if "gated_ff" in f)
+    assert all(f" {name}(" in text for name in build_ext.SHARED_REGISTERS)
