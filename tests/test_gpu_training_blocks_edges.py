@@ -352,3 +352,29 @@ def test_kernel_timer_counts_launches(cuda_device):
     if not any(seen for _, seen in counts):
         pytest.skip("the profiler records no kernels here")
     assert all(a == b and a > 0 for a, b in counts), counts
+
+
+@pytest.mark.parametrize("dtype,n,l_max,c,h", [(F32, 27648, 3, 128, 128), (BF16, 27648, 3, 128, 128),
+                                               (F32, 9001, 2, 200, 136), (BF16, 100003, 0, 96, 200),
+                                               (F32, 13869, 3, 48, 88), (F32, 27648, 2, 96, 96),
+                                               (F32, 27648, 3, 24, 32), (F32, 27648, 1, 160, 224),
+                                               (F32, 9001, 1, 320, 352), (BF16, 20001, 2, 40, 72),
+                                               (BF16, 9001, 1, 300, 136), (BF16, 20001, 1, 72, 264)])
+def test_gated_large_passes_are_right(cuda_device, dtype, n, l_max, c, h):
+    """The first passes at sizes whose kernels have every role busy, against 64 bits: weights or rows
+    used before they are there, or after they have gone, show here (odd and even numbers of slabs,
+    resident and streamed weights). Errors as in test_gated_error_of_long_reductions; bfloat16
+    results add one rounding to 8 bits, and what is handed between the backward's halves in two
+    bfloat16 parts (2^-17)."""
+    x, wv, wg, _, scales, g = R.gated_inputs(n, l_max, c, h, False, dtype, "cuda", seed=3)
+    ins = [t.requires_grad_(True) for t in (x, wg, *wv)]
+    want_y, want = R.gated_grads(x, wv, wg, None, scales, l_max, "silu", g)
+    want = [want_y, *(t for t in want if t is not None)]
+    bound = 2 * (3 * 2.0 ** -22 + 48 * 2.0 ** -24 + 16 * 2.0 ** -24) + (2.0 ** -8 + 2.0 ** -17 if dtype == BF16 else 0.0)
+    for _ in range(3):
+        y = ops.gated_feed_forward(x, wv, wg, None, scales, l_max, "silu")
+        for got, ref in zip((y.detach(), *torch.autograd.grad(y, ins, g)), want):
+            assert ((got.double() - ref).norm() / ref.norm()).item() <= bound
+            # and no single row off: a few wrong values hide in a norm over 10^8
+            worst = (got.double() - ref).abs().amax() / ref.abs().amax()
+            assert worst.item() <= 16 * bound
