@@ -1915,8 +1915,9 @@ def _gated_composed(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Ten
         z = z + gate_bias.to(acc)
     s = torch.sigmoid(z)
     a = (scales[ranks + 1] * (s if activation == "sigmoid" else z * s)).view(n, ranks, h)
-    of = _expand_index(l_max, x.device)
-    return (v.view(n, ranks * ranks, h) * a.index_select(1, of)).reshape(n, ranks * ranks * h).to(dtype)
+    # (no index tensor: it would come from the host, which a captured step cannot wait for)
+    a = torch.cat([a[:, l:l + 1].expand(n, 2 * l + 1, h) for l in range(ranks)], 1)
+    return (v.view(n, ranks * ranks, h) * a).reshape(n, ranks * ranks * h).to(dtype)
 
 
 def _gated_composed_grads(g: Tensor, x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor,

@@ -378,3 +378,27 @@ def test_gated_large_passes_are_right(cuda_device, dtype, n, l_max, c, h):
             # and no single row off: a few wrong values hide in a norm over 10^8
             worst = (got.double() - ref).abs().amax() / ref.abs().amax()
             assert worst.item() <= 16 * bound
+
+
+def test_gated_force_step_is_captured(cuda_device):
+    """A step with a second derivative in a CUDA graph: the replay's gradients are the eager ones."""
+    x, wv, wg, b, sc, g = R.gated_inputs(40, 2, 16, 24, True, F32, "cuda", seed=8)
+    ins = [t.requires_grad_(True) for t in (x, wg, b, *wv)]
+
+    def step():
+        y = ops.gated_feed_forward(x, wv, wg, b, sc, 2, "silu")
+        (gx,) = torch.autograd.grad(y, x, g, create_graph=True)
+        return torch.autograd.grad(gx.square().sum(), ins)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for t in got:
+        t.zero_()
+    graph.replay()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
