@@ -1599,11 +1599,13 @@ def _grad_needed(*tensors: Optional[Tensor]) -> bool:
             or forward_ad._current_level >= 0)
 
 
+_dispatch_modes, _tracing_state = torch._C._len_torch_dispatch_stack, torch._C._get_tracing_state
+
+
 def _recorded() -> bool:
     """Whether operator calls are compiled, traced, or seen by a dispatch mode (make_fx, fake
     tensors, counters): a call past the dispatcher would be missing there."""
-    return (torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() > 0
-            or torch._C._get_tracing_state() is not None)
+    return torch.compiler.is_compiling() or _dispatch_modes() > 0 or _tracing_state() is not None
 
 
 # The host's share of a call decides small sizes, so these calls pass plain integers and look
@@ -1780,7 +1782,9 @@ class _IrrepsDropout(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         (rng,) = ctx.saved_tensors
-        return irreps_dropout(g, rng, *ctx.args), None, None, None
+        if _grad_needed(g):
+            return _IrrepsDropout.apply(g, rng, *ctx.args), None, None, None
+        return _irreps_dropout(g, rng, *ctx.args), None, None, None
 
     @staticmethod
     def jvp(ctx, x_t, *_):
@@ -1841,7 +1845,9 @@ def _gated_args(x: Tensor, value_weights: Sequence[Tensor], gate_weight: Tensor,
 def _gated_rows(t: Tensor, width: int) -> Tensor:
     """Contiguous rows; aligned, where rows of whole 16 bytes are read in place."""
     t = t.contiguous()
-    return t.clone() if t.data_ptr() & 15 and width * t.element_size() & 15 == 0 else t
+    if t.data_ptr() & 15 and width * t.element_size() & 15 == 0:
+        return t.clone()
+    return t
 
 
 def _gated_workspace(lib, d: N.GatedFfDesc, n: int, backward: bool, device) -> Tensor:
