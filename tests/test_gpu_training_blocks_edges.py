@@ -226,7 +226,7 @@ def test_embedding_gradients_from_several_threads(cuda_device):
 def test_embedding_of_the_widest_rows(cuda_device, dtype):
     """2^22 features, over several chunks of sorted rows: the joining kernel's column tiles exceed
     what a launch takes in 64 bits."""
-    rows, dim = 40, 2 ** 22
+    rows, dim = 264, 2 ** 22  # (chunks are up to 256 rows)
     idx = torch.arange(rows, device="cuda") % 2
     grad = torch.ones(rows, dim, dtype=dtype, device="cuda")
     grad[:, -1] = 2.0
