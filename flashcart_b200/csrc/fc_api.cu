@@ -979,9 +979,10 @@ static int gated_check(const fc_gated_ff_desc* d, int64_t n_rows, const char* wh
 
 // Rows of whole 16 bytes are read and written in place, by copies that want them aligned (other
 // rows are copied, and 64-bit rows go element by element).
-static int gated_rows_check(const void* rows, int32_t width, int32_t dtype, const char* name, const char* what) {
+static int gated_rows_check(const void* rows, int64_t n_rows, int32_t width, int32_t dtype, const char* name,
+                            const char* what) {
   const int size = dtype == FC_BF16 ? 2 : 4;
-  if (dtype != FC_F64 && (int64_t)width * size % 16 == 0 && (reinterpret_cast<uintptr_t>(rows) & 15))
+  if (n_rows > 0 && dtype != FC_F64 && (int64_t)width * size % 16 == 0 && (reinterpret_cast<uintptr_t>(rows) & 15))
     return fail(FC_ERR_INVALID, "%s: %s must be 16-byte aligned", what, name);
   return FC_OK;
 }
@@ -1003,7 +1004,7 @@ static int gated_args(const fc_gated_ff_desc* d, const void* x, const void* cons
     return fail(FC_ERR_INVALID, "%s: null tensor", what);
   if (reinterpret_cast<uintptr_t>(workspace) & 15)
     return fail(FC_ERR_INVALID, "%s: workspace must be 16-byte aligned", what);
-  if (int rc = gated_rows_check(x, d->in_features, d->dtype, "x", what)) return rc;
+  if (int rc = gated_rows_check(x, n_rows, d->in_features, d->dtype, "x", what)) return rc;
   a = GatedArgs{};
   a.L = d->l_max;
   a.C = d->in_features;
@@ -1032,7 +1033,7 @@ int fc_gated_ff_fwd(const fc_gated_ff_desc* desc, const void* x, const void* con
     return rc;
   if (n_rows == 0) return FC_OK;
   if (!y) return fail(FC_ERR_INVALID, "%s: null tensor", what);
-  if (int rc = gated_rows_check(y, desc->hidden_features, desc->dtype, "y", what)) return rc;
+  if (int rc = gated_rows_check(y, n_rows, desc->hidden_features, desc->dtype, "y", what)) return rc;
   a.y = y;
   const auto run = desc->dtype == FC_F32   ? gated_fwd<float>
                    : desc->dtype == FC_F64 ? gated_simple_fwd<double>
@@ -1050,8 +1051,8 @@ int fc_gated_ff_bwd(const fc_gated_ff_desc* desc, const void* grad_y, const void
   if (int rc = gated_args(desc, x, value_weights, gate_weight, gate_bias, scales, n_rows, workspace, status, what, a))
     return rc;
   if (n_rows > 0 && !grad_y) return fail(FC_ERR_INVALID, "%s: null tensor", what);
-  if (int rc = gated_rows_check(grad_y, desc->hidden_features, desc->dtype, "grad_y", what)) return rc;
-  if (int rc = gated_rows_check(grad_x, desc->in_features, desc->dtype, "grad_x", what)) return rc;
+  if (int rc = gated_rows_check(grad_y, n_rows, desc->hidden_features, desc->dtype, "grad_y", what)) return rc;
+  if (int rc = gated_rows_check(grad_x, n_rows, desc->in_features, desc->dtype, "grad_x", what)) return rc;
   a.gy = grad_y;
   a.gx = grad_x;
   for (int l = 0; l <= desc->l_max; ++l) a.gwv[l] = grad_value_weights ? grad_value_weights[l] : nullptr;

@@ -52,15 +52,16 @@ def test_gated_rows_in_place_have_to_be_aligned(emu_lib):
     ws = torch.zeros(2 ** 16, dtype=torch.uint8)
     one = (ctypes.c_void_p * 1)(t.data_ptr())
 
-    def call(c, h, x=p(t), y=p(t), gy=p(t), gx=p(t)):
+    def call(c, h, x=p(t), y=p(t), gy=p(t), gx=p(t), n=1):
         d = ctypes.byref(N.GatedFfDesc(0, c, h, N.FC_GATE_SILU, N.FC_F32))
-        return (emu_lib.fc_gated_ff_fwd(d, x, one, p(t), None, p(t), 1, p(ws), y, None, None),
-                emu_lib.fc_gated_ff_bwd(d, gy, x, one, p(t), None, p(t), 1, p(ws), gx, None, None, None, None, None))
+        return (emu_lib.fc_gated_ff_fwd(d, x, one, p(t), None, p(t), n, p(ws), y, None, None),
+                emu_lib.fc_gated_ff_bwd(d, gy, x, one, p(t), None, p(t), n, p(ws), gx, None, None, None, None, None))
 
     ok, no = N.FC_OK, N.FC_ERR_INVALID
     assert call(4, 4) == (ok, ok)
     assert call(4, 4, x=off) == (no, no) and b"x must be 16-byte aligned" in emu_lib.fc_last_error()
     assert call(4, 4, y=off) == (no, ok) and call(4, 4, gy=off) == (ok, no) and call(4, 4, gx=off) == (ok, no)
+    assert call(4, 4, x=off, y=off, gy=off, gx=off, n=0) == (ok, ok)
     assert call(3, 3, x=off, y=off, gy=off, gx=off) == (ok, ok)
 
 
