@@ -17,8 +17,10 @@
 // What bounds it: DRAM, one read and one write of every element (one 16-byte vector per
 // thread and component). One generator block serves 4 (2l+1) elements. Measured: 27,648 x 16 rows
 // of 128 float32 channels 70 us a pass (6.4 TB/s, the copy rate); 2^26 plain elements 86 us in
-// float32 (6.2 TB/s) and 84 us in bfloat16 (3.2 TB/s), where the generator's 64-bit products are
-// the bound; channel counts that are no fours (99) go element by element, 117 us in float32.
+// float32 (6.2 TB/s) and 84 us in bfloat16 (3.2 TB/s), where instructions are the bound: 122 for four
+// elements, of which the generator's wide products are 20 and its keys' steps 20 (issue slots 71% busy,
+// integer pipe 57%, DRAM 32%); channel counts that are no fours (99) go element by element, 117 us in
+// float32.
 #include "fc_vec.cuh"
 
 namespace fc {

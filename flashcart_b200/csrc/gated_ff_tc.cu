@@ -1,5 +1,5 @@
 // Gated feed-forward block on tcgen05 tensor cores, fed by TMA (sm_100a): float32 rows as
-// 3xTF32 products (bfloat16 rows: gated_ff_bf16.cu, but for the input gradient).
+// 3xTF32 products, and the input gradient of bfloat16 rows that are too long for gated_ff_bf16.cu.
 //
 // Mathematics and row layout: gated_ff.cu. The scales s_l, s_g are folded into the split
 // weights, so the accumulators hold v_k and z_l - b_l themselves.
