@@ -1797,8 +1797,8 @@ def irreps_dropout(x: Tensor, rng: Tensor, p: float, l_max: int = 0) -> Tensor:
     elementwise dropout of plain rows.
 
     ``rng`` holds (seed, offset) as two int64 values on the device: the mask is regenerated
-    from them in the gradient and never stored, so they must not change in between (advance a
-    copy, as :class:`flashcart_b200.nn.blocks.IrrepsDropout` does). ``p = 1`` drops everything;
+    from them in the gradient and never stored, so they must not change in between (give every
+    call a tensor of its own, as :class:`flashcart_b200.nn.blocks.IrrepsDropout` does). ``p = 1`` drops everything;
     a dropped element is 0 whatever it held."""
     if _recorded():
         return torch.ops.flashcart.irreps_dropout(x, rng, float(p), int(l_max))
